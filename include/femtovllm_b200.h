@@ -280,6 +280,99 @@ FVB_API int fvb_paged_attention_prefill(const void* q, void* out, const void* k_
                                 const int32_t* positions, int dtype, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/*
+ * Paged attention with a sliding window and sinks.  No counterpart in the reference.
+ * As fvb_paged_attention_decode_strided / _prefill_strided, with the key range of every query cut down to
+ * the last `window` keys and the first `num_sinks`: a query at position p (decode: kv_len - 1) sees key j
+ * iff j < kv_len, j <= p, and p - j < window or j < num_sinks.  window >= 1, num_sinks >= 0.  A query whose
+ * mask leaves nothing (its window lies past kv_len and there are no sinks) gives zeros.
+ * Table entries of pages that hold no visible key of any of the sequence's queries are not read and may be
+ * -1 (pages the engine has taken back); keys of such pages, and keys between sinks and window in the pages
+ * that are read, may hold anything, NaN included.  Prefill: the positions of a sequence's tokens must not
+ * descend.  max_kv_len at most fvb_max_kv_len(), at most 65535 sequences.
+ * Workspace: decode fvb_paged_attention_window_decode_workspace_size bytes, prefill
+ * fvb_paged_attention_prefill_workspace_size bytes; 256-byte aligned.
+ */
+FVB_API size_t fvb_paged_attention_window_decode_workspace_size(int num_seqs, int n_heads, int n_kv_heads,
+                                                                int head_dim, int max_kv_len, int window,
+                                                                int num_sinks);
+FVB_API int fvb_paged_attention_window_decode(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                                              int64_t out_token_stride, int64_t out_head_stride, const void* k_pool,
+                                              const void* v_pool, int64_t num_blocks, int n_heads, int n_kv_heads,
+                                              int head_dim, int block_size, int num_seqs, const int32_t* block_tables,
+                                              int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len,
+                                              int window, int num_sinks, int dtype, void* workspace,
+                                              size_t workspace_bytes, void* stream);
+FVB_API int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                                               int64_t out_token_stride, int64_t out_head_stride, const void* k_pool,
+                                               const void* v_pool, int64_t num_blocks, int n_heads, int n_kv_heads,
+                                               int head_dim, int block_size, int num_seqs, int64_t q_len_flatten,
+                                               const int32_t* cu_seqlens, int max_q_len, const int32_t* block_tables,
+                                               int max_blocks_per_seq, const int32_t* kv_lens,
+                                               const int32_t* positions, int window, int num_sinks, int dtype,
+                                               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Decode paged attention for a batch whose sequences share prefixes by groups: the result of
+ * fvb_paged_attention_decode_strided on the same tables, with each group's prefix read once for all its
+ * sequences (tensor cores for 16-bit types).  No counterpart in the reference, whose prefix cache shares
+ * the pages but whose decode kernel reads them once per sequence and query head.
+ * Group g is sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int32, num_groups + 1 ascending entries within
+ * [0, num_seqs]; sequences outside every group share nothing).  The caller says that the table rows of a
+ * group agree in their first prefix_lens[g] / 16 pages; those pages are read through the row of the group's
+ * first sequence, whatever its kv_len.  prefix_lens[g] need not be a multiple of 16 nor below every
+ * kv_len of the group; max_prefix_len bounds it (keys past it are read per sequence).
+ * Malformed groups are recorded in the device error word and never read out of bounds.
+ * max_kv_len at most fvb_max_kv_len(); workspace 256-byte aligned.
+ */
+FVB_API size_t fvb_paged_attention_shared_prefix_workspace_size(int num_seqs, int n_heads, int n_kv_heads,
+                                                                int head_dim, int num_groups, int max_prefix_len,
+                                                                int dtype);
+FVB_API int fvb_paged_attention_shared_prefix_decode(
+    const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
+    int64_t out_head_stride, const void* k_pool, const void* v_pool, int64_t num_blocks, int n_heads, int n_kv_heads,
+    int head_dim, int block_size, int num_seqs, const int32_t* block_tables, int max_blocks_per_seq,
+    const int32_t* kv_lens, int max_kv_len, const int32_t* cu_groups, int num_groups, const int32_t* prefix_lens,
+    int max_prefix_len, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Beam search, selection: for every request the num_select best continuations of its num_beams beams.  No
+ * counterpart in the reference (one continuation per request).  Row r = request * num_beams + w:
+ *   score(w, i) = scores[r] + logits[r * row_stride + i] - log sum_j exp(logits[r * row_stride + j])
+ * tokens / parents / out_scores [num_requests][num_select], best first, ties to the lowest w * vocab + i.  A
+ * score that is not a number (a NaN or +inf logit, a row of -inf) counts as -inf; -inf candidates are chosen
+ * last, in the same order.  finished (one byte per row, may be NULL): a beam with a nonzero entry has the
+ * single continuation eos_token_id at scores[r], and its logits are not read.
+ * num_beams and num_select 1 to 64, num_select <= num_beams * vocab, vocab < 2^31, rows at any element
+ * alignment.  Sums in fp32, the order of the beams' candidates decided in fp64.
+ * workspace: fvb_beam_search_workspace_size bytes, 256-byte aligned, no initial value.  Two launches.
+ */
+FVB_API size_t fvb_beam_search_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select,
+                                              int dtype);
+FVB_API int fvb_beam_search_select(const void* logits, int64_t row_stride, int num_requests, int num_beams,
+                                   int64_t vocab, int dtype, const float* scores, const uint8_t* finished,
+                                   int64_t eos_token_id, int num_select, int64_t* tokens, int64_t* parents,
+                                   float* out_scores, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Beam search, reordering of the paged KV cache: row r of every request becomes the continuation of its row
+ * parents[r] (int64, [num_requests][num_beams], entries in [0, num_beams)).  No counterpart in the reference.
+ * All rows of a request hold kv_lens[r] tokens, the same number.  Their full pages may be shared between
+ * rows; the open pages (table columns from kv_len / block_size on) of every row must be its own.
+ * new_block_tables[r] (must not overlap block_tables) takes the parent's full pages by reference; the
+ * parent's first child also takes its open pages, every further child those of a row without a child, into
+ * which the kv_len % block_size newest tokens are copied in all num_layers pools (host arrays of device
+ * pointers, one K and one V pool per layer, layout as fvb_store_kvcache's).  No page is allocated or
+ * freed; the other slots of the pages are left as they were.  A request with a bad parent, differing kv_lens
+ * or a kv_len past its table row keeps its rows (FVB_ERR_INVALID_ARGUMENT in the device error word).
+ * num_beams 1 to 64; head_dim * element size a multiple of 16 bytes.
+ */
+FVB_API int fvb_beam_reorder_kvcache(const void* const* k_pools, const void* const* v_pools, int num_layers,
+                                     int64_t num_blocks, int n_kv_heads, int head_dim, int block_size, int dtype,
+                                     const int32_t* block_tables, int32_t* new_block_tables, int max_blocks_per_seq,
+                                     const int32_t* kv_lens, const int64_t* parents, int num_requests, int num_beams,
+                                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -67,6 +67,9 @@ int esize_of(int dtype) {
   }
 }
 
+// Largest y and z extent of a grid.
+constexpr int kMaxGridYZ = 65535;
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int cuda_status(cudaError_t e) {
@@ -496,6 +499,207 @@ int fvb_paged_attention_prefill_strided(const void* q, int64_t q_token_stride, i
   return cuda_status(launch_prefill(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, num_seqs,
                                     q_len_flatten, cu_seqlens, max_q_len, block_tables, max_blocks_per_seq, kv_lens,
                                     positions, dtype, plan, lay, workspace, err, static_cast<cudaStream_t>(stream)));
+}
+
+size_t fvb_paged_attention_window_decode_workspace_size(int num_seqs, int n_heads, int n_kv_heads, int head_dim,
+                                                        int max_kv_len, int window, int num_sinks) {
+  if (num_seqs <= 0 || !gqa_ok(n_heads, n_kv_heads) || max_kv_len < 0 || window < 1 || num_sinks < 0) return 0;
+  const int sms = device_sm_count();
+  const size_t split_ws =
+      plan_window_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms).ws_bytes;
+  if (!decode_on_tensor_cores(n_heads, n_kv_heads, FVB_DTYPE_BF16)) return split_ws;
+  const size_t tc_ws =
+      plan_window_tc_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms).ws_bytes;
+  return split_ws > tc_ws ? split_ws : tc_ws;  // fp32, 16-bit
+}
+
+int fvb_paged_attention_window_decode(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                                      int64_t out_token_stride, int64_t out_head_stride, const void* k_pool,
+                                      const void* v_pool, int64_t num_blocks, int n_heads, int n_kv_heads,
+                                      int head_dim, int block_size, int num_seqs, const int32_t* block_tables,
+                                      int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len, int window,
+                                      int num_sinks, int dtype, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+  TraceRange trace("fvb_paged_attention_window_decode");
+  int st = check_attention(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, block_size, num_seqs,
+                           block_tables, max_blocks_per_seq, kv_lens, dtype);
+  if (st) return st;
+  const QOLayout lay{q_token_stride, q_head_stride, out_token_stride, out_head_stride};
+  st = check_layout(lay, dtype);
+  if (st) return st;
+  if (window < 1 || num_sinks < 0) return FVB_ERR_INVALID_ARGUMENT;
+  if (num_seqs == 0) return FVB_OK;
+  if (max_kv_len < 0 || max_kv_len > fvb_max_kv_len() ||
+      int64_t(max_kv_len) > int64_t(max_blocks_per_seq) * kPageSize)
+    return FVB_ERR_INVALID_ARGUMENT;
+  if (num_seqs > kMaxGridYZ || int64_t(n_heads) > kMaxGridYZ) return FVB_ERR_UNSUPPORTED;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;
+  const int sms = device_sm_count();
+  const bool tc = decode_on_tensor_cores(n_heads, n_kv_heads, dtype);
+  DecodePlan plan{};
+  TcDecodePlan tp{};
+  if (tc) tp = plan_window_tc_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms);
+  else plan = plan_window_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms);
+  const size_t need = tc ? tp.ws_bytes : plan.ws_bytes;
+  if (need > 0 && (!workspace || workspace_bytes < need)) return FVB_ERR_WORKSPACE_TOO_SMALL;
+  cudaError_t e;
+  int* err = device_error_ptr(&e);
+  if (!err) return cuda_status(e);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (tc)
+    return cuda_status(launch_window_tc_decode(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim,
+                                               num_seqs, block_tables, max_blocks_per_seq, kv_lens, max_kv_len,
+                                               window, num_sinks, dtype, tp, lay, workspace, err, s));
+  return cuda_status(launch_window_decode(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, num_seqs,
+                                          block_tables, max_blocks_per_seq, kv_lens, max_kv_len, window, num_sinks,
+                                          dtype, plan, lay, workspace, err, s));
+}
+
+int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
+                                       int64_t out_token_stride, int64_t out_head_stride, const void* k_pool,
+                                       const void* v_pool, int64_t num_blocks, int n_heads, int n_kv_heads,
+                                       int head_dim, int block_size, int num_seqs, int64_t q_len_flatten,
+                                       const int32_t* cu_seqlens, int max_q_len, const int32_t* block_tables,
+                                       int max_blocks_per_seq, const int32_t* kv_lens, const int32_t* positions,
+                                       int window, int num_sinks, int dtype, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  TraceRange trace("fvb_paged_attention_window_prefill");
+  int st = check_attention(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, block_size, num_seqs,
+                           block_tables, max_blocks_per_seq, kv_lens, dtype);
+  if (st) return st;
+  const QOLayout lay{q_token_stride, q_head_stride, out_token_stride, out_head_stride};
+  st = check_layout(lay, dtype);
+  if (st) return st;
+  if (q_len_flatten < 0 || max_q_len < 0 || window < 1 || num_sinks < 0) return FVB_ERR_INVALID_ARGUMENT;
+  if (num_seqs == 0 || q_len_flatten == 0) return FVB_OK;
+  if (!cu_seqlens || !positions) return FVB_ERR_INVALID_ARGUMENT;
+  if (q_len_flatten > int64_t(0x7fffffff) || int64_t(max_blocks_per_seq) * kPageSize > fvb_max_kv_len())
+    return FVB_ERR_UNSUPPORTED;
+  cudaError_t e;
+  int* err = device_error_ptr(&e);
+  if (!err) return cuda_status(e);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == FVB_DTYPE_F32)
+    return cuda_status(launch_window_prefill_simt(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim,
+                                                  num_seqs, q_len_flatten, cu_seqlens, block_tables,
+                                                  max_blocks_per_seq, kv_lens, positions, window, num_sinks, lay, err,
+                                                  s));
+  const PrefillPlan plan = plan_prefill(num_seqs, n_heads, n_kv_heads, head_dim, q_len_flatten, max_q_len, dtype);
+  if (!workspace || workspace_bytes < plan.ws_bytes) return FVB_ERR_WORKSPACE_TOO_SMALL;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;
+  return cuda_status(launch_window_prefill(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim,
+                                           num_seqs, q_len_flatten, cu_seqlens, block_tables, max_blocks_per_seq,
+                                           kv_lens, positions, window, num_sinks, dtype, plan, lay, workspace, err,
+                                           s));
+}
+
+size_t fvb_paged_attention_shared_prefix_workspace_size(int num_seqs, int n_heads, int n_kv_heads, int head_dim,
+                                                        int num_groups, int max_prefix_len, int dtype) {
+  if (num_seqs <= 0 || num_groups < 0 || !gqa_ok(n_heads, n_kv_heads) || esize_of(dtype) == 0) return 0;
+  return plan_shared_prefix(num_seqs, n_heads, n_kv_heads, head_dim, num_groups, max_prefix_len, dtype,
+                            device_sm_count())
+      .ws_bytes;
+}
+
+int fvb_paged_attention_shared_prefix_decode(
+    const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
+    int64_t out_head_stride, const void* k_pool, const void* v_pool, int64_t num_blocks, int n_heads, int n_kv_heads,
+    int head_dim, int block_size, int num_seqs, const int32_t* block_tables, int max_blocks_per_seq,
+    const int32_t* kv_lens, int max_kv_len, const int32_t* cu_groups, int num_groups, const int32_t* prefix_lens,
+    int max_prefix_len, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  TraceRange trace("fvb_paged_attention_shared_prefix_decode");
+  int st = check_attention(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, block_size, num_seqs,
+                           block_tables, max_blocks_per_seq, kv_lens, dtype);
+  if (st) return st;
+  const QOLayout lay{q_token_stride, q_head_stride, out_token_stride, out_head_stride};
+  st = check_layout(lay, dtype);
+  if (st) return st;
+  if (num_groups < 0 || max_prefix_len < 0 || (num_groups > 0 && (!cu_groups || !prefix_lens)))
+    return FVB_ERR_INVALID_ARGUMENT;
+  if (num_seqs == 0) return FVB_OK;
+  if (max_kv_len < 0 || max_kv_len > fvb_max_kv_len() ||
+      int64_t(max_kv_len) > int64_t(max_blocks_per_seq) * kPageSize)
+    return FVB_ERR_INVALID_ARGUMENT;
+  if (num_groups > kMaxGridYZ || int64_t(n_heads) > kMaxGridYZ) return FVB_ERR_UNSUPPORTED;
+  const SharedPrefixPlan plan = plan_shared_prefix(num_seqs, n_heads, n_kv_heads, head_dim, num_groups,
+                                                   max_prefix_len, dtype, device_sm_count());
+  if (!workspace || workspace_bytes < plan.ws_bytes) return FVB_ERR_WORKSPACE_TOO_SMALL;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;
+  cudaError_t e;
+  int* err = device_error_ptr(&e);
+  if (!err) return cuda_status(e);
+  return cuda_status(launch_shared_prefix(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, num_seqs,
+                                          block_tables, max_blocks_per_seq, kv_lens, max_kv_len, cu_groups,
+                                          num_groups, prefix_lens, max_prefix_len, dtype, plan, lay, workspace, err,
+                                          static_cast<cudaStream_t>(stream)));
+}
+
+size_t fvb_beam_search_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select, int dtype) {
+  if (num_requests <= 0 || num_beams <= 0 || vocab <= 0 || num_select <= 0 || esize_of(dtype) == 0) return 0;
+  return beam_workspace_size(num_requests, num_beams, vocab, num_select, esize_of(dtype));
+}
+
+int fvb_beam_search_select(const void* logits, int64_t row_stride, int num_requests, int num_beams, int64_t vocab,
+                           int dtype, const float* scores, const uint8_t* finished, int64_t eos_token_id,
+                           int num_select, int64_t* tokens, int64_t* parents, float* out_scores, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  TraceRange trace("fvb_beam_search_select");
+  const int es = esize_of(dtype);
+  if (es == 0) return FVB_ERR_UNSUPPORTED;
+  if (num_requests < 0 || num_beams < 1 || num_select < 1 || vocab < 1 || row_stride < vocab)
+    return FVB_ERR_INVALID_ARGUMENT;
+  if (num_beams > kMaxBeams || num_select > kMaxBeams || vocab >= (int64_t(1) << 31)) return FVB_ERR_UNSUPPORTED;
+  if (num_select > num_beams * vocab) return FVB_ERR_INVALID_ARGUMENT;
+  if (finished && (eos_token_id < 0 || eos_token_id >= vocab)) return FVB_ERR_INVALID_ARGUMENT;
+  if (num_requests == 0) return FVB_OK;
+  if (!logits || !scores || !tokens || !parents || !out_scores) return FVB_ERR_INVALID_ARGUMENT;
+  // One CTA per part of a row, parts of 2048 columns at least.
+  if (int64_t(num_requests) * num_beams * (vocab / 2048 + 1) >= (int64_t(1) << 31)) return FVB_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < beam_workspace_size(num_requests, num_beams, vocab, num_select, es))
+    return FVB_ERR_WORKSPACE_TOO_SMALL;
+  if ((reinterpret_cast<uintptr_t>(logits) % es) != 0 || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||
+      (reinterpret_cast<uintptr_t>(scores) & 3) != 0 || (reinterpret_cast<uintptr_t>(tokens) & 7) != 0 ||
+      (reinterpret_cast<uintptr_t>(parents) & 7) != 0 || (reinterpret_cast<uintptr_t>(out_scores) & 3) != 0)
+    return FVB_ERR_MISALIGNED;
+  return cuda_status(launch_beam_select(logits, row_stride, num_requests, num_beams, vocab, dtype, scores, finished,
+                                        eos_token_id, num_select, tokens, parents, out_scores, workspace,
+                                        static_cast<cudaStream_t>(stream)));
+}
+
+int fvb_beam_reorder_kvcache(const void* const* k_pools, const void* const* v_pools, int num_layers,
+                             int64_t num_blocks, int n_kv_heads, int head_dim, int block_size, int dtype,
+                             const int32_t* block_tables, int32_t* new_block_tables, int max_blocks_per_seq,
+                             const int32_t* kv_lens, const int64_t* parents, int num_requests, int num_beams,
+                             void* stream) {
+  TraceRange trace("fvb_beam_reorder_kvcache");
+  const int es = esize_of(dtype);
+  if (es == 0) return FVB_ERR_UNSUPPORTED;
+  if (num_layers < 1 || num_blocks < 0 || n_kv_heads < 1 || head_dim < 1 || block_size < 1 || max_blocks_per_seq < 0 ||
+      num_requests < 0 || num_beams < 1 || !k_pools || !v_pools)
+    return FVB_ERR_INVALID_ARGUMENT;
+  if (num_beams > kMaxBeams) return FVB_ERR_UNSUPPORTED;
+  if ((int64_t(head_dim) * es) % 16 != 0) return FVB_ERR_MISALIGNED;
+  // rows in the grid, vectors of one page in an int
+  if (int64_t(num_requests) * num_beams >= (int64_t(1) << 31) ||
+      int64_t(n_kv_heads) * block_size >= (int64_t(1) << 31) / (int64_t(head_dim) * es))
+    return FVB_ERR_UNSUPPORTED;
+  if (num_requests == 0) return FVB_OK;
+  if (!kv_lens || !parents || (max_blocks_per_seq > 0 && (!block_tables || !new_block_tables)))
+    return FVB_ERR_INVALID_ARGUMENT;
+  const uintptr_t from = reinterpret_cast<uintptr_t>(block_tables), to = reinterpret_cast<uintptr_t>(new_block_tables);
+  const uintptr_t table_bytes = uintptr_t(num_requests) * num_beams * max_blocks_per_seq * 4;
+  if (from < to + table_bytes && to < from + table_bytes) return FVB_ERR_INVALID_ARGUMENT;
+  if ((reinterpret_cast<uintptr_t>(parents) & 7) != 0) return FVB_ERR_MISALIGNED;
+  for (int i = 0; i < num_layers; ++i) {
+    if (num_blocks > 0 && (!k_pools[i] || !v_pools[i])) return FVB_ERR_INVALID_ARGUMENT;
+    if (!aligned16(k_pools[i]) || !aligned16(v_pools[i])) return FVB_ERR_MISALIGNED;
+  }
+  cudaError_t e;
+  int* err = device_error_ptr(&e);
+  if (!err) return cuda_status(e);
+  return cuda_status(launch_beam_reorder(k_pools, v_pools, num_layers, num_blocks, n_kv_heads, head_dim, block_size,
+                                         es, block_tables, new_block_tables, max_blocks_per_seq, kv_lens, parents,
+                                         num_requests, num_beams, err, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include "femtovllm_b200.h"
+#include "kernels.h"
 
 namespace fvb {
 
@@ -30,6 +31,39 @@ __device__ __forceinline__ void record_error(int* err, int code, int info) {
   if (atomicCAS(err, 0, code) == 0) atomicExch(err + 1, info);
 }
 
+// ---------------------------------------------------------------------------
+// Key ranges
+// ---------------------------------------------------------------------------
+
+// The units (pages or tiles of `unit` keys) that hold a key visible through a window with
+// sinks: units [0, head) and [head + gap, head + gap + count - head).  Queries at positions
+// first .. kv_len - 1 see key j iff j <= position and (position - j < window or j < sinks);
+// lo is the first key of the earliest query's window.  A query at or past kv_len may have its
+// whole window behind the last key: then only the sinks are left.
+struct KeySpan {
+  int head, gap, count, lo;
+};
+__host__ __device__ __forceinline__ KeySpan window_span(int first_end, int kv_len, int window, int sinks, int unit) {
+  KeySpan s;
+  s.lo = first_end > window ? first_end - window : 0;  // first_end: earliest query position + 1
+  const int n = (kv_len + unit - 1) / unit;
+  s.head = ((sinks < kv_len ? sinks : kv_len) + unit - 1) / unit;
+  const int near = s.lo < kv_len ? s.lo / unit : n;
+  const int begin = near > s.head ? near : s.head;
+  s.gap = begin - s.head;
+  s.count = s.head + (n - begin);
+  return s;
+}
+
+// Sequences of group g, inside [0, num_seqs) whatever cu_groups holds.
+__device__ __forceinline__ int2 group_rows(const DecodeExtra& ex, int g, int num_seqs) {
+  const int lo = min(max(__ldg(ex.cu_groups + g), 0), num_seqs);
+  return make_int2(lo, min(max(__ldg(ex.cu_groups + g + 1), lo), num_seqs));
+}
+// Keys of group g's shared prefix, in whole pages; a sequence alone in its group shares nothing.
+__device__ __forceinline__ int group_prefix(const DecodeExtra& ex, int g, int2 rows) {
+  return rows.y - rows.x < 2 ? 0 : min(max(__ldg(ex.prefix_lens + g), 0), ex.prefix_cap) / kPageSize * kPageSize;
+}
 // ---------------------------------------------------------------------------
 // Element types
 // ---------------------------------------------------------------------------

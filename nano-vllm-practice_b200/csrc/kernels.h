@@ -72,6 +72,19 @@ struct DecodePlan {
 };
 DecodePlan plan_decode(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int max_kv_len, int num_sms);
 
+// What the window and shared-prefix forms of the decode and combine kernels take besides the
+// plain form's arguments.
+struct DecodeExtra {
+  int window = 0, sinks = 0;  // keys behind the query that stay visible (itself included), first keys that do
+  int unit = 0;               // combine: keys a split counts in (a page, or a 128-key tile)
+  const int32_t* cu_groups = nullptr;    // shared prefix: sequences cu_groups[g] .. cu_groups[g + 1] - 1 ...
+  const int32_t* prefix_lens = nullptr;  // ... share the pages of their first prefix_lens[g] keys
+  int num_groups = 0;
+  int prefix_cap = 0;  // longest prefix that is shared; what is longer counts as the sequences' own
+  int slots = 0;       // prefix partials of a row (sequence, head)
+  const int4* items = nullptr;  // the rest: {sequence (-1: none), first page, pages, -} of each CTA
+};
+
 cudaError_t launch_decode(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
                           int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
                           int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len, int dtype,
@@ -138,6 +151,70 @@ cudaError_t launch_prefill_simt(const void* q, void* out, const void* k_pool, co
                                 const int32_t* kv_lens, const int32_t* positions, int dtype, const QOLayout& lay,
                                 int* err, cudaStream_t stream);
 
+// Sliding window with sinks (decode_window.cu, prefill_window.cu): a query at position p
+// sees key j iff the plain form does and p - j < window or j < sinks.  Pages without a
+// visible key are not read.
+// Units (pages, tiles) of `unit` keys one query's visible keys touch at most.
+int window_max_units(int max_kv_len, int window, int sinks, int unit);
+DecodePlan plan_window_decode(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int max_kv_len, int window,
+                              int sinks, int num_sms);
+cudaError_t launch_window_decode(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
+                                 int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
+                                 int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len, int window, int sinks,
+                                 int dtype, const DecodePlan& plan, const QOLayout& lay, void* workspace, int* err,
+                                 cudaStream_t stream, const int32_t* q_index = nullptr,
+                                 const int32_t* q_pos = nullptr);
+cudaError_t launch_window_combine(const float* ws_o, const float* ws_lse, void* out, const int32_t* kv_lens,
+                                  int kv_cap, int num_seqs, int n_heads, int head_dim, int window, int sinks, int unit,
+                                  int units_per_split, int max_splits, int dtype, const QOLayout& lay,
+                                  cudaStream_t stream);
+TcDecodePlan plan_window_tc_decode(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int max_kv_len, int window,
+                                   int sinks, int num_sms);
+cudaError_t launch_window_tc_decode(const void* q, void* out, const void* k_pool, const void* v_pool,
+                                    int64_t num_blocks, int n_heads, int n_kv_heads, int head_dim, int num_seqs,
+                                    const int32_t* block_tables, int max_blocks_per_seq, const int32_t* kv_lens,
+                                    int max_kv_len, int window, int sinks, int dtype, const TcDecodePlan& plan,
+                                    const QOLayout& lay, void* workspace, int* err, cudaStream_t stream);
+cudaError_t launch_window_prefill(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
+                                  int n_heads, int n_kv_heads, int head_dim, int num_seqs, int64_t q_len_flatten,
+                                  const int32_t* cu_seqlens, const int32_t* block_tables, int max_blocks_per_seq,
+                                  const int32_t* kv_lens, const int32_t* positions, int window, int sinks, int dtype,
+                                  const PrefillPlan& plan, const QOLayout& lay, void* workspace, int* err,
+                                  cudaStream_t stream);
+// fp32 (prefill_simt.cu).
+cudaError_t launch_window_prefill_simt(const void* q, void* out, const void* k_pool, const void* v_pool,
+                                       int64_t num_blocks, int n_heads, int n_kv_heads, int head_dim, int num_seqs,
+                                       int64_t q_len_flatten, const int32_t* cu_seqlens, const int32_t* block_tables,
+                                       int max_blocks_per_seq, const int32_t* kv_lens, const int32_t* positions,
+                                       int window, int sinks, const QOLayout& lay, int* err, cudaStream_t stream);
+
+// Decode of sequences that share prefixes by groups (shared_prefix.cu): every group's prefix
+// is attended once for all its sequences (on the tensor cores for 16-bit types,
+// shared_prefix_tc.cu), every sequence's own keys by the split-KV kernel, and the partials
+// of both are merged.
+struct SharedPrefixPlan {
+  int keys_per_split;  // of a prefix; 0 = no prefix to share
+  int prefix_splits;   // prefix partials per (sequence, head)
+  bool single_tiles;   // tensor cores: items of one query tile (small groups) instead of two
+  int target_items;    // page ranges the sequences' own keys are cut into, at most + num_seqs
+  int max_items;
+  size_t off_spans, off_po, off_pl, off_ro, off_rl;  // items at 0, spans, prefix and rest partials
+  size_t ws_bytes;
+};
+SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int num_groups,
+                                    int max_prefix_len, int dtype, int num_sms);
+cudaError_t launch_shared_prefix(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
+                                 int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
+                                 int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len,
+                                 const int32_t* cu_groups, int num_groups, const int32_t* prefix_lens,
+                                 int max_prefix_len, int dtype, const SharedPrefixPlan& plan, const QOLayout& lay,
+                                 void* workspace, int* err, cudaStream_t stream);
+cudaError_t launch_prefix_tc(const void* q, const void* k_pool, const void* v_pool, int64_t num_blocks, int n_heads,
+                             int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
+                             int max_blocks_per_seq, const int32_t* kv_lens, int dtype, const SharedPrefixPlan& plan,
+                             const QOLayout& lay, float* ws_o, float* ws_lse, const DecodeExtra& ex, int* err,
+                             cudaStream_t stream);
+
 // Fused q/k RMSNorm + rotary embedding + K/V pool write (qk_norm_rope.cu).
 // Strides are in elements; q_out is [n_heads][num_tokens][head_dim].
 cudaError_t launch_qk_norm_rope_store(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts,
@@ -162,6 +239,21 @@ cudaError_t launch_sample(const void* logits, int64_t row_stride, int num_rows, 
                           const float* temps, const float* pens, const int64_t* table, int64_t table_stride,
                           int64_t table_len, unsigned long long* rng, int64_t* out, void* workspace,
                           cudaStream_t stream);
+
+// Beam search (beam_search.cu, beam_reorder.cu).  At most kMaxBeams beams a request and
+// kMaxBeams selected continuations.
+constexpr int kMaxBeams = 64;
+size_t beam_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select, int esize);
+cudaError_t launch_beam_select(const void* logits, int64_t row_stride, int num_requests, int num_beams, int64_t vocab,
+                               int dtype, const float* scores, const uint8_t* finished, int64_t eos, int num_select,
+                               int64_t* tokens, int64_t* parents, float* out_scores, void* workspace,
+                               cudaStream_t stream);
+// k_pools / v_pools: host arrays of num_layers device pointers.
+cudaError_t launch_beam_reorder(const void* const* k_pools, const void* const* v_pools, int num_layers,
+                                int64_t num_blocks, int n_kv_heads, int head_dim, int block_size, int esize,
+                                const int32_t* block_tables, int32_t* new_tables, int max_blocks_per_seq,
+                                const int32_t* kv_lens, const int64_t* parents, int num_requests, int num_beams,
+                                int* err, cudaStream_t stream);
 
 int device_sm_count();
 

@@ -1,0 +1,421 @@
+// Decode paged attention for a batch whose sequences share long prefixes by groups.
+//
+// The reference's prefix cache lets requests share the pages of a common prompt, and its
+// decode kernel reads those pages once per request and query head
+// (csrc/paged_attention/paged_attention_gemv.cu:16-221).  softmax(q K^T) V splits over the
+// keys: with (o_i, lse_i) of disjoint key ranges i, o = sum_i 2^(lse_i - m) o_i / sum_i
+// 2^(lse_i - m), m = max lse_i.  Here the prefix of a group is one range (or a few) that
+// all its sequences attend together, so its K and V leave HBM once per group and feed
+// 128-row tensor-core tiles of (sequence, query head) rows; the keys behind it are
+// attended per sequence by the split-KV kernel, bound by HBM.  Four launches:
+//
+//   plan     one CTA: cuts the sequences' own pages into about target_items ranges of equal
+//            length, whatever their lengths are (a grid of max_splits x sequences would be
+//            mostly empty CTAs here, since the longest context bounds what every sequence
+//            may hold behind its prefix);
+//   prefix   prefill_tc.cuh (kTcPrefix), fp32: decode_split.cuh (kDecodePrefix); it reads
+//            nothing of the plan and starts beside it (programmatic dependent launch);
+//   rest     decode_split.cuh (kDecodeRest), one CTA per (range, kv head): starts as soon as
+//            the prefix's CTAs are placed and fills the SMs they leave;
+//   merge    one or four warps per (sequence, query head).
+#include "decode_split.cuh"
+
+namespace fvb {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kMinRangePages = 4;
+
+// Sum over the CTA of v (every thread gets it) and the exclusive prefix of the thread's v.
+__device__ __forceinline__ int2 block_scan(int v, int* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  if (lane == 31) sh[warp] = upto;
+  __syncthreads();
+  int w = sh[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  const int total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = warp > 0 ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
+  __syncthreads();
+  return make_int2(total, before + upto - v);
+}
+
+// items[i] = {sequence, first page, pages, 0} ({-1, ..} behind the last one) and
+// spans[b] = {prefix partials, first item, items, 0} of sequence b.
+__global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int32_t* __restrict__ kv_lens, int kv_cap,
+                                                                   int num_seqs, int keys_per_split, int target_items,
+                                                                   int max_items, const DecodeExtra ex,
+                                                                   int4* __restrict__ items, int4* __restrict__ spans,
+                                                                   int* __restrict__ err) {
+  __shared__ int sh[32];
+  launch_dependents();
+  // {pages of sequence b's own keys, keys of its shared prefix}
+  auto own_pages = [&](int b) {
+    int kv = __ldg(kv_lens + b);
+    if (kv > kv_cap) record_error(err, FVB_ERR_INVALID_ARGUMENT, b);
+    kv = min(max(kv, 0), kv_cap);
+    int lo = 0, hi = ex.num_groups;  // first group whose end lies behind b
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(ex.cu_groups + mid + 1) > b) hi = mid; else lo = mid + 1;
+    }
+    int prefix = 0;
+    if (keys_per_split > 0 && lo < ex.num_groups) {
+      const int2 rows = group_rows(ex, lo, num_seqs);
+      if (b >= rows.x) prefix = group_prefix(ex, lo, rows);
+    }
+    return make_int2(max((kv + kPageSize - 1) / kPageSize - prefix / kPageSize, 0), prefix);
+  };
+  for (int g = threadIdx.x; g < ex.num_groups; g += kPlanThreads) {
+    const int lo = __ldg(ex.cu_groups + g), hi = __ldg(ex.cu_groups + g + 1);
+    if (lo < 0 || hi < lo || hi > num_seqs || __ldg(ex.prefix_lens + g) < 0)
+      record_error(err, FVB_ERR_INVALID_ARGUMENT, g);
+  }
+  int2 mine = make_int2(0, 0);
+  int sum = 0;
+  for (int b = threadIdx.x; b < num_seqs; b += kPlanThreads) {
+    mine = own_pages(b);
+    sum += mine.x;
+  }
+  const int total = block_scan(sum, sh).x;
+  // Whole stages of two pages; sum over b of ceil(pages_b / per) <= target_items + num_seqs.
+  int per = max(kMinRangePages, (total + target_items - 1) / target_items);
+  per += per & 1;
+  int done = 0;
+  for (int base = 0; base < num_seqs; base += kPlanThreads) {
+    const int b = base + threadIdx.x;
+    if (b < num_seqs && num_seqs > kPlanThreads) mine = own_pages(b);
+    const int n = b < num_seqs ? (mine.x + per - 1) / per : 0;
+    const int2 at = block_scan(n, sh);
+    const int first = done + at.y;
+    if (b < num_seqs) {
+      const int skip = mine.y / kPageSize;
+      for (int i = 0; i < n && first + i < max_items; ++i)
+        items[first + i] = make_int4(b, skip + i * per, min(per, mine.x - i * per), 0);
+      spans[b] = make_int4(keys_per_split > 0 ? (mine.y + keys_per_split - 1) / keys_per_split : 0, first, n, 0);
+    }
+    done += at.x;
+  }
+  for (int i = done + threadIdx.x; i < max_items; i += kPlanThreads) items[i] = make_int4(-1, 0, 0, 0);
+}
+
+// out[h][b] from the partials of its prefix and of its own keys; WARPS warps per row, whose
+// lanes hold D / 32 dims each and take every WARPS-th partial, kInFlight at a time.
+constexpr int kMergeThreads = 128;
+constexpr int kInFlight = 4;
+
+template <typename T, int D, int WARPS>
+__global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const float* __restrict__ po,
+                                                                     const float* __restrict__ pl,
+                                                                     const float* __restrict__ ro,
+                                                                     const float* __restrict__ rl,
+                                                                     const int4* __restrict__ spans,
+                                                                     T* __restrict__ out, int num_seqs, int n_heads,
+                                                                     int prefix_slots, const QOLayout lay) {
+  constexpr int kDims = D / 32;
+  constexpr int kRows = kMergeThreads / 32 / WARPS;
+  __shared__ float sh_acc[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
+  __shared__ float sh_m[WARPS], sh_l[WARPS];
+  grid_dependency_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = int64_t(blockIdx.x) * kRows + (WARPS > 1 ? 0 : warp);  // (sequence, head), head fastest
+  if (row >= int64_t(num_seqs) * n_heads) return;
+  const int b = int(row / n_heads), head = int(row % n_heads);
+  const int4 span = __ldcg(spans + b);
+  const int n = span.x + span.z, w = WARPS > 1 ? warp : 0;
+  float m = -INFINITY, l = 0.f, acc[kDims];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) acc[d] = 0.f;
+  for (int i0 = w; i0 < n; i0 += WARPS * kInFlight) {
+    float o[kInFlight][kDims], ls[kInFlight];
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      const int i = i0 + u * WARPS;
+      const bool prefix = i < span.x;
+      const int64_t at = prefix ? row * prefix_slots + i : int64_t(span.y + i - span.x) * n_heads + head;
+      ls[u] = i < n ? __ldcg((prefix ? pl : rl) + at) : -INFINITY;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) o[u][d] = 0.f;
+      if (i < n) {
+        const float* src = (prefix ? po : ro) + at * D + lane * kDims;
+        if constexpr (kDims == 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          o[u][0] = v.x, o[u][1] = v.y, o[u][2] = v.z, o[u][3] = v.w;
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+          o[u][0] = v.x, o[u][1] = v.y;
+        }
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) mn = fmaxf(mn, ls[u]);
+    if (mn == -INFINITY) continue;  // no key seen so far
+    const float corr = fast_exp2(m - mn);
+    l *= corr;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) acc[d] *= corr;
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u) {
+      if (ls[u] == -INFINITY) continue;  // its O is not a number
+      const float wt = fast_exp2(ls[u] - mn);
+      l += wt;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) acc[d] = fmaf(wt, o[u][d], acc[d]);
+    }
+    m = mn;
+  }
+  if constexpr (WARPS > 1) {
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) sh_acc[warp][lane * kDims + d] = acc[d];
+    if (lane == 0) {
+      sh_m[warp] = m;
+      sh_l[warp] = l;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    float mx = m;
+#pragma unroll
+    for (int k = 1; k < WARPS; ++k) mx = fmaxf(mx, sh_m[k]);
+    const float ms = mx == -INFINITY ? 0.f : mx;
+    const float own = fast_exp2(m - ms);
+    l *= own;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) acc[d] *= own;
+#pragma unroll
+    for (int k = 1; k < WARPS; ++k) {
+      const float wt = fast_exp2(sh_m[k] - ms);
+      l = fmaf(sh_l[k], wt, l);
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) acc[d] = fmaf(wt, sh_acc[k][lane * kDims + d], acc[d]);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;  // an empty context gives zeros
+  T* dst = out + int64_t(b) * lay.o_ts + int64_t(head) * lay.o_hs + lane * kDims;
+  __align__(16) T v[kDims];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) v[d] = Elem<T>::from_f(acc[d] * inv);
+  if constexpr (sizeof(v) == 16) {
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+  } else if constexpr (sizeof(v) == 8) {
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(v);
+  }
+}
+
+struct SharedArgs {
+  const void *q, *k_pool, *v_pool;
+  void* out;
+  int64_t num_blocks;
+  int n_heads, n_kv_heads, num_seqs;
+  const int32_t* block_tables;
+  int max_blocks_per_seq;
+  const int32_t* kv_lens;
+  int kv_cap;
+  SharedPrefixPlan plan;
+  QOLayout lay;
+  float *po, *pl, *ro, *rl;
+  const int4* spans;
+  DecodeExtra ex;
+  int* err;
+  cudaStream_t stream;
+};
+
+cudaLaunchConfig_t config(dim3 grid, int threads, int smem, cudaStream_t stream, cudaLaunchAttribute* dependent) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  if (dependent) {
+    dependent->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    dependent->val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = dependent;
+    cfg.numAttrs = 1;
+  }
+  return cfg;
+}
+
+template <typename T, int D, int NREP, int MODE>
+cudaError_t launch_split(const SharedArgs& a, dim3 grid, int pages_per_split, int splits, float* ws_o, float* ws_lse,
+                         bool dependent) {
+  using Tr = DecodeTraits<T, D, NREP>;
+  const int group = a.n_heads / a.n_kv_heads, chunks = (group + NREP - 1) / NREP;
+  CUtensorMap kmap;
+  cudaError_t ce = make_k_map<T, D>(&kmap, a.k_pool, a.num_blocks, a.n_kv_heads);
+  if (ce == cudaSuccess) ce = set_smem_once<decode_split_kernel<T, D, NREP, MODE>>(Tr::kSmemBytes);
+  if (ce != cudaSuccess) return ce;
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg =
+      config(grid, kDecodeThreads, Tr::kSmemBytes, a.stream, dependent ? attr : nullptr);
+  return cudaLaunchKernelEx(&cfg, decode_split_kernel<T, D, NREP, MODE>, kmap, static_cast<const T*>(a.q),
+                            static_cast<T*>(a.out), static_cast<const uint8_t*>(a.v_pool), a.num_blocks, a.n_kv_heads,
+                            a.num_seqs, a.block_tables, a.max_blocks_per_seq, a.kv_lens, a.kv_cap, pages_per_split,
+                            splits, ws_o, ws_lse, a.lay, group, chunks, static_cast<const int32_t*>(nullptr),
+                            static_cast<const int32_t*>(nullptr), a.ex, a.err);
+}
+
+template <typename T, int D, int NREP>
+cudaError_t launch_rest(const SharedArgs& a) {
+  const int chunks = (a.n_heads / a.n_kv_heads + NREP - 1) / NREP;
+  // A dependent of the prefix kernel, which waits for the plan; without one an ordinary launch.
+  return launch_split<T, D, NREP, kDecodeRest>(a, dim3(a.plan.max_items, a.n_kv_heads * chunks), 0, 1, a.ro, a.rl,
+                                               a.plan.keys_per_split > 0);
+}
+
+template <typename T, int D, int WARPS>
+cudaError_t launch_merge(const SharedArgs& a) {
+  constexpr int kRows = kMergeThreads / 32 / WARPS;
+  const int64_t ctas = (int64_t(a.num_seqs) * a.n_heads + kRows - 1) / kRows;
+  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = config(dim3(unsigned(ctas)), kMergeThreads, 0, a.stream, attr);
+  return cudaLaunchKernelEx(&cfg, shared_merge_kernel<T, D, WARPS>, static_cast<const float*>(a.po),
+                            static_cast<const float*>(a.pl), static_cast<const float*>(a.ro),
+                            static_cast<const float*>(a.rl), a.spans, static_cast<T*>(a.out), a.num_seqs, a.n_heads,
+                            a.plan.prefix_splits, a.lay);
+}
+
+template <typename T, int D>
+cudaError_t run(const SharedArgs& a, int head_dim, int dtype) {
+  const int group = a.n_heads / a.n_kv_heads;
+  cudaError_t ce = cudaSuccess;
+  if (a.plan.keys_per_split > 0) {
+    if constexpr (sizeof(T) == 4) {
+      // Rows are (sequence, head) pairs of a group, eight a CTA.
+      const int64_t row_chunks = (int64_t(a.num_seqs) * group + 7) / 8;
+      if (row_chunks * a.plan.prefix_splits > 0x7fffffff) return cudaErrorInvalidValue;
+      ce = launch_split<T, D, 8, kDecodePrefix>(
+          a, dim3(unsigned(row_chunks * a.plan.prefix_splits), a.n_kv_heads, a.ex.num_groups),
+          a.plan.keys_per_split / kPageSize, a.plan.prefix_splits, a.po, a.pl, false);
+    } else {
+      ce = launch_prefix_tc(a.q, a.k_pool, a.v_pool, a.num_blocks, a.n_heads, a.n_kv_heads, head_dim, a.num_seqs,
+                            a.block_tables, a.max_blocks_per_seq, a.kv_lens, dtype, a.plan, a.lay, a.po, a.pl, a.ex,
+                            a.err, a.stream);
+    }
+    if (ce != cudaSuccess) return ce;
+  }
+  switch (decode_tile_heads(group)) {
+    case 1:
+      ce = launch_rest<T, D, 1>(a);
+      break;
+    case 2:
+      ce = launch_rest<T, D, 2>(a);
+      break;
+    case 4:
+      ce = launch_rest<T, D, 4>(a);
+      break;
+    default:
+      ce = launch_rest<T, D, 8>(a);
+  }
+  if (ce != cudaSuccess) return ce;
+  // Partials a row merges on average: prefix splits and its share of the ranges.
+  const int64_t partials = a.plan.prefix_splits + a.plan.max_items / a.num_seqs;
+  ce = partials > 8 ? launch_merge<T, D, 4>(a) : launch_merge<T, D, 1>(a);
+  return ce != cudaSuccess ? ce : cudaGetLastError();
+}
+
+}  // namespace
+
+SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int num_groups,
+                                    int max_prefix_len, int dtype, int num_sms) {
+  SharedPrefixPlan p{};
+  if (num_seqs <= 0 || n_kv_heads <= 0) return p;
+  const int group = n_heads / n_kv_heads;
+  const int prefix = std::max(0, max_prefix_len) / kPageSize * kPageSize;
+  if (prefix > 0 && num_groups > 0) {
+    // The prefix is split until its CTAs fill the SMs once; a group's rows are cut into
+    // tensor-core tiles (fp32: chunks of eight rows).  Groups of the average size that fit one
+    // query tile take items of one tile, whose two softmax groups share it.
+    const bool tc = dtype != FVB_DTYPE_F32;
+    const int unit = tc ? 128 : kPageSize * 4;
+    const int tile = tc ? 128 / tc_tile_heads(group) : 1;  // sequences of a query tile
+    const int average = (num_seqs + num_groups - 1) / num_groups;
+    p.single_tiles = tc && average <= tile;
+    const int64_t per_group = tc ? (average + tile * (p.single_tiles ? 1 : 2) - 1) / (tile * (p.single_tiles ? 1 : 2))
+                                 : (int64_t(average) * group + 7) / 8;
+    const int heads = tc ? n_kv_heads * ((group + tc_tile_heads(group) - 1) / tc_tile_heads(group)) : n_kv_heads;
+    const int64_t ctas = std::max<int64_t>(1, per_group * num_groups * heads);
+    const int units = (prefix + unit - 1) / unit;
+    const int64_t wanted = std::max<int64_t>(1, (tc ? num_sms : num_sms * 6) / ctas);
+    const int per = int((units + std::min<int64_t>(wanted, units) - 1) / std::min<int64_t>(wanted, units));
+    p.keys_per_split = per * unit;
+    p.prefix_splits = (prefix + p.keys_per_split - 1) / p.keys_per_split;
+  }
+  // About four waves of three resident split-KV CTAs per SM, as plan_decode.
+  const int tile_heads = decode_tile_heads(group);
+  const int units = n_kv_heads * ((group + tile_heads - 1) / tile_heads);
+  p.target_items = std::max(1, (num_sms * 12 + units - 1) / units);
+  p.max_items = p.target_items + num_seqs;
+  auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+  const size_t rows = size_t(num_seqs) * n_heads * p.prefix_splits;
+  const size_t rest = size_t(p.max_items) * n_heads;
+  p.off_spans = up(size_t(p.max_items) * 16);
+  p.off_po = p.off_spans + up(size_t(num_seqs) * 16);
+  p.off_pl = p.off_po + up(rows * head_dim * 4);
+  p.off_ro = p.off_pl + up(rows * 4);
+  p.off_rl = p.off_ro + up(rest * head_dim * 4);
+  p.ws_bytes = p.off_rl + up(rest * 4);
+  return p;
+}
+
+cudaError_t launch_shared_prefix(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
+                                 int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
+                                 int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len,
+                                 const int32_t* cu_groups, int num_groups, const int32_t* prefix_lens,
+                                 int max_prefix_len, int dtype, const SharedPrefixPlan& plan, const QOLayout& lay,
+                                 void* workspace, int* err, cudaStream_t stream) {
+  if (num_seqs == 0) return cudaSuccess;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  SharedArgs a{};
+  a.q = q;
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.out = out;
+  a.num_blocks = num_blocks;
+  a.n_heads = n_heads;
+  a.n_kv_heads = n_kv_heads;
+  a.num_seqs = num_seqs;
+  a.block_tables = block_tables;
+  a.max_blocks_per_seq = max_blocks_per_seq;
+  a.kv_lens = kv_lens;
+  a.kv_cap = int(std::min<int64_t>(max_kv_len, int64_t(max_blocks_per_seq) * kPageSize));
+  a.plan = plan;
+  a.lay = lay;
+  a.po = reinterpret_cast<float*>(ws + plan.off_po);
+  a.pl = reinterpret_cast<float*>(ws + plan.off_pl);
+  a.ro = reinterpret_cast<float*>(ws + plan.off_ro);
+  a.rl = reinterpret_cast<float*>(ws + plan.off_rl);
+  a.spans = reinterpret_cast<const int4*>(ws + plan.off_spans);
+  a.ex.cu_groups = cu_groups;
+  a.ex.prefix_lens = prefix_lens;
+  a.ex.num_groups = num_groups;
+  a.ex.prefix_cap = std::min(max_prefix_len, a.kv_cap);
+  a.ex.slots = plan.prefix_splits;
+  a.ex.items = reinterpret_cast<const int4*>(ws);
+  a.err = err;
+  a.stream = stream;
+  shared_plan_kernel<<<1, kPlanThreads, 0, stream>>>(kv_lens, a.kv_cap, num_seqs, plan.keys_per_split,
+                                                     plan.target_items, plan.max_items, a.ex,
+                                                     reinterpret_cast<int4*>(ws),
+                                                     reinterpret_cast<int4*>(ws + plan.off_spans), err);
+  cudaError_t ce = cudaGetLastError();
+  if (ce != cudaSuccess) return ce;
+  if (dtype == FVB_DTYPE_BF16)
+    return head_dim == 128 ? run<__nv_bfloat16, 128>(a, head_dim, dtype) : run<__nv_bfloat16, 64>(a, head_dim, dtype);
+  if (dtype == FVB_DTYPE_F16)
+    return head_dim == 128 ? run<__half, 128>(a, head_dim, dtype) : run<__half, 64>(a, head_dim, dtype);
+  return head_dim == 128 ? run<float, 128>(a, head_dim, dtype) : run<float, 64>(a, head_dim, dtype);
+}
+
+}  // namespace fvb

@@ -5,7 +5,8 @@
 // PagedAttentionGemmCuda) and the same attributes (kMaxKVLenNonSplit,
 // kKVLenPerPage, kDimHead), plus StoreKVCacheCuda for the slot-mapped KV write
 // the reference does in Python, QKNormRopeStoreCuda for the fused q/k norm +
-// rotary embedding + KV write and SampleTokensCuda for the sampler.  Each
+// rotary embedding + KV write, SampleTokensCuda for the sampler, the window and shared-prefix
+// forms of the attention and BeamSearchSelectCuda / BeamReorderKVCacheCuda for beam search.  Each
 // function validates like the reference's TORCH_CHECKs (csrc/paged_attention/paged_attention_gemv.cu:231-274,
 // paged_attention_gemm.cu:314-358), allocates the output (and the split-KV
 // workspace) with the caching allocator, and calls the C ABI on the current
@@ -310,6 +311,195 @@ torch::Tensor SampleTokensCuda(torch::Tensor logits, torch::Tensor temperatures,
   return out;
 }
 
+namespace {
+
+// One int32 table row and kv_len per sequence, on q's device.
+void check_tables(const at::Tensor& q, const at::Tensor& tables, const at::Tensor& kv_lens, int64_t num_seqs) {
+  TORCH_CHECK(tables.scalar_type() == torch::kInt32 && kv_lens.scalar_type() == torch::kInt32,
+              "kv_page_tables and kv_lens must be int32");
+  TORCH_CHECK(tables.get_device() == q.get_device() && kv_lens.get_device() == q.get_device(),
+              "kv_page_tables and kv_lens must be on q's device");
+  TORCH_CHECK(tables.dim() == 2 && tables.is_contiguous() && kv_lens.is_contiguous(),
+              "kv_page_tables must be (B, max_blocks), kv_page_tables and kv_lens contiguous");
+  TORCH_CHECK(tables.size(0) == num_seqs && kv_lens.numel() == num_seqs,
+              "one block table row and one kv_len per sequence");
+}
+
+int checked_int(int64_t x, const char* name) {
+  TORCH_CHECK(x >= 0 && x <= 0x7fffffff, name, " must be an int32 that is not negative, got ", x);
+  return int(x);
+}
+
+torch::Tensor new_workspace(size_t bytes, const at::Tensor& like) {
+  return torch::empty({int64_t(bytes > 0 ? bytes : 1)}, like.options().dtype(torch::kUInt8));
+}
+
+}  // namespace
+
+// Decode attention over the last `window` keys and the first `num_sinks` of every sequence.
+torch::Tensor PagedAttentionWindowGemvCuda(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool,
+                                           torch::Tensor kv_page_tables, torch::Tensor kv_lens, int64_t max_kv_len,
+                                           int64_t window, int64_t num_sinks, bool out_token_major) {
+  check_pools(q, k_pool, v_pool);
+  check_tables(q, kv_page_tables, kv_lens, q.size(1));
+  const int n_heads = int(q.size(0)), num_seqs = int(q.size(1)), head_dim = int(q.size(2));
+  const int kv = checked_int(max_kv_len, "max_kv_len"), win = checked_int(window, "window"),
+            sinks = checked_int(num_sinks, "num_sinks");
+  c10::cuda::CUDAGuard guard(q.device());
+  auto out = new_out(q, out_token_major);
+  const size_t ws_bytes = fvb_paged_attention_window_decode_workspace_size(num_seqs, n_heads, int(k_pool.size(1)),
+                                                                           head_dim, kv, win, sinks);
+  torch::Tensor ws = new_workspace(ws_bytes, q);
+  check_status(fvb_paged_attention_window_decode(
+                   q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), out.stride(1), out.stride(0),
+                   k_pool.data_ptr(), v_pool.data_ptr(), k_pool.size(0), n_heads, int(k_pool.size(1)), head_dim,
+                   int(k_pool.size(2)), num_seqs, kv_page_tables.data_ptr<int32_t>(), int(kv_page_tables.size(1)),
+                   kv_lens.data_ptr<int32_t>(), kv, win, sinks, dtype_code(q.scalar_type()), ws.data_ptr(), ws_bytes,
+                   stream_of(q)),
+               "PagedAttentionWindowGemvCuda");
+  return out;
+}
+
+// Varlen chunked prefill with the same mask.
+torch::Tensor PagedAttentionWindowGemmCuda(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool,
+                                           torch::Tensor cu_seqlens, int64_t max_q_len, torch::Tensor kv_page_tables,
+                                           torch::Tensor kv_lens, torch::Tensor positions, int64_t window,
+                                           int64_t num_sinks, bool out_token_major) {
+  check_pools(q, k_pool, v_pool);
+  for (const auto* t : {&cu_seqlens, &positions}) {
+    TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->is_contiguous() && t->get_device() == q.get_device(),
+                "cu_seqlens and positions must be contiguous int32 tensors on q's device");
+  }
+  TORCH_CHECK(cu_seqlens.numel() >= 1, "cu_seqlens must have num_seqs + 1 entries");
+  const int num_seqs = int(cu_seqlens.numel()) - 1;
+  check_tables(q, kv_page_tables, kv_lens, num_seqs);
+  const int n_heads = int(q.size(0)), head_dim = int(q.size(2));
+  const int64_t q_len_flatten = q.size(1);
+  TORCH_CHECK(positions.numel() == q_len_flatten, "one position per query token");
+  const int max_q = checked_int(max_q_len, "max_q_len"), win = checked_int(window, "window"),
+            sinks = checked_int(num_sinks, "num_sinks");
+  c10::cuda::CUDAGuard guard(q.device());
+  auto out = new_out(q, out_token_major);
+  const size_t ws_bytes = fvb_paged_attention_prefill_workspace_size(num_seqs, n_heads, int(k_pool.size(1)), head_dim,
+                                                                     q_len_flatten, max_q);
+  torch::Tensor ws = new_workspace(ws_bytes, q);
+  check_status(fvb_paged_attention_window_prefill(
+                   q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), out.stride(1), out.stride(0),
+                   k_pool.data_ptr(), v_pool.data_ptr(), k_pool.size(0), n_heads, int(k_pool.size(1)), head_dim,
+                   int(k_pool.size(2)), num_seqs, q_len_flatten, cu_seqlens.data_ptr<int32_t>(), max_q,
+                   kv_page_tables.data_ptr<int32_t>(), int(kv_page_tables.size(1)), kv_lens.data_ptr<int32_t>(),
+                   positions.data_ptr<int32_t>(), win, sinks, dtype_code(q.scalar_type()), ws.data_ptr(), ws_bytes,
+                   stream_of(q)),
+               "PagedAttentionWindowGemmCuda");
+  return out;
+}
+
+// Decode attention for sequences that share prefixes by groups.
+torch::Tensor PagedAttentionSharedPrefixGemvCuda(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool,
+                                                 torch::Tensor kv_page_tables, torch::Tensor kv_lens,
+                                                 int64_t max_kv_len, torch::Tensor cu_groups,
+                                                 torch::Tensor prefix_lens, int64_t max_prefix_len,
+                                                 bool out_token_major) {
+  check_pools(q, k_pool, v_pool);
+  check_tables(q, kv_page_tables, kv_lens, q.size(1));
+  for (const auto* t : {&cu_groups, &prefix_lens}) {
+    TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->is_contiguous() && t->get_device() == q.get_device(),
+                "cu_groups and prefix_lens must be contiguous int32 tensors on q's device");
+  }
+  TORCH_CHECK(cu_groups.numel() == prefix_lens.numel() + 1, "cu_groups must have one entry more than prefix_lens");
+  const int n_heads = int(q.size(0)), num_seqs = int(q.size(1)), head_dim = int(q.size(2));
+  const int groups = int(prefix_lens.numel()), dt = dtype_code(q.scalar_type());
+  const int kv = checked_int(max_kv_len, "max_kv_len"), prefix = checked_int(max_prefix_len, "max_prefix_len");
+  c10::cuda::CUDAGuard guard(q.device());
+  auto out = new_out(q, out_token_major);
+  const size_t ws_bytes = fvb_paged_attention_shared_prefix_workspace_size(num_seqs, n_heads, int(k_pool.size(1)),
+                                                                           head_dim, groups, prefix, dt);
+  torch::Tensor ws = new_workspace(ws_bytes, q);
+  check_status(fvb_paged_attention_shared_prefix_decode(
+                   q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), out.stride(1), out.stride(0),
+                   k_pool.data_ptr(), v_pool.data_ptr(), k_pool.size(0), n_heads, int(k_pool.size(1)), head_dim,
+                   int(k_pool.size(2)), num_seqs, kv_page_tables.data_ptr<int32_t>(), int(kv_page_tables.size(1)),
+                   kv_lens.data_ptr<int32_t>(), kv, cu_groups.data_ptr<int32_t>(), groups,
+                   prefix_lens.data_ptr<int32_t>(), prefix, dt, ws.data_ptr(), ws_bytes, stream_of(q)),
+               "PagedAttentionSharedPrefixGemvCuda");
+  return out;
+}
+
+// (tokens, parents, scores), each (N, num_select), of N requests of W beams.
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> BeamSearchSelectCuda(torch::Tensor logits,
+                                                                             torch::Tensor scores, int64_t num_select,
+                                                                             c10::optional<torch::Tensor> finished,
+                                                                             int64_t eos_token_id) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
+              "logits must be an (N * W, vocab) CUDA tensor with contiguous rows");
+  TORCH_CHECK(scores.dim() == 2 && scores.scalar_type() == torch::kFloat32 && scores.is_contiguous() &&
+                  scores.get_device() == logits.get_device(),
+              "scores must be a contiguous float32 (N, W) tensor on the logits' device");
+  const int64_t N = scores.size(0), W = scores.size(1), V = logits.size(1);
+  TORCH_CHECK(logits.size(0) == N * W, "one row of logits per beam");
+  TORCH_CHECK(N <= 0x7fffffff && W <= 0x7fffffff, "too many beams");
+  const uint8_t* done = nullptr;
+  if (finished.has_value()) {
+    TORCH_CHECK(finished->scalar_type() == torch::kBool && finished->sizes() == scores.sizes() &&
+                    finished->is_contiguous() && finished->get_device() == logits.get_device(),
+                "finished must be a contiguous bool (N, W) tensor on the logits' device");
+    done = reinterpret_cast<const uint8_t*>(finished->data_ptr<bool>());
+  }
+  const int K = checked_int(num_select, "num_select"), dt = dtype_code(logits.scalar_type());
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto tokens = torch::empty({N, K}, logits.options().dtype(torch::kInt64));
+  auto parents = torch::empty({N, K}, logits.options().dtype(torch::kInt64));
+  auto out = torch::empty({N, K}, scores.options());
+  const size_t ws_bytes = fvb_beam_search_workspace_size(int(N), int(W), V, K, dt);
+  torch::Tensor ws = new_workspace(ws_bytes, logits);
+  // A single row's stride is free: torch leaves any value there.
+  const int64_t stride = logits.size(0) > 1 ? logits.stride(0) : V;
+  check_status(fvb_beam_search_select(logits.data_ptr(), stride, int(N), int(W), V, dt, scores.data_ptr<float>(), done,
+                                      eos_token_id, K, tokens.data_ptr<int64_t>(), parents.data_ptr<int64_t>(),
+                                      out.data_ptr<float>(), ws.data_ptr(), ws_bytes, stream_of(logits)),
+               "BeamSearchSelectCuda");
+  return {tokens, parents, out};
+}
+
+// New block tables; moves the open pages' tokens in every layer's pools.
+torch::Tensor BeamReorderKVCacheCuda(std::vector<torch::Tensor> k_pools, std::vector<torch::Tensor> v_pools,
+                                     torch::Tensor block_tables, torch::Tensor kv_lens, torch::Tensor parents) {
+  TORCH_CHECK(!k_pools.empty() && k_pools.size() == v_pools.size(), "one K and one V pool per layer");
+  const at::Tensor& pool = k_pools[0];
+  TORCH_CHECK(pool.is_cuda() && pool.dim() == 4, "pools must be (num_blocks, n_kv_heads, block_size, d_head) CUDA tensors");
+  std::vector<const void*> k(k_pools.size()), v(v_pools.size());
+  for (size_t i = 0; i < k_pools.size(); ++i) {
+    for (const at::Tensor* t : {&k_pools[i], &v_pools[i]}) {
+      TORCH_CHECK(t->sizes() == pool.sizes() && t->scalar_type() == pool.scalar_type() &&
+                      t->get_device() == pool.get_device() && t->is_contiguous(),
+                  "pools must be contiguous, of one shape and dtype, on one device");
+    }
+    k[i] = k_pools[i].data_ptr();
+    v[i] = v_pools[i].data_ptr();
+  }
+  TORCH_CHECK(block_tables.scalar_type() == torch::kInt32 && kv_lens.scalar_type() == torch::kInt32 &&
+                  parents.scalar_type() == torch::kInt64,
+              "block_tables and kv_lens must be int32, parents int64");
+  TORCH_CHECK(block_tables.dim() == 2 && parents.dim() == 2 && block_tables.is_contiguous() &&
+                  kv_lens.is_contiguous() && parents.is_contiguous(),
+              "block_tables must be (N * W, max_blocks), parents (N, W), all contiguous");
+  TORCH_CHECK(block_tables.get_device() == pool.get_device() && kv_lens.get_device() == pool.get_device() &&
+                  parents.get_device() == pool.get_device(),
+              "block_tables, kv_lens and parents must be on the pools' device");
+  const int64_t N = parents.size(0), W = parents.size(1);
+  TORCH_CHECK(block_tables.size(0) == N * W && kv_lens.numel() == N * W, "one block table row and one kv_len per beam");
+  TORCH_CHECK(N <= 0x7fffffff && W <= 0x7fffffff, "too many beams");
+  c10::cuda::CUDAGuard guard(pool.device());
+  auto out = torch::empty_like(block_tables);
+  check_status(fvb_beam_reorder_kvcache(k.data(), v.data(), int(k.size()), pool.size(0), int(pool.size(1)),
+                                        int(pool.size(3)), int(pool.size(2)), dtype_code(pool.scalar_type()),
+                                        block_tables.data_ptr<int32_t>(), out.data_ptr<int32_t>(),
+                                        int(block_tables.size(1)), kv_lens.data_ptr<int32_t>(),
+                                        parents.data_ptr<int64_t>(), int(N), int(W), stream_of(pool)),
+               "BeamReorderKVCacheCuda");
+  return out;
+}
+
 int64_t SampleWorkspaceSize(int64_t num_rows, int64_t vocab) {
   return int64_t(fvb_sample_workspace_size(int(num_rows), vocab));
 }
@@ -343,6 +533,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "next-token ids: presence penalty, greedy argmax / temperature sampling (one pass over the logits)", py::arg("logits"),
         py::arg("temperatures"), py::arg("presence_penalties") = py::none(), py::arg("token_table") = py::none(),
         py::arg("rng_state"), py::arg("workspace") = py::none());
+  m.def("PagedAttentionWindowGemvCuda", &PagedAttentionWindowGemvCuda,
+        "decode paged attention with a sliding window and sinks", py::arg("q"), py::arg("k_pool"), py::arg("v_pool"),
+        py::arg("kv_page_tables"), py::arg("kv_lens"), py::arg("max_kv_len"), py::arg("window"),
+        py::arg("num_sinks") = 0, py::arg("out_token_major") = false);
+  m.def("PagedAttentionWindowGemmCuda", &PagedAttentionWindowGemmCuda,
+        "varlen chunked-prefill paged attention with a sliding window and sinks", py::arg("q"), py::arg("k_pool"),
+        py::arg("v_pool"), py::arg("cu_seqlens"), py::arg("max_q_len"), py::arg("kv_page_tables"),
+        py::arg("kv_lens"), py::arg("positions"), py::arg("window"), py::arg("num_sinks") = 0,
+        py::arg("out_token_major") = false);
+  m.def("PagedAttentionSharedPrefixGemvCuda", &PagedAttentionSharedPrefixGemvCuda,
+        "decode paged attention for sequences that share prefixes by groups", py::arg("q"), py::arg("k_pool"),
+        py::arg("v_pool"), py::arg("kv_page_tables"), py::arg("kv_lens"), py::arg("max_kv_len"),
+        py::arg("cu_groups"), py::arg("prefix_lens"), py::arg("max_prefix_len"), py::arg("out_token_major") = false);
+  m.def("BeamSearchSelectCuda", &BeamSearchSelectCuda, "best continuations over beams x vocabulary",
+        py::arg("logits"), py::arg("scores"), py::arg("num_select"), py::arg("finished") = py::none(),
+        py::arg("eos_token_id") = -1);
+  m.def("BeamReorderKVCacheCuda", &BeamReorderKVCacheCuda, "paged KV cache and block tables follow the chosen beams",
+        py::arg("k_pools"), py::arg("v_pools"), py::arg("block_tables"), py::arg("kv_lens"), py::arg("parents"));
   m.def("SampleWorkspaceSize", &SampleWorkspaceSize, "workspace bytes of SampleTokensCuda");
   m.def("ReadDeviceError", &ReadDeviceError, "read and clear the device error word (synchronizes)");
 }
@@ -366,6 +574,23 @@ TORCH_LIBRARY(femtovllm_b200, m) {
   m.def(
       "sample_tokens(Tensor logits, Tensor temperatures, Tensor? presence_penalties, Tensor? token_table, "
       "Tensor(a!) rng_state, Tensor(b!)? workspace) -> Tensor");
+  m.def(
+      "paged_attention_window_decode(Tensor q, Tensor k_pool, Tensor v_pool, Tensor block_tables, Tensor kv_lens, "
+      "int max_kv_len, int window, int num_sinks=0, bool out_token_major=False) -> Tensor");
+  m.def(
+      "paged_attention_window_prefill(Tensor q, Tensor k_pool, Tensor v_pool, Tensor cu_seqlens, int max_q_len, "
+      "Tensor block_tables, Tensor kv_lens, Tensor positions, int window, int num_sinks=0, "
+      "bool out_token_major=False) -> Tensor");
+  m.def(
+      "paged_attention_shared_prefix_decode(Tensor q, Tensor k_pool, Tensor v_pool, Tensor block_tables, "
+      "Tensor kv_lens, int max_kv_len, Tensor cu_groups, Tensor prefix_lens, int max_prefix_len, "
+      "bool out_token_major=False) -> Tensor");
+  m.def(
+      "beam_search_select(Tensor logits, Tensor scores, int num_select, Tensor? finished=None, "
+      "int eos_token_id=-1) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "beam_reorder_kvcache(Tensor(a!)[] k_pools, Tensor(b!)[] v_pools, Tensor block_tables, Tensor kv_lens, "
+      "Tensor parents) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(femtovllm_b200, CUDA, m) {
@@ -376,4 +601,9 @@ TORCH_LIBRARY_IMPL(femtovllm_b200, CUDA, m) {
   m.impl("qk_norm_rope_store", &QKNormRopeStoreCuda);
   m.impl("build_varlen_metadata", &BuildVarlenMetadataCuda);
   m.impl("sample_tokens", &SampleTokensCuda);
+  m.impl("paged_attention_window_decode", &PagedAttentionWindowGemvCuda);
+  m.impl("paged_attention_window_prefill", &PagedAttentionWindowGemmCuda);
+  m.impl("paged_attention_shared_prefix_decode", &PagedAttentionSharedPrefixGemvCuda);
+  m.impl("beam_search_select", &BeamSearchSelectCuda);
+  m.impl("beam_reorder_kvcache", &BeamReorderKVCacheCuda);
 }

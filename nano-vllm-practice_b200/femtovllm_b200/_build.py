@@ -54,10 +54,16 @@ CU_SOURCES = [
     "qk_norm_rope.cu",
     "metadata.cu",
     "sampler.cu",
+    "beam_search.cu",
+    "beam_reorder.cu",
     "decode.cu",
+    "decode_window.cu",
     "decode_noalloc.cu",
     "prefill_simt.cu",
     "prefill_sm100.cu",
+    "prefill_window.cu",
+    "shared_prefix.cu",
+    "shared_prefix_tc.cu",
 ]
 
 

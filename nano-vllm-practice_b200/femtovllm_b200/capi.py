@@ -83,6 +83,40 @@ _SIGNATURES = {
          c_int, c_int, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_size_t,
          c_void_p],
     ),
+    "fvb_paged_attention_window_decode_workspace_size": (
+        c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]
+    ),
+    "fvb_paged_attention_window_decode": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+         c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p],
+    ),
+    "fvb_paged_attention_window_prefill": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+         c_int, c_int, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "fvb_paged_attention_shared_prefix_workspace_size": (
+        c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]
+    ),
+    "fvb_paged_attention_shared_prefix_decode": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+         c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_size_t,
+         c_void_p],
+    ),
+    "fvb_beam_search_workspace_size": (c_size_t, [c_int, c_int, c_int64, c_int, c_int]),
+    "fvb_beam_search_select": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_int, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "fvb_beam_reorder_kvcache": (
+        c_int,
+        [ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), c_int, c_int64, c_int, c_int, c_int, c_int, c_void_p,
+         c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p],
+    ),
     "fvb_paged_attention_prefill_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int64, c_int]),
     "fvb_paged_attention_prefill": (
         c_int,

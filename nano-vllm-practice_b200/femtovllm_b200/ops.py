@@ -17,6 +17,12 @@ loops of ``femtovllm/models/qwen/qwen3.py:240-264, 322-366``,
 ``sample_tokens``, the arithmetic of ``femtovllm/engine/sampler.py`` in one
 launch (the drop-in ``Sampler`` module is ``femtovllm_b200.sampler``).
 
+Without a counterpart in the reference, on the same pools and tables:
+``paged_attention_window_gemv`` / ``paged_attention_window_gemm`` (sliding
+window with sinks), ``paged_attention_shared_prefix_gemv`` (sequences that
+share long prefixes), ``beam_search_select`` (best continuations over beams x
+vocabulary) and ``beam_reorder_kvcache`` (the cache follows the chosen beams).
+
 The reference routes each op through a Triton/CUDA backend switch
 (``femtovllm._DEV``, ``ImplCustomKernel``).  That router is gone: ``impl`` is
 accepted for signature compatibility and ignored; every call runs the sm_100a
@@ -127,6 +133,92 @@ def paged_attention_gemm(
     return _cuda_backend.PagedAttentionGemmCuda(
         q, k_pool, v_pool, cu_seqlens, int(max_q_len), kv_page_tables, kv_lens, positions, bool(out_token_major)
     )
+
+
+def _require_cuda(**tensors) -> None:
+    for n, t in tensors.items():
+        if not t.is_cuda:
+            raise ValueError(f"Argument '{n}' must be a CUDA tensor. Got device={t.device}")
+
+
+def paged_attention_window_gemv(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    max_kv_len: int,
+    window: int,
+    num_sinks: int = 0,
+    out_token_major: bool = False,
+) -> torch.Tensor:
+    """:func:`paged_attention_gemv` over the last ``window`` keys and the first ``num_sinks`` of each sequence.
+
+    The query of a sequence sits at position ``kv_len - 1`` and sees key ``j`` iff
+    ``kv_len - 1 - j < window`` or ``j < num_sinks``.  Pages that hold no such key are not read: their
+    table entries may be ``-1`` and their contents anything (NaN included), so an engine may take them
+    back.  ``window >= 1``; ``max_kv_len`` still bounds ``kv_lens``, not the window.
+    """
+    q = _q_view(q)
+    _require_cuda(k_pool=k_pool, v_pool=v_pool, kv_page_tables=kv_page_tables, kv_lens=kv_lens)
+    return _cuda_backend.PagedAttentionWindowGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens, int(max_kv_len),
+                                                      int(window), int(num_sinks), bool(out_token_major))
+
+
+def paged_attention_window_gemm(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    max_q_len: int,
+    kv_page_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    positions: torch.Tensor,
+    window: int,
+    num_sinks: int = 0,
+    out_token_major: bool = False,
+) -> torch.Tensor:
+    """:func:`paged_attention_gemm` where the query at position ``p`` sees key ``j`` iff ``j < kv_len``,
+    ``j <= p``, and ``p - j < window`` or ``j < num_sinks``.
+
+    Pages without a key that some query of the sequence sees are not read, as in
+    :func:`paged_attention_window_gemv`.  The positions of a sequence's tokens must not descend.  A query
+    whose mask leaves nothing gives zeros.
+    """
+    q = _q_view(q)
+    _require_cuda(k_pool=k_pool, v_pool=v_pool, cu_seqlens=cu_seqlens, kv_page_tables=kv_page_tables,
+                  kv_lens=kv_lens, positions=positions)
+    return _cuda_backend.PagedAttentionWindowGemmCuda(q, k_pool, v_pool, cu_seqlens, int(max_q_len), kv_page_tables,
+                                                      kv_lens, positions, int(window), int(num_sinks),
+                                                      bool(out_token_major))
+
+
+def paged_attention_shared_prefix_gemv(
+    q: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    kv_page_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    max_kv_len: int,
+    cu_groups: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    max_prefix_len: int,
+    out_token_major: bool = False,
+) -> torch.Tensor:
+    """:func:`paged_attention_gemv` for a batch whose sequences share prefixes by groups.
+
+    Group ``g`` is sequences ``cu_groups[g] .. cu_groups[g + 1] - 1`` (int32, ``G + 1`` ascending entries;
+    sequences outside every group share nothing); the caller says that their table rows agree in the first
+    ``prefix_lens[g] // 16`` pages (int32, ``G``), which are read once for the group, through its first
+    sequence's row.  The result is that of ``paged_attention_gemv`` on the same tables.
+    ``max_prefix_len`` bounds ``prefix_lens``; keys past it are read per sequence.
+    """
+    q = _q_view(q)
+    _require_cuda(k_pool=k_pool, v_pool=v_pool, kv_page_tables=kv_page_tables, kv_lens=kv_lens, cu_groups=cu_groups,
+                  prefix_lens=prefix_lens)
+    return _cuda_backend.PagedAttentionSharedPrefixGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens,
+                                                            int(max_kv_len), cu_groups, prefix_lens,
+                                                            int(max_prefix_len), bool(out_token_major))
 
 
 def store_kvcache(
@@ -284,6 +376,60 @@ def sample_tokens(
         rng_state = new_rng_state(device=dev)
     return _cuda_backend.SampleTokensCuda(logits, temperatures, presence_penalties, token_table, rng_state,
                                           workspace)
+
+
+def beam_search_select(
+    logits: torch.Tensor,
+    scores: torch.Tensor,
+    num_select: int,
+    finished: torch.Tensor | None = None,
+    eos_token_id: int = -1,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(tokens, parents, scores)``, each ``(N, num_select)``: the best continuations of N requests, best first.
+
+    ``logits`` is ``(N * W, vocab)``, row ``n * W + w`` for beam ``w`` of request ``n``; ``scores``
+    ``(N, W)`` float32 the beams' summed log-probabilities.  A continuation scores
+    ``scores[n, w] + log_softmax(logits)[i]``; ties go to the lowest ``w * vocab + i``, and a score that is
+    not a number (NaN or ``+inf`` logits, a row of ``-inf``) counts as ``-inf``.  ``parents`` (int64) is the
+    beam continued, ``tokens`` (int64) the token.  A beam marked in ``finished`` ``(N, W)`` bool goes on with
+    ``eos_token_id`` at its own score only.  W and ``num_select`` up to 64; the first step after a
+    prompt gives every beam but one a score of ``-inf``.
+    """
+    _require_cuda(logits=logits, scores=scores)
+    if logits.dim() == 2 and logits.stride(-1) != 1:
+        logits = logits.contiguous()
+    if finished is not None:
+        _require_cuda(finished=finished)
+        finished = finished.contiguous()
+    return _cuda_backend.BeamSearchSelectCuda(logits, scores.contiguous(), int(num_select), finished,
+                                              int(eos_token_id))
+
+
+def beam_reorder_kvcache(
+    k_pools: list[torch.Tensor] | torch.Tensor,
+    v_pools: list[torch.Tensor] | torch.Tensor,
+    block_tables: torch.Tensor,
+    kv_lens: torch.Tensor,
+    parents: torch.Tensor,
+) -> torch.Tensor:
+    """Block tables ``(N * W, max_blocks)`` after row ``r`` of each request continues row ``parents[n, r]``.
+
+    ``k_pools`` / ``v_pools``: one ``(num_blocks, n_kv_heads, block_size, d_head)`` pool per layer (a list,
+    or one pool).  All W rows of a request hold ``kv_lens`` tokens, the same number; their full pages may be
+    shared, and the open pages (columns from ``kv_len // block_size`` on) of every row must be its own.
+    A parent's first child takes over its open pages; every further child takes those of a row
+    without a child, into which the tokens of the unfinished page are copied, in every layer.  No page is
+    allocated or freed.  W up to 64.
+    """
+    k_pools = [k_pools] if isinstance(k_pools, torch.Tensor) else list(k_pools)
+    v_pools = [v_pools] if isinstance(v_pools, torch.Tensor) else list(v_pools)
+    for n, pools in (("k_pools", k_pools), ("v_pools", v_pools)):
+        for t in pools:
+            if not t.is_cuda:
+                raise ValueError(f"Argument '{n}' must be CUDA tensors. Got device={t.device}")
+    _require_cuda(block_tables=block_tables, kv_lens=kv_lens, parents=parents)
+    return _cuda_backend.BeamReorderKVCacheCuda(k_pools, v_pools, block_tables.contiguous(), kv_lens.contiguous(),
+                                                parents.contiguous())
 
 
 def read_device_error() -> tuple[int, int]:
