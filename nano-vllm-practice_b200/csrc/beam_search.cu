@@ -11,13 +11,14 @@
 // the beams' best num_select logits can be chosen, and only the comparison of candidates of
 // different beams depends on lse.  Two launches:
 //
-//   partials  CTA (part of a row): each of 8 warps streams a contiguous run of it, folds
-//             sum 2^(x log2e - m) with a lazily moved m, and keeps the run's best logits as
-//             a sorted list across its lanes.  A tile of 32 lanes x 4 vectors enters the
-//             list only where it holds a logit above the list's last one and the last one
-//             of the CTA's best list, so the list costs little once it is warm.
-//   finish    CTA per request (programmatic dependent): merges each row's lists and sums,
-//             then merges the rows by their scores in fp64.  The sums carry an error of
+//   partials  CTA (part of a row): its warps stream the part once, fold sum 2^(x log2e - m)
+//             with a lazily moved m, and keep one number per segment of 32 logits, the
+//             largest.  Of 64 or 128 groups of segments the num_select-th largest maximum is a
+//             bound that at least num_select logits reach, and hardly any more do: only the
+//             segments that reach it are read again, from L2, and their few logits at or above
+//             it are ranked against each other.
+//   finish    CTA per request (programmatic dependent): lse of each beam, then a merge of the
+//             beams' and parts' sorted lists by their scores in fp64, again by a bound.  The sums carry an error of
 //             about 1e-7 from ex2.approx and fp32; where two chosen candidates of different
 //             beams are closer than kNearTie, the lse of the request's beams is computed
 //             again in fp64 (about one request in a thousand), so the order does not
@@ -37,7 +38,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kVecs = 4;  // 16-byte vectors per lane and tile
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kNearTie = 2e-6;
 
@@ -64,44 +64,16 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float unordered(uint32_t u) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
-__device__ __forceinline__ uint64_t make_key(float x, uint32_t i) { return uint64_t(ordered(x)) << 32 | uint32_t(~i); }
+// The same for fp64 scores.
+__device__ __forceinline__ uint64_t ordered64(double x) {
+  const int64_t b = __double_as_longlong(x == 0.0 ? 0.0 : x);
+  return b < 0 ? ~uint64_t(b) : uint64_t(b) | (uint64_t(1) << 63);
+}
+__device__ __forceinline__ double unordered64(uint64_t u) {
+  return __longlong_as_double(int64_t(u >> 63 ? u & ~(uint64_t(1) << 63) : ~u));
+}
 __device__ __forceinline__ float key_logit(uint64_t k) { return unordered(uint32_t(k >> 32)); }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) { return ~uint32_t(k); }
-
-// The best `n` keys of a warp, best first: lane l holds entries l and (KL = 2) l + 32.
-template <int KL>
-struct TopList {
-  uint64_t k[KL];
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < KL; ++i) k[i] = 0;
-  }
-  __device__ __forceinline__ uint64_t at(int i) const {
-    uint64_t v = __shfl_sync(0xffffffffu, k[0], i & 31);
-    if constexpr (KL == 2) {
-      const uint64_t w = __shfl_sync(0xffffffffu, k[1], i & 31);
-      if (i >= 32) v = w;
-    }
-    return v;
-  }
-  // c is the same in every lane; what falls off the end is lost.
-  __device__ __forceinline__ void insert(uint64_t c) {
-    const int lane = threadIdx.x & 31;
-    const int pos = __popc(__ballot_sync(0xffffffffu, k[0] > c));
-    const uint64_t up = __shfl_up_sync(0xffffffffu, k[0], 1);
-    if constexpr (KL == 2) {
-      const int pos2 = 32 + __popc(__ballot_sync(0xffffffffu, k[1] > c));
-      const uint64_t last = __shfl_sync(0xffffffffu, k[0], 31);
-      const uint64_t up2 = __shfl_up_sync(0xffffffffu, k[1], 1);
-      if (pos < 32) {
-        k[1] = lane == 0 ? last : up2;
-      } else if (lane + 32 >= pos2) {
-        k[1] = lane + 32 == pos2 ? c : up2;
-      }
-    }
-    if (lane >= pos) k[0] = lane == pos ? c : up;
-  }
-};
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -114,21 +86,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// The n-th largest (n from 1) of the 32 lanes' v, in every lane: one bitonic sort.
-__device__ __forceinline__ float nth_largest(float v, int n) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int k = 2; k <= 32; k <<= 1) {
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const float o = __shfl_xor_sync(0xffffffffu, v, j);
-      const bool keep_max = ((lane & k) == 0) == ((lane & j) == 0);
-      v = keep_max ? fmaxf(v, o) : fminf(v, o);
-    }
-  }
-  return __shfl_sync(0xffffffffu, v, n - 1);
 }
 
 // Rows may start at any element: vectors are counted from the 16-byte boundary at or before
@@ -146,171 +103,308 @@ struct Row {
   }
   __device__ __forceinline__ int64_t vecs() const { return (vocab + shift + VE - 1) / VE; }
   __device__ __forceinline__ int64_t index(int64_t vec) const { return vec * VE - shift; }
-  __device__ __forceinline__ bool whole(int64_t vec) const {
+  // Vector vec with -inf past the row's ends.
+  __device__ __forceinline__ uint4 load_ragged(int64_t vec) const {
     const int64_t i = index(vec);
-    return i >= 0 && i + VE <= vocab;
-  }
-  __device__ __forceinline__ uint4 load(int64_t vec) const { return ldg_nc_v4(p + index(vec)); }
-  __device__ __forceinline__ void load_ragged(int64_t vec, float* x) const {
-    const int64_t i = index(vec);
+    __align__(16) T x[VE];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) x[e] = i + e >= 0 && i + e < vocab ? Elem<T>::to_f(p[i + e]) : -INFINITY;
+    for (int e = 0; e < VE; ++e) x[e] = i + e >= 0 && i + e < vocab ? p[i + e] : Elem<T>::from_f(-INFINITY);
+    return *reinterpret_cast<const uint4*>(x);
   }
 };
 
-template <typename T, int KL>
+// Elementwise maximum of 32-bit words (one float, or two 16-bit logits); of a number and a NaN the number.
+template <typename T>
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 4) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 m = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float word_max(uint32_t a) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(a);
+  float f[8];
+  unpack16<T>(make_uint4(a, 0, 0, 0), f);
+  return fmaxf(f[0], f[1]);
+}
+
+constexpr int kCtasPerSm = 4;          // CTAs the parts are sized for
+constexpr int kLists = 2;              // sorted lists a thread of the finish kernel merges
+constexpr int kRanked = 512;           // candidates it ranks at once
+constexpr int kFinishThreads = 512;
+constexpr int kFinishWarps = kFinishThreads / 32;
+constexpr int kSegment = 32;           // logits
+constexpr int kMaxSegments = 4096;     // of a part: their maxima fill 16 KB of shared memory
+constexpr int kVecs = 4;               // vectors per lane and tile
+constexpr int kListSegs = 1024, kListLogits = 1024;  // segments and logits at or above the bound that are ranked
+
+// The k-th largest (from 0) of `groups` values (64 or 128) into *bound; whole CTAs of WARPS warps.
+template <int WARPS>
+__device__ __forceinline__ void kth_largest(const uint32_t* values, int groups, int k, uint32_t* bound) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = lane + 32 * j < groups ? values[lane + 32 * j] : 0;
+#pragma unroll 2
+  for (int g = warp; g < groups; g += WARPS) {
+    const uint32_t own = values[g];
+    int before = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j < 2 || groups > 64)
+        before += __popc(__ballot_sync(0xffffffffu, v[j] > own || (v[j] == own && lane + 32 * j < g)));
+    }
+    if (before == k && lane == 0) *bound = own;
+  }
+}
+
+// The n best (value, lower index first) of what the warp's lanes hold, one at a time: lane
+// state (best, at) is each lane's best and its index; take(n-th best's index) is called in
+// the lane that held it and must refresh its state.  Values of 0 are void.
+template <typename Take, typename Emit>
+__device__ __forceinline__ void extract(int n, uint32_t& best, uint32_t& at, Take take, Emit emit) {
+  for (int k = 0; k < n; ++k) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    if (top == 0) {
+      emit(k, 0u, 0u);
+      continue;
+    }
+    const uint32_t index = __reduce_min_sync(0xffffffffu, best == top ? at : 0xffffffffu);
+    emit(k, top, index);
+    if (best == top && at == index) take(index);
+  }
+}
+
+template <typename T>
 __global__ void __launch_bounds__(kThreads) beam_partials_kernel(const BeamArgs a) {
   constexpr int VE = 16 / sizeof(T);
-  __shared__ int cta_last;  // ordered() of the best last entry of the warps' lists, as a signed maximum
-  __shared__ uint64_t sh_keys[kWarps][32 * KL];
+  constexpr int kSegVecs = kSegment / VE;  // 4 (16-bit) or 8 (fp32) lanes share a segment
+  constexpr int kTile = 32 * kVecs;        // vectors of a warp's tile
+  extern __shared__ uint32_t sh[];         // segment maxima as ordered(); then the chosen segments' logits
   __shared__ float2 sh_sums[kWarps];
+  __shared__ uint32_t sh_runs[kThreads / 2];  // largest segment maximum of each group of two or four lanes
+  __shared__ uint64_t cand[kListLogits];
+  __shared__ uint16_t list[kListSegs];
+  __shared__ uint32_t bound;
+  __shared__ int n_list, n_cand;
   launch_dependents();
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (a.finished != nullptr && __ldg(a.finished + row) != 0) return;
   const Row<T> r(a, row);
-  if (threadIdx.x == 0) cta_last = INT_MIN;
-  __syncthreads();
   const int64_t part_begin = part * a.part_vecs;
-  const int64_t part_end = min(r.vecs(), part_begin + a.part_vecs);
-  // Each warp's run: whole tiles of the part, in vocabulary order.
-  constexpr int kTile = 32 * kVecs;
-  const int64_t tiles = part_end > part_begin ? (part_end - part_begin + kTile - 1) / kTile : 0;
-  const int64_t per_warp = (tiles + kWarps - 1) / kWarps;
-  const int64_t begin = part_begin + warp * per_warp * kTile;
-  const int64_t end = min(part_end, begin + per_warp * kTile);
+  const int n_vecs = int(max(min(r.vecs() - part_begin, a.part_vecs), int64_t(0)));
+  const int n_segs = (n_vecs + kSegVecs - 1) / kSegVecs;
 
-  const int K = a.num_select;
-  TopList<KL> top;
-  top.clear();
-  float m = -INFINITY, s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-  float last = -INFINITY;  // the list's K-th logit, once it has one
-  bool first = true;
-  for (int64_t v0 = begin; v0 < end; v0 += kTile) {
-    float x[kVecs][VE];
-    if (v0 > 0 && v0 + kTile <= end && r.whole(v0 + kTile - 1)) {
-      uint4 raw[kVecs];
+  if (threadIdx.x == 0) n_list = n_cand = 0;
+  float m = -INFINITY;
+  uint32_t run = 0;  // of segments of this thread alone; 0: none
+  float2 s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  // Vectors [w0, w1) of the part lie wholly inside the row.
+  const int w0 = part_begin == 0 && r.shift != 0 ? 1 : 0;
+  const int w1 = int(min((a.vocab + r.shift) / VE - part_begin, int64_t(n_vecs)));
+  const T* lane_p = r.p + r.index(part_begin + lane);
+  uint4 ahead[kVecs];  // the warp's next tile, in flight while this one is folded
+  auto fetch = [&](int v0) {
+    if (v0 >= w0 && v0 + kTile <= w1) {
+      const T* p = lane_p + int64_t(v0) * VE;
 #pragma unroll
-      for (int u = 0; u < kVecs; ++u) raw[u] = r.load(v0 + u * 32 + lane);
-#pragma unroll
-      for (int u = 0; u < kVecs; ++u) unpack16<T>(raw[u], x[u]);
+      for (int u = 0; u < kVecs; ++u) ahead[u] = ldg_nc_v4(p + u * 32 * VE);
     } else {
-#pragma unroll
+#pragma unroll 1
       for (int u = 0; u < kVecs; ++u) {
-        const int64_t v = v0 + u * 32 + lane;
-        if (v < end) {
-          r.load_ragged(v, x[u]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) x[u][e] = -INFINITY;
-        }
+        // (past the part: void, no logit of the row)
+        const int v = v0 + u * 32 + lane;
+        const uint4 x = r.load_ragged(v < n_vecs ? part_begin + v : r.vecs() + 1);
+        ahead[0] = u == 0 ? x : ahead[0];
+        ahead[1] = u == 1 ? x : ahead[1];
+        ahead[2] = u == 2 ? x : ahead[2];
+        ahead[3] = u == 3 ? x : ahead[3];
       }
     }
-    float vmax[kVecs];
+  };
+  if (warp * kTile < n_vecs) fetch(warp * kTile);
+  for (int v0 = warp * kTile; v0 < n_vecs; v0 += kWarps * kTile) {
+    uint4 x[kVecs];
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      vmax[u] = x[u][0];
+    for (int u = 0; u < kVecs; ++u) x[u] = ahead[u];
+    if (v0 + kWarps * kTile < n_vecs) fetch(v0 + kWarps * kTile);
+    // ---- segment maxima: in the lane, then over the segment's lanes, which end up with one u each ----
+    uint32_t w[kVecs];
 #pragma unroll
-      for (int e = 1; e < VE; ++e) vmax[u] = fmaxf(vmax[u], x[u][e]);
+    for (int u = 0; u < kVecs; ++u) w[u] = max_word<T>(max_word<T>(x[u].x, x[u].y), max_word<T>(x[u].z, x[u].w));
+    {
+      const bool odd = lane & 1;
+      const uint32_t a0 = __shfl_xor_sync(0xffffffffu, odd ? w[0] : w[1], 1);
+      const uint32_t a1 = __shfl_xor_sync(0xffffffffu, odd ? w[2] : w[3], 1);
+      w[0] = max_word<T>(odd ? w[1] : w[0], a0);  // u = lane & 1
+      w[1] = max_word<T>(odd ? w[3] : w[2], a1);  // u = 2 + (lane & 1)
+      const bool two = lane & 2;
+      const uint32_t b0 = __shfl_xor_sync(0xffffffffu, two ? w[0] : w[1], 2);
+      w[0] = max_word<T>(two ? w[1] : w[0], b0);  // u = lane & 3
+      if constexpr (kSegVecs == 8) w[0] = max_word<T>(w[0], __shfl_xor_sync(0xffffffffu, w[0], 4));
     }
-    const float g = fmaxf(fmaxf(vmax[0], vmax[1]), fmaxf(vmax[2], vmax[3]));
-    // ---- sum of exponentials: m moves only when a tile passes it by more than 2^8 ----
-    const float gm = g * kLog2e;
-    if (gm > m + 8.f) {
-      const float f = ex2(m - gm);  // 0 while m is -inf
-      s0 *= f;
-      s1 *= f;
-      s2 *= f;
-      s3 *= f;
-      m = gm;
+    const float g = word_max<T>(w[0]);
+    const int seg = (v0 + (lane & 3) * 32) / kSegVecs + lane / kSegVecs;
+    if (seg < n_segs && (kSegVecs == 4 || (lane & 4) == 0)) {
+      const uint32_t og = ordered(g);
+      sh[seg] = og;
+      run = max(run, og);
+    }
+    // ---- sum of exponentials; the warp's m moves only when a tile passes it by more than 2^8 ----
+    if (__any_sync(0xffffffffu, g * kLog2e > m + 8.f)) {
+      const float tile_max = unordered(__reduce_max_sync(0xffffffffu, ordered(g))) * kLog2e;
+      const float f = ex2(m - tile_max);  // 0 while m is -inf
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i] = __fmul2_rn(s[i], make_float2(f, f));
+      m = tile_max;
     }
     // m is -inf while every logit was: nothing to add, except that a NaN has to show in the sum
-    const float ms = m == -INFINITY ? 0.f : m;
+    const float ms = m == -INFINITY ? 0.f : -m;
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
+      float f[VE];
+      unpack16<T>(x[u], f);
 #pragma unroll
-      for (int e = 0; e < VE; e += 4) {
-        s0 += ex2(fmaf(x[u][e], kLog2e, -ms));
-        s1 += ex2(fmaf(x[u][e + 1], kLog2e, -ms));
-        s2 += ex2(fmaf(x[u][e + 2], kLog2e, -ms));
-        s3 += ex2(fmaf(x[u][e + 3], kLog2e, -ms));
+      for (int e = 0; e < VE; e += 2) {
+        const float2 t = __ffma2_rn(make_float2(f[e], f[e + 1]), make_float2(kLog2e, kLog2e), make_float2(ms, ms));
+        s[(e >> 1) & 1] = __fadd2_rn(s[(e >> 1) & 1], make_float2(ex2(t.x), ex2(t.y)));
       }
     }
-    // ---- the list ----
-    float least = last, cta = -INFINITY;
-    if (first) {
-      // At least K of the tile's logits are at or above this (all of them where K > 32 or the tile is ragged).
-      least = K <= 32 ? nth_largest(g, K) : -INFINITY;
-    } else {
-      const int c = *reinterpret_cast<volatile int*>(&cta_last);
-      if (c != INT_MIN) cta = unordered(uint32_t(c) ^ 0x80000000u);
-    }
-    // Later logits of a run lose ties against its list, so > the list's last one; other warps' lists may
-    // lie behind this run, so >= theirs.  The first tile fills the list: >=, and -inf counts.
-    auto hit = [&](float y) { return first ? y >= least : (y > least && y >= cta && y >= last); };
-    if (__any_sync(0xffffffffu, hit(g))) {
+  }
+  // ---- the part's sum ----
+  float sum = (s[0].x + s[0].y) + (s[1].x + s[1].y);
 #pragma unroll
-      for (int u = 0; u < kVecs; ++u) {
-        if (!__any_sync(0xffffffffu, hit(vmax[u]))) continue;
-        const int64_t i0 = r.index(v0 + u * 32 + lane);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);  // m is the warp's
+  if (lane == 0) sh_sums[warp] = make_float2(m, sum);
+  const int64_t out = row * a.parts + part;
+  const int K = a.num_select;
+  // Groups of four lanes give 64 maxima (fp32: 32, every other lane's segments are its neighbour's), pairs twice as
+  // many; the fewer there are above K, the more logits reach the bound (about G ln(G / (G - K)) of them).
+  const int shift = K <= (kSegVecs == 4 ? 32 : 16) ? 2 : 1, groups = kThreads >> shift;
+  run = max(run, __shfl_xor_sync(0xffffffffu, run, 1));
+  if (shift == 2) run = max(run, __shfl_xor_sync(0xffffffffu, run, 2));
+  if ((lane & ((1 << shift) - 1)) == 0) sh_runs[threadIdx.x >> shift] = run;
+  __syncthreads();
+  if (warp == kWarps - 1) {  // (a warp that ranks no group)
+    const float2 v = lane < kWarps ? sh_sums[lane] : make_float2(-INFINITY, 0.f);
+    const float mm = warp_max(v.x);
+    float ss = v.x == -INFINITY ? v.y : v.y * ex2(v.x - mm);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const int64_t i = i0 + e;
-          // (the bounds matter in the first tile only, where -inf fills the list)
-          const bool in = v0 + u * 32 + lane < end && i >= 0 && i < a.vocab;
-          uint32_t mask = __ballot_sync(0xffffffffu, in && hit(x[u][e]));
-          const uint64_t key = make_key(x[u][e], uint32_t(i));
-          while (mask) {
-            const int src = __ffs(mask) - 1;
-            mask &= mask - 1;
-            top.insert(__shfl_sync(0xffffffffu, key, src));
-          }
-          if (!first) last = key_logit(top.at(K - 1));
+    for (int o = kWarps / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (lane == 0) a.sums[out] = make_float2(mm, ss);
+  }
+  // ---- bound: the K-th largest group (0, every logit, where fewer than K groups have one) ----
+  kth_largest<kWarps>(sh_runs, groups, K - 1, &bound);
+  __syncthreads();
+  const uint32_t least = bound;
+  // ---- segments that reach it, and their logits that do ----
+  for (int i = threadIdx.x; i < n_segs; i += kThreads) {
+    if (sh[i] < least) continue;
+    const int n = atomicAdd(&n_list, 1);
+    if (n < kListSegs) list[n] = uint16_t(i);
+  }
+  __syncthreads();
+  const int segs = n_list;
+  if (segs <= kListSegs) {
+    constexpr int kReads = 4;  // segments a warp reads at once
+    for (int n0 = warp; n0 < segs; n0 += kWarps * kReads) {
+      uint32_t v[kReads], id[kReads];
+#pragma unroll
+      for (int u = 0; u < kReads; ++u) {
+        const int n = n0 + u * kWarps;
+        v[u] = id[u] = 0;
+        if (n < segs) {
+          const int64_t i = r.index(part_begin + int64_t(list[n]) * kSegVecs) + lane;
+          id[u] = uint32_t(i);
+          if (i >= 0 && i < a.vocab) v[u] = ordered(Elem<T>::to_f(r.p[i]));
         }
       }
-      const uint64_t kth = top.at(K - 1);
-      if (kth != 0) {
-        last = key_logit(kth);
-        if (lane == 0) atomicMax(&cta_last, int(uint32_t(kth >> 32) ^ 0x80000000u));
+#pragma unroll
+      for (int u = 0; u < kReads; ++u) {
+        if (v[u] == 0 || v[u] < least) continue;
+        const int at = atomicAdd(&n_cand, 1);
+        if (at < kListLogits) cand[at] = uint64_t(v[u]) << 32 | ~id[u];
       }
-      // Fewer than K logits so far can only be a run that ends inside its first tile.
     }
-    first = false;
   }
-  // ---- merge the warps' lists and sums ----
-  float s = (s0 + s1) + (s2 + s3);
-  const float M = warp_max(m);
-  s = M == -INFINITY ? s : s * ex2(m - M);  // (a lane without a logit: s = 0, m = -inf)
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) sh_sums[warp] = make_float2(M, s);
-#pragma unroll
-  for (int j = 0; j < KL; ++j) sh_keys[warp][lane + 32 * j] = top.k[j];
   __syncthreads();
-  if (warp != 0) return;
-  for (int w = 1; w < kWarps; ++w) {
-    uint64_t kth = top.at(K - 1);
-    for (int i = 0; i < K; ++i) {
-      const uint64_t c = sh_keys[w][i];
-      if (c <= kth) break;  // sorted: the rest of the list is smaller
-      top.insert(c);
-      kth = top.at(K - 1);
+  const int n = n_cand;
+  if (segs <= kListSegs && n <= kListLogits) {
+    // ---- rank them: keys are different, and fewer than K logits in the part leave 0 behind them ----
+    for (int i = threadIdx.x; i < max(n, K); i += kThreads) {
+      const uint64_t mine = i < n ? cand[i] : 0;
+      int before = i < n ? 0 : i;
+      if (i < n) {
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) before += cand[j] > mine;
+      }
+      if (before < K) a.keys[out * K + before] = mine;
     }
+    return;
   }
-  const int64_t at = row * a.parts + part;
-#pragma unroll
-  for (int j = 0; j < KL; ++j) {
-    if (lane + 32 * j < K) a.keys[at * K + lane + 32 * j] = top.k[j];
+  // ---- too many logits tie with the bound (masked vocabularies), or a few threads hold nearly all of the
+  // largest ones: one warp takes the K largest segments (on ties the lower ones) one by one, then the K best
+  // of their logits.  No other segment can hold one of those: each of the chosen has a logit that is larger,
+  // or equal and of a lower index.  (About 40 us where the ranking takes 2.) ----
+  if (warp != 0) return;
+  const int picks = min(K, n_segs);
+  uint32_t best = 0, at = 0;
+  auto rescan = [&]() {  // the lane's segments lane, lane + 32, ..: the largest, among equal ones the lowest
+    best = 0;
+    for (int i = lane; i < n_segs; i += 32) {
+      const uint32_t v = sh[i];
+      if (v > best) {
+        best = v;
+        at = i;
+      }
+    }
+  };
+  rescan();
+  extract(
+      picks, best, at,
+      [&](uint32_t i) {
+        sh[i] = 0;
+        rescan();
+      },
+      [&](int k, uint32_t, uint32_t i) {
+        if (lane == 0) list[k] = uint16_t(i);
+      });
+  __syncwarp();
+  auto index_of = [&](int k) { return r.index(part_begin + int64_t(list[k]) * kSegVecs) + lane; };
+  for (int k = 0; k < picks; ++k) {
+    const int64_t i = index_of(k);
+    sh[k * 32 + lane] = i >= 0 && i < a.vocab ? ordered(Elem<T>::to_f(r.p[i])) : 0u;
   }
-  if (lane == 0) {
-    float mm = -INFINITY;
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_sums[w].x);
-    float ss = 0.f;
-    for (int w = 0; w < kWarps; ++w)
-      ss += mm == -INFINITY ? sh_sums[w].y : sh_sums[w].y * ex2(sh_sums[w].x - mm);
-    a.sums[at] = make_float2(mm, ss);
-  }
+  int mine = 0;
+  auto rescan_logits = [&]() {  // entry [k][lane] is the lane's own
+    best = 0;
+    for (int k = 0; k < picks; ++k) {
+      const uint32_t v = sh[k * 32 + lane];
+      if (v > best || (v == best && v != 0 && uint32_t(index_of(k)) < at)) {
+        best = v;
+        at = uint32_t(index_of(k));
+        mine = k;
+      }
+    }
+  };
+  rescan_logits();
+  extract(
+      K, best, at,
+      [&](uint32_t) {
+        sh[mine * 32 + lane] = 0;
+        rescan_logits();
+      },
+      [&](int k, uint32_t v, uint32_t i) {
+        if (lane == 0) a.keys[out * K + k] = v == 0 ? 0 : uint64_t(v) << 32 | uint32_t(~i);
+      });
 }
 
 // State of one beam in the finish kernel.
@@ -322,71 +416,77 @@ struct Beam {
 };
 __device__ __forceinline__ bool finite(double x) { return x >= -DBL_MAX && x <= DBL_MAX; }
 
-template <typename T, int KL>
-__global__ void __launch_bounds__(kThreads) beam_finish_kernel(const BeamArgs a) {
-  extern __shared__ uint64_t row_keys[];  // [num_beams][num_select]
+// The next candidate of a sorted list: `score` as ordered64() (0: none left), its token.
+struct Head {
+  uint64_t score;
+  uint32_t token;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamArgs a) {
   __shared__ Beam beams[64];
-  __shared__ double red[kWarps];
-  __shared__ int again;
+  __shared__ double red[kFinishWarps];
+  __shared__ uint32_t best_of[kFinishThreads / 4];
+  __shared__ uint64_t cand_score[kRanked], cand_id[kRanked];
+  __shared__ uint32_t bound;
+  __shared__ uint16_t sorted[65];
+  __shared__ uint64_t top_score[kFinishWarps];
+  __shared__ uint32_t top_beam[kFinishWarps], top_token[kFinishWarps];
+  __shared__ int again, n_cand;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int W = a.num_beams, K = a.num_select;
   const int64_t row0 = int64_t(blockIdx.x) * W;
-  if (threadIdx.x == 0) again = 0;
+  const int per_row = a.parts * K;
+  if (threadIdx.x == 0) again = n_cand = 0;
+  // The call's inputs (the kernel in front only reads them): each beam's score and kind.
+  for (int w = threadIdx.x; w < W; w += kFinishThreads) {
+    const double score = a.scores[row0 + w];
+    const bool done = a.finished != nullptr && a.finished[row0 + w] != 0;
+    beams[w] = Beam{score, 0.f, !finite(score) ? kDead : done ? kDone : kLive};
+  }
   __syncthreads();
+  const unsigned long long* lists = reinterpret_cast<const unsigned long long*>(a.keys) + row0 * per_row;
   grid_dependency_wait();
+  const int n_keys = W * per_row;
+  // Key of the thread's turn: 512 of them at a time, eight neighbours' (a group's, below) from eight different
+  // places of eight different lists, since the best ones stand together at the heads of the lists.
+  const int my_key = (threadIdx.x & 7) * 64 + ((threadIdx.x >> 3) + 5 * (threadIdx.x & 7)) % 64;
+  const uint64_t first_key = my_key < n_keys ? __ldcg(lists + my_key) : 0;  // in flight with the sums
+  __syncthreads();
 
-  // ---- each row's best K and lse ----
-  for (int w = warp; w < W; w += kWarps) {
-    const int64_t row = row0 + w;
-    Beam b;
-    b.base = a.scores[row];
-    b.best = 0.f;
-    b.kind = finite(b.base) ? kDone : kDead;
-    if (a.finished == nullptr || a.finished[row] == 0) {
-      TopList<KL> top;
-      top.clear();
-      const int64_t n = int64_t(a.parts) * K;
-      const unsigned long long* src = reinterpret_cast<const unsigned long long*>(a.keys) + row * n;
-      uint64_t kth = 0;
-      for (int64_t i0 = 0; i0 < n; i0 += 32) {
-        const uint64_t key = i0 + lane < n ? __ldcg(src + i0 + lane) : 0;
-        uint32_t mask = __ballot_sync(0xffffffffu, key > kth);
-        while (mask) {
-          const int from = __ffs(mask) - 1;
-          mask &= mask - 1;
-          top.insert(__shfl_sync(0xffffffffu, key, from));
-        }
-        kth = top.at(K - 1);
-      }
+  // ---- each beam's lse ----
+  for (int w = warp; w < W; w += kFinishWarps) {
+    if (beams[w].kind != kLive) continue;
+    const float2* sums = a.sums + (row0 + w) * a.parts;
+    const unsigned long long* heads = lists + int64_t(w) * per_row;
+    uint64_t first = 0;  // of the parts' best keys, the best
+    float m = -INFINITY;
+    float2 v = make_float2(-INFINITY, 0.f);
+    for (int p = lane; p < a.parts; p += 32) {
+      v = __ldcg(sums + p);
+      m = fmaxf(m, v.x);
+      first = max(first, uint64_t(__ldcg(heads + int64_t(p) * K)));
+    }
+    m = warp_max(m);
+    const float best = unordered(__reduce_max_sync(0xffffffffu, uint32_t(first >> 32)));
+    float s = 0.f;
+    for (int p = lane; p < a.parts; p += 32) {
+      if (a.parts > 32) v = __ldcg(sums + p);
+      s += v.x == -INFINITY ? v.y : v.y * ex2(v.x - m);
+    }
 #pragma unroll
-      for (int j = 0; j < KL; ++j) {
-        if (lane + 32 * j < K) row_keys[w * K + lane + 32 * j] = top.k[j];
-      }
-      b.best = key_logit(top.at(0));
-      const float2* sums = a.sums + row * a.parts;
-      float m = -INFINITY;
-      for (int p = lane; p < a.parts; p += 32) m = fmaxf(m, __ldcg(sums + p).x);
-      m = warp_max(m);
-      double s = 0.0;
-      for (int p = lane; p < a.parts; p += 32) {
-        const float2 v = __ldcg(sums + p);
-        s += v.x == -INFINITY ? double(v.y) : double(v.y) * exp2(double(v.x) - double(m));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) {
       // s 2^m = sum 2^(x c), c = kLog2e in fp32; taken relative to the largest logit, so that c's own
       // rounding acts on differences of logits only.
-      const double above = 0.69314718055994530942 * (log2(s) + (double(m) - double(b.best) * double(kLog2e)));
-      if (b.kind == kDone) {
-        b.kind = kLive;
-        b.base -= above;  // lse - best
-        // +inf or only -inf: no distribution.  Otherwise a NaN, or logits so large that x log2e left the
-        // range of fp32: fp64 tells.
-        if (b.best == INFINITY || b.best == -INFINITY) b.kind = kDead;
-        else if (!finite(b.base) && lane == 0) again = 1;
-      }
+      const double above = 0.69314718055994530942 * (log2(double(s)) + (double(m) - double(best) * double(kLog2e)));
+      beams[w].base -= above;  // lse - best
+      beams[w].best = best;
+      // +inf or only -inf: no distribution.  Otherwise a NaN, or logits so large that x log2e left the
+      // range of fp32: fp64 tells.
+      if (best == INFINITY || best == -INFINITY) beams[w].kind = kDead;
+      else if (!finite(beams[w].base)) again = 1;
     }
-    if (lane == 0) beams[w] = b;
   }
   __syncthreads();
 
@@ -397,14 +497,14 @@ __global__ void __launch_bounds__(kThreads) beam_finish_kernel(const BeamArgs a)
       const T* p = static_cast<const T*>(a.logits) + (row0 + w) * a.row_stride;
       const double top = double(beams[w].best);
       double s = 0.0;
-      for (int64_t i = threadIdx.x; i < a.vocab; i += kThreads) s += exp(double(Elem<T>::to_f(p[i])) - top);
+      for (int64_t i = threadIdx.x; i < a.vocab; i += kFinishThreads) s += exp(double(Elem<T>::to_f(p[i])) - top);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (lane == 0) red[warp] = s;
       __syncthreads();
       if (threadIdx.x == 0) {
         double t = 0.0;
-        for (int k = 0; k < kWarps; ++k) t += red[k];
+        for (int k = 0; k < kFinishWarps; ++k) t += red[k];
         beams[w].base = double(a.scores[row0 + w]) - log(t);
         if (!finite(beams[w].base)) beams[w].kind = kDead;
       }
@@ -413,118 +513,241 @@ __global__ void __launch_bounds__(kThreads) beam_finish_kernel(const BeamArgs a)
   };
   if (again) exact_bases(false);
 
-  // Candidate i of beam w: its score and token; false past the vocabulary.
-  auto candidate = [&](int w, int i, double* score, int64_t* token) {
+  // Close scores of two beams, one of them from logits.  (Beams that are each other's copies tie exactly, in
+  // any precision.)
+  auto near_tie = [&](uint64_t s, int w, uint64_t s2, int w2) {
+    const Beam &b = beams[w], &b2 = beams[w2];
+    return w != w2 && s2 != ordered64(-INFINITY) && unordered64(s) - unordered64(s2) < kNearTie &&
+           (b.kind == kLive || b2.kind == kLive) &&
+           !(s == s2 && b.kind == b2.kind && b.base == b2.base && b.best == b2.best);
+  };
+  // Entry i of beam w's list of part p, whose key is `key`.  A live beam has a list per part; a beam without
+  // logits has one, its first: eos and then every other token (done), or every token (dead), at -inf.
+  auto candidate = [&](int w, int p, int i, uint64_t key) {
+    Head h{0, 0};
     const Beam& b = beams[w];
-    *score = -INFINITY;
-    *token = i;
-    if (i >= K || i >= a.vocab) return false;
     if (b.kind == kLive) {
-      const uint64_t key = row_keys[w * K + i];
-      *token = key_index(key);
+      if (key == 0) return h;
       const float x = key_logit(key);
-      if (x != -INFINITY) *score = b.base + (double(x) - double(b.best));
-    } else if (b.kind == kDone) {
-      if (i == 0) *score = b.base;
-      *token = i == 0 ? a.eos : i - 1 + (i - 1 >= a.eos ? 1 : 0);
+      h.token = key_index(key);
+      h.score = ordered64(x == -INFINITY ? double(-INFINITY) : b.base + (double(x) - double(b.best)));
+    } else if (p == 0 && i < a.vocab) {
+      h.score = ordered64(b.kind == kDone && i == 0 ? b.base : double(-INFINITY));
+      h.token = b.kind == kDead ? i : i == 0 ? uint32_t(a.eos) : i - 1 + (i - 1 >= a.eos ? 1 : 0);
     }
-    return true;
+    return h;
+  };
+  bool exact = false;  // every live beam's base is from fp64
+  // ---- most requests: the candidates that reach a bound which at least K + 1 do, ranked against each other.
+  // The bound is the (K + 1)-th largest of 64 or 128 groups' best scores, rounded to fp32. ----
+  {
+    const int shift = K < 32 ? 3 : 2, groups = kFinishThreads >> shift;
+    auto rounded = [](uint64_t score) { return score == 0 ? 0u : ordered(float(unordered64(score))); };
+    auto beam_of = [&](int i) { return i / per_row; };
+    auto nth = [&](int i, uint64_t key) {
+      const int w = beam_of(i), p = (i - w * per_row) / K;
+      return candidate(w, p, i - w * per_row - p * K, key);
+    };
+    const Head mine = my_key < n_keys ? nth(my_key, first_key) : Head{0, 0};
+    uint32_t run = rounded(mine.score);
+#pragma unroll 1
+    for (int i = my_key + kFinishThreads; i < n_keys; i += kFinishThreads)
+      run = max(run, rounded(nth(i, __ldcg(lists + i)).score));
+    const uint32_t first_run = rounded(mine.score);
+    for (int o = 1; o < 1 << shift; o <<= 1) run = max(run, __shfl_xor_sync(0xffffffffu, run, o));
+    if ((lane & ((1 << shift) - 1)) == 0) best_of[threadIdx.x >> shift] = run;
+    __syncthreads();
+    kth_largest<kFinishWarps>(best_of, groups, K, &bound);
+    __syncthreads();
+    const uint32_t least = bound;
+    if (least > ordered(-INFINITY)) {
+      auto keep = [&](int i, const Head& h) {
+        const int at = atomicAdd(&n_cand, 1);
+        if (at >= kRanked) return;
+        cand_score[at] = h.score;
+        cand_id[at] = uint64_t(beam_of(i)) << 32 | h.token;
+      };
+      if (first_run != 0 && first_run >= least) keep(my_key, mine);
+#pragma unroll 1
+      for (int i = my_key + kFinishThreads; i < n_keys; i += kFinishThreads) {
+        const Head h = nth(i, __ldcg(lists + i));
+        if (h.score != 0 && rounded(h.score) >= least) keep(i, h);
+      }
+      __syncthreads();
+      const int c = n_cand;
+      if (c <= kRanked) {
+        if (threadIdx.x < c) {  // kRanked <= kFinishThreads
+          const uint64_t score = cand_score[threadIdx.x], id = cand_id[threadIdx.x];
+          int before = 0, equal = 0;
+#pragma unroll 8
+          for (int j = 0; j < c; ++j) {
+            before += cand_score[j] > score;
+            equal += cand_score[j] == score;
+          }
+          if (equal > 1) {
+            for (int j = 0; j < c; ++j) before += cand_score[j] == score && cand_id[j] < id;
+          }
+          if (before <= K) sorted[before] = threadIdx.x;
+        }
+        __syncthreads();
+        for (int k = threadIdx.x; k < K; k += kFinishThreads) {
+          const uint64_t score = cand_score[sorted[k]], id = cand_id[sorted[k]];
+          const uint64_t score2 = cand_score[sorted[k + 1]], id2 = cand_id[sorted[k + 1]];
+          const int64_t o = int64_t(blockIdx.x) * K + k;
+          a.tokens[o] = uint32_t(id);
+          a.parents[o] = id >> 32;
+          a.out_scores[o] = float(unordered64(score));
+          if (near_tie(score, int(id >> 32), score2, int(id2 >> 32))) again = 1;
+        }
+        __syncthreads();
+        if (again == 0) return;
+        exact_bases(true);
+        exact = true;
+      }
+    }
+  }
+
+  // ---- else (fewer than K + 1 finite candidates, a crowd of equal ones, or scores computed again above), one
+  // by one: a merge of the W * parts sorted lists, up to kLists a thread ----
+  auto entry = [&](int l, int i) {
+    const int w = l / a.parts;
+    return i < K ? candidate(w, l - w * a.parts, i, __ldcg(lists + int64_t(l) * K + i)) : Head{0, 0};
+  };
+  // (score, beam, token) order: the higher score, then the lower beam, then the lower token
+  auto better = [](uint64_t s, uint32_t w, uint32_t t, uint64_t s2, uint32_t w2, uint32_t t2) {
+    return s != s2 ? s > s2 : w != w2 ? w < w2 : t < t2;
+  };
+  // The warp's best of its lanes' (score, beam, token), in every lane.
+  auto warp_best = [&](uint64_t& s, uint32_t& w, uint32_t& t) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(s >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, uint32_t(s >> 32) == hi ? uint32_t(s) : 0u);
+    const uint64_t top = uint64_t(hi) << 32 | lo;
+    const uint32_t who = __ballot_sync(0xffffffffu, s == top);
+    uint32_t w1 = w, t1 = t;
+    if (__popc(who) == 1) {
+      const int src = __ffs(who) - 1;
+      w1 = __shfl_sync(0xffffffffu, w, src);
+      t1 = __shfl_sync(0xffffffffu, t, src);
+    } else {  // equal scores
+      w1 = __reduce_min_sync(0xffffffffu, s == top ? w : 0xffffffffu);
+      t1 = __reduce_min_sync(0xffffffffu, s == top && w == w1 ? t : 0xffffffffu);
+    }
+    s = top;
+    w = w1;
+    t = t1;
   };
 
-  // ---- the request's best K: a merge of W sorted lists, one or two a lane ----
-  for (int pass = 0; pass < 2; ++pass) {
+  const int L = W * a.parts;
+  const int warps = L <= 32 * kLists ? 1 : kFinishWarps;
+  for (int pass = exact ? 1 : 0; pass < 2; ++pass) {
     __syncthreads();
-    if (warp == 0) {
-      int at[2] = {0, 0};
-      double sc[2];
-      int64_t tk[2];
-      bool have[2];
+    bool near = false;
+    if (warp < warps) {
+      Head head[kLists], next[kLists];  // each list's first candidate that is left, and the one behind it
+      int at[kLists];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) have[j] = lane + 32 * j < W && candidate(lane + 32 * j, 0, &sc[j], &tk[j]);
-      double prev = 0.0;
-      int prev_w = 0;
-      bool near = false;
-      for (int n = 0; n <= K; ++n) {
-        // the lane's better head, then the warp's: higher score, then lower beam
-        int w = -1;
-        double best = 0.0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          if (have[j] && (w < 0 || sc[j] > best)) {
-            w = lane + 32 * j;
-            best = sc[j];
-          }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const double ob = __shfl_xor_sync(0xffffffffu, best, o);
-          const int ow = __shfl_xor_sync(0xffffffffu, w, o);
-          if (ow >= 0 && (w < 0 || ob > best || (ob == best && ow < w))) {
-            best = ob;
-            w = ow;
-          }
-        }
-        if (w < 0) break;  // fewer than K + 1 candidates
-        // Close scores of two beams, one of them from logits.  (Beams that are each other's copies tie
-        // exactly, in any precision.)
-        if (n > 0 && w != prev_w && best != -INFINITY && prev - best < kNearTie &&
-            (beams[w].kind == kLive || beams[prev_w].kind == kLive) &&
-            !(best == prev && beams[w].kind == beams[prev_w].kind && beams[w].base == beams[prev_w].base &&
-              beams[w].best == beams[prev_w].best))
-          near = true;
-        prev = best;
-        prev_w = w;
-        if (n == K) break;
-        const int j = w >> 5;
-        if (lane == (w & 31)) {
-          const int64_t o = int64_t(blockIdx.x) * K + n;
-          a.tokens[o] = tk[j];
-          a.parents[o] = w;
-          a.out_scores[o] = float(best);
-          ++at[j];
-          have[j] = candidate(w, at[j], &sc[j], &tk[j]);
+      for (int j = 0; j < kLists; ++j) {
+        const int l = threadIdx.x + j * 32 * warps;
+        head[j] = next[j] = Head{0, 0};
+        at[j] = 1;
+        if (l < L) {
+          head[j] = entry(l, 0);
+          next[j] = entry(l, 1);
         }
       }
-      if (lane == 0) again = near && pass == 0;
+      uint64_t prev = 0;
+      uint32_t prev_w = 0;
+      for (int n = 0; n <= K; ++n) {
+        const uint32_t w0 = threadIdx.x / a.parts, w1 = (threadIdx.x + 32 * warps) / a.parts;
+        const int mine = better(head[1].score, w1, head[1].token, head[0].score, w0, head[0].token) ? 1 : 0;
+        uint64_t s = mine ? head[1].score : head[0].score;
+        uint32_t t = mine ? head[1].token : head[0].token;
+        uint32_t w = mine ? w1 : w0;
+        const uint64_t own = s;
+        const uint32_t own_w = w, own_t = t;
+        warp_best(s, w, t);
+        if (warps > 1) {
+          if (lane == 0) {
+            top_score[warp] = s;
+            top_beam[warp] = w;
+            top_token[warp] = t;
+          }
+          __syncthreads();
+          s = lane < kFinishWarps ? top_score[lane] : 0;
+          w = lane < kFinishWarps ? top_beam[lane] : 0;
+          t = lane < kFinishWarps ? top_token[lane] : 0;
+          warp_best(s, w, t);
+          __syncthreads();
+        }
+        if (s == 0) break;  // fewer than K + 1 candidates
+        const double best = unordered64(s);
+        if (n > 0 && near_tie(prev, prev_w, s, w)) near = true;
+        prev = s;
+        prev_w = w;
+        if (n == K) break;
+        if (own == s && own_w == w && own_t == t) {  // one list alone holds a beam's token
+          const int64_t o = int64_t(blockIdx.x) * K + n;
+          a.tokens[o] = t;
+          a.parents[o] = w;
+          a.out_scores[o] = float(best);
+#pragma unroll
+          for (int j = 0; j < kLists; ++j) {
+            if (j != mine) continue;
+            head[j] = next[j];
+            next[j] = entry(threadIdx.x + j * 32 * warps, ++at[j]);
+          }
+        }
+      }
     }
+    if (threadIdx.x == 0) again = near && pass == 0;
     __syncthreads();
     if (again == 0) return;
     exact_bases(true);
   }
 }
 
-template <typename T, int KL>
+template <typename T>
 cudaError_t launch_t(const BeamArgs& a, int num_requests, cudaStream_t stream) {
-  beam_partials_kernel<T, KL><<<unsigned(num_requests) * a.num_beams * a.parts, kThreads, 0, stream>>>(a);
+  const int segs = std::max(int((a.part_vecs * 16 / sizeof(T) + kSegment - 1) / kSegment), 32 * a.num_select);
+  beam_partials_kernel<T><<<unsigned(num_requests) * a.num_beams * a.parts, kThreads, segs * 4, stream>>>(a);
   cudaError_t ce = cudaGetLastError();
   if (ce != cudaSuccess) return ce;
-  const int smem = a.num_beams * a.num_select * 8;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(num_requests);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(kFinishThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, beam_finish_kernel<T, KL>, a);
+  return cudaLaunchKernelEx(&cfg, beam_finish_kernel<T>, a);
 }
 
-// Parts a row is cut into: enough CTAs for the device, parts of at least one tile a warp.
-int beam_parts(int rows, int64_t vocab, int esize) {
-  const int64_t vecs = (vocab * esize + 15) / 16 + 1;
-  const int64_t most = std::max<int64_t>(1, vecs / (32 * kVecs * 2));
-  const int64_t wanted = (int64_t(device_sm_count()) * 4 + rows - 1) / rows;
-  return int(std::max<int64_t>(1, std::min(most, wanted)));
+// Vectors of a part, in whole tiles of a CTA's warps: enough CTAs for the device, at most kMaxSegments
+// segments, and no more lists a request than the finish kernel's threads merge where that allows.
+int64_t beam_part_vecs(int num_requests, int num_beams, int64_t vocab, int esize) {
+  const int64_t vecs = (vocab * esize + 15) / 16 + 1;  // a row may straddle one vector more
+  const int64_t rows = int64_t(num_requests) * num_beams, tile = 32 * kVecs * kWarps;
+  const int64_t wanted = std::min<int64_t>((int64_t(device_sm_count()) * kCtasPerSm + rows - 1) / rows,
+                                           kLists * kFinishThreads / num_beams);
+  const int64_t per = ((vecs + wanted - 1) / wanted + tile - 1) / tile * tile;
+  return std::min<int64_t>(per, int64_t(kMaxSegments) * kSegment * esize / 16);
+}
+int64_t beam_parts(int num_requests, int num_beams, int64_t vocab, int esize) {
+  const int64_t vecs = (vocab * esize + 15) / 16 + 1, per = beam_part_vecs(num_requests, num_beams, vocab, esize);
+  return (vecs + per - 1) / per;
 }
 
 }  // namespace
 
+bool beam_supported(int num_requests, int num_beams, int64_t vocab, int esize) {
+  const int64_t parts = beam_parts(num_requests, num_beams, vocab, esize);
+  return parts * num_beams <= kLists * kFinishThreads && parts * num_beams * num_requests < (int64_t(1) << 31);
+}
+
 size_t beam_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select, int esize) {
-  const size_t rows = size_t(num_requests) * num_beams;
-  const size_t parts = rows * beam_parts(int(rows), vocab, esize);
+  const size_t parts = size_t(num_requests) * num_beams * beam_parts(num_requests, num_beams, vocab, esize);
   return ((parts * num_select * 8 + 255) & ~size_t(255)) + parts * 8;
 }
 
@@ -532,7 +755,7 @@ cudaError_t launch_beam_select(const void* logits, int64_t row_stride, int num_r
                                int dtype, const float* scores, const uint8_t* finished, int64_t eos, int num_select,
                                int64_t* tokens, int64_t* parents, float* out_scores, void* workspace,
                                cudaStream_t stream) {
-  const int rows = num_requests * num_beams;
+  const int64_t rows = int64_t(num_requests) * num_beams;
   const int es = dtype == FVB_DTYPE_F32 ? 4 : 2;
   BeamArgs a{};
   a.logits = logits;
@@ -543,21 +766,17 @@ cudaError_t launch_beam_select(const void* logits, int64_t row_stride, int num_r
   a.eos = eos;
   a.num_beams = num_beams;
   a.num_select = num_select;
-  a.parts = beam_parts(rows, vocab, es);
-  const int64_t vecs = (vocab * es + 15) / 16 + 1;  // a row may straddle one vector more
-  a.part_vecs = (vecs + a.parts - 1) / a.parts;
+  a.parts = int(beam_parts(num_requests, num_beams, vocab, es));
+  a.part_vecs = beam_part_vecs(num_requests, num_beams, vocab, es);
   a.keys = static_cast<uint64_t*>(workspace);
   const size_t key_bytes = (size_t(rows) * a.parts * num_select * 8 + 255) & ~size_t(255);
   a.sums = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + key_bytes);
   a.tokens = tokens;
   a.parents = parents;
   a.out_scores = out_scores;
-#define FVB_BEAM(T) \
-  (num_select <= 32 ? launch_t<T, 1>(a, num_requests, stream) : launch_t<T, 2>(a, num_requests, stream))
-  if (dtype == FVB_DTYPE_BF16) return FVB_BEAM(__nv_bfloat16);
-  if (dtype == FVB_DTYPE_F16) return FVB_BEAM(__half);
-  return FVB_BEAM(float);
-#undef FVB_BEAM
+  if (dtype == FVB_DTYPE_BF16) return launch_t<__nv_bfloat16>(a, num_requests, stream);
+  if (dtype == FVB_DTYPE_F16) return launch_t<__half>(a, num_requests, stream);
+  return launch_t<float>(a, num_requests, stream);
 }
 
 }  // namespace fvb

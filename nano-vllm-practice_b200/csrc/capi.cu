@@ -635,7 +635,9 @@ int fvb_paged_attention_shared_prefix_decode(
 }
 
 size_t fvb_beam_search_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select, int dtype) {
-  if (num_requests <= 0 || num_beams <= 0 || vocab <= 0 || num_select <= 0 || esize_of(dtype) == 0) return 0;
+  if (num_requests <= 0 || num_beams <= 0 || num_beams > kMaxBeams || vocab <= 0 || num_select <= 0 ||
+      esize_of(dtype) == 0)
+    return 0;
   return beam_workspace_size(num_requests, num_beams, vocab, num_select, esize_of(dtype));
 }
 
@@ -653,8 +655,8 @@ int fvb_beam_search_select(const void* logits, int64_t row_stride, int num_reque
   if (finished && (eos_token_id < 0 || eos_token_id >= vocab)) return FVB_ERR_INVALID_ARGUMENT;
   if (num_requests == 0) return FVB_OK;
   if (!logits || !scores || !tokens || !parents || !out_scores) return FVB_ERR_INVALID_ARGUMENT;
-  // One CTA per part of a row, parts of 2048 columns at least.
-  if (int64_t(num_requests) * num_beams * (vocab / 2048 + 1) >= (int64_t(1) << 31)) return FVB_ERR_UNSUPPORTED;
+  // One CTA per part of a row, and at most 1024 parts a request.
+  if (!beam_supported(num_requests, num_beams, vocab, es)) return FVB_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < beam_workspace_size(num_requests, num_beams, vocab, num_select, es))
     return FVB_ERR_WORKSPACE_TOO_SMALL;
   if ((reinterpret_cast<uintptr_t>(logits) % es) != 0 || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0 ||

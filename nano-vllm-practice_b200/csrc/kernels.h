@@ -243,6 +243,7 @@ cudaError_t launch_sample(const void* logits, int64_t row_stride, int num_rows, 
 // Beam search (beam_search.cu, beam_reorder.cu).  At most kMaxBeams beams a request and
 // kMaxBeams selected continuations.
 constexpr int kMaxBeams = 64;
+bool beam_supported(int num_requests, int num_beams, int64_t vocab, int esize);
 size_t beam_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select, int esize);
 cudaError_t launch_beam_select(const void* logits, int64_t row_stride, int num_requests, int num_beams, int64_t vocab,
                                int dtype, const float* scores, const uint8_t* finished, int64_t eos, int num_select,
