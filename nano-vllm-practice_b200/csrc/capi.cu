@@ -507,10 +507,9 @@ size_t fvb_paged_attention_window_decode_workspace_size(int num_seqs, int n_head
   const int sms = device_sm_count();
   const size_t split_ws =
       plan_window_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms).ws_bytes;
-  if (!decode_on_tensor_cores(n_heads, n_kv_heads, FVB_DTYPE_BF16)) return split_ws;
-  const size_t tc_ws =
-      plan_window_tc_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms).ws_bytes;
-  return split_ws > tc_ws ? split_ws : tc_ws;  // fp32, 16-bit
+  if (num_seqs > kKeysMaxSeqs) return split_ws;
+  const size_t keys_ws = plan_keys(num_seqs, n_heads, head_dim, kKeysWindow, sms).ws_bytes;
+  return split_ws > keys_ws ? split_ws : keys_ws;  // fp32, 16-bit
 }
 
 int fvb_paged_attention_window_decode(const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out,
@@ -535,21 +534,27 @@ int fvb_paged_attention_window_decode(const void* q, int64_t q_token_stride, int
   if (num_seqs > kMaxGridYZ || int64_t(n_heads) > kMaxGridYZ) return FVB_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;
   const int sms = device_sm_count();
-  const bool tc = decode_on_tensor_cores(n_heads, n_kv_heads, dtype);
+  // 16-bit: the tensor-core kernel, whose table of sequences fits its shared memory; fp32 and larger batches
+  // the split-KV kernel.
+  const bool tc = dtype != FVB_DTYPE_F32 && num_seqs <= kKeysMaxSeqs;
   DecodePlan plan{};
-  TcDecodePlan tp{};
-  if (tc) tp = plan_window_tc_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms);
+  KeysPlan kp{};
+  if (tc) kp = plan_keys(num_seqs, n_heads, head_dim, kKeysWindow, sms);
   else plan = plan_window_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms);
-  const size_t need = tc ? tp.ws_bytes : plan.ws_bytes;
+  const size_t need = tc ? kp.ws_bytes : plan.ws_bytes;
   if (need > 0 && (!workspace || workspace_bytes < need)) return FVB_ERR_WORKSPACE_TOO_SMALL;
   cudaError_t e;
   int* err = device_error_ptr(&e);
   if (!err) return cuda_status(e);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (tc)
-    return cuda_status(launch_window_tc_decode(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim,
-                                               num_seqs, block_tables, max_blocks_per_seq, kv_lens, max_kv_len,
-                                               window, num_sinks, dtype, tp, lay, workspace, err, s));
+  if (tc) {
+    DecodeExtra ex;
+    ex.window = window;
+    ex.sinks = num_sinks;
+    return cuda_status(launch_keys_decode(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, num_seqs,
+                                          block_tables, max_blocks_per_seq, kv_lens, max_kv_len, ex, kKeysWindow,
+                                          dtype, kp, lay, workspace, false, err, s));
+  }
   return cuda_status(launch_window_decode(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, num_seqs,
                                           block_tables, max_blocks_per_seq, kv_lens, max_kv_len, window, num_sinks,
                                           dtype, plan, lay, workspace, err, s));

@@ -55,6 +55,11 @@ __host__ __device__ __forceinline__ KeySpan window_span(int first_end, int kv_le
   return s;
 }
 
+// CTA that holds tile g of `total` dealt evenly to `grid` CTAs: CTA c has [total c / grid, total (c + 1) / grid).
+__device__ __forceinline__ int keys_cta_of(int64_t g, int64_t total, int grid) {
+  return int(((g + 1) * grid - 1) / total);
+}
+
 // Sequences of group g, inside [0, num_seqs) whatever cu_groups holds.
 __device__ __forceinline__ int2 group_rows(const DecodeExtra& ex, int g, int num_seqs) {
   const int lo = min(max(__ldg(ex.cu_groups + g), 0), num_seqs);
@@ -269,6 +274,18 @@ __device__ __forceinline__ bool named_barrier_and(int id, int nthreads, bool pre
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(uint32_t(pred)), "r"(id), "r"(nthreads)
+      : "memory");
+  return r != 0;
+}
+
+// ... the OR of pred over them.
+__device__ __forceinline__ bool named_barrier_or(int id, int nthreads, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"(uint32_t(pred)), "r"(id), "r"(nthreads)

@@ -526,9 +526,7 @@ __global__ void __launch_bounds__(kCmbThreads) decode_combine_kernel(const float
       kv_len = min(kv_len, first_end);
     }
   }
-  // (window mode: ranges of ex.unit keys, pages for the split kernel above and 128-key tiles for the
-  // tensor-core one, and pages_per_split of those)
-  const int npages = MODE == kDecodeWindow ? window_span(first_end, kv_len, ex.window, ex.sinks, ex.unit).count
+  const int npages = MODE == kDecodeWindow ? window_span(first_end, kv_len, ex.window, ex.sinks, kPageSize).count
                                            : (kv_len + kPageSize - 1) / kPageSize;
   const int nsplits = (npages + pages_per_split - 1) / pages_per_split;
   // Every CTA waits for the split grid, also those with nothing to merge: the combine grid

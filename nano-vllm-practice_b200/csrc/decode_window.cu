@@ -21,9 +21,7 @@ cudaError_t dispatch(int nrep, const void* q, void* out, const void* k_pool, con
     case 4:
       return launch_decode_t<T, D, 4, kDecodeWindow>(FVB_DW_ARGS);
     default:
-      // 16-bit groups of 5 and more take the tensor-core kernel; only fp32 comes here
-      if constexpr (sizeof(T) == 4) return launch_decode_t<T, D, 8, kDecodeWindow>(FVB_DW_ARGS);
-      return cudaErrorInvalidValue;
+      return launch_decode_t<T, D, 8, kDecodeWindow>(FVB_DW_ARGS);
   }
 #undef FVB_DW_ARGS
 }
@@ -54,7 +52,6 @@ cudaError_t launch_window_decode(const void* q, void* out, const void* k_pool, c
   DecodeExtra ex;
   ex.window = window;
   ex.sinks = sinks;
-  ex.unit = kPageSize;
 #define FVB_DW_ARGS nrep, q, out, k_pool, v_pool, num_blocks, n_kv_heads, num_seqs, block_tables, \
                     max_blocks_per_seq, kv_lens, max_kv_len, plan, lay, workspace, err, stream, q_index, q_pos, ex
   if (dtype == FVB_DTYPE_BF16)
@@ -63,25 +60,6 @@ cudaError_t launch_window_decode(const void* q, void* out, const void* k_pool, c
     return head_dim == 128 ? dispatch<__half, 128>(FVB_DW_ARGS) : dispatch<__half, 64>(FVB_DW_ARGS);
   return head_dim == 128 ? dispatch<float, 128>(FVB_DW_ARGS) : dispatch<float, 64>(FVB_DW_ARGS);
 #undef FVB_DW_ARGS
-}
-
-cudaError_t launch_window_combine(const float* ws_o, const float* ws_lse, void* out, const int32_t* kv_lens,
-                                  int kv_cap, int num_seqs, int n_heads, int head_dim, int window, int sinks, int unit,
-                                  int units_per_split, int max_splits, int dtype, const QOLayout& lay,
-                                  cudaStream_t stream) {
-  DecodeExtra ex;
-  ex.window = window;
-  ex.sinks = sinks;
-  ex.unit = unit;
-#define FVB_WC_ARGS ws_o, ws_lse, out, kv_lens, kv_cap, num_seqs, n_heads, units_per_split, max_splits, lay, stream, \
-                    nullptr, nullptr, ex
-  if (dtype == FVB_DTYPE_BF16) {
-    return head_dim == 128 ? launch_combine_t<__nv_bfloat16, 128, kDecodeWindow>(FVB_WC_ARGS)
-                           : launch_combine_t<__nv_bfloat16, 64, kDecodeWindow>(FVB_WC_ARGS);
-  }
-  return head_dim == 128 ? launch_combine_t<__half, 128, kDecodeWindow>(FVB_WC_ARGS)
-                         : launch_combine_t<__half, 64, kDecodeWindow>(FVB_WC_ARGS);
-#undef FVB_WC_ARGS
 }
 
 }  // namespace fvb

@@ -76,7 +76,6 @@ DecodePlan plan_decode(int num_seqs, int n_heads, int n_kv_heads, int head_dim, 
 // plain form's arguments.
 struct DecodeExtra {
   int window = 0, sinks = 0;  // keys behind the query that stay visible (itself included), first keys that do
-  int unit = 0;               // combine: keys a split counts in (a page, or a 128-key tile)
   const int32_t* cu_groups = nullptr;    // shared prefix: sequences cu_groups[g] .. cu_groups[g + 1] - 1 ...
   const int32_t* prefix_lens = nullptr;  // ... share the pages of their first prefix_lens[g] keys
   int num_groups = 0;
@@ -164,17 +163,6 @@ cudaError_t launch_window_decode(const void* q, void* out, const void* k_pool, c
                                  int dtype, const DecodePlan& plan, const QOLayout& lay, void* workspace, int* err,
                                  cudaStream_t stream, const int32_t* q_index = nullptr,
                                  const int32_t* q_pos = nullptr);
-cudaError_t launch_window_combine(const float* ws_o, const float* ws_lse, void* out, const int32_t* kv_lens,
-                                  int kv_cap, int num_seqs, int n_heads, int head_dim, int window, int sinks, int unit,
-                                  int units_per_split, int max_splits, int dtype, const QOLayout& lay,
-                                  cudaStream_t stream);
-TcDecodePlan plan_window_tc_decode(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int max_kv_len, int window,
-                                   int sinks, int num_sms);
-cudaError_t launch_window_tc_decode(const void* q, void* out, const void* k_pool, const void* v_pool,
-                                    int64_t num_blocks, int n_heads, int n_kv_heads, int head_dim, int num_seqs,
-                                    const int32_t* block_tables, int max_blocks_per_seq, const int32_t* kv_lens,
-                                    int max_kv_len, int window, int sinks, int dtype, const TcDecodePlan& plan,
-                                    const QOLayout& lay, void* workspace, int* err, cudaStream_t stream);
 cudaError_t launch_window_prefill(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
                                   int n_heads, int n_kv_heads, int head_dim, int num_seqs, int64_t q_len_flatten,
                                   const int32_t* cu_seqlens, const int32_t* block_tables, int max_blocks_per_seq,
@@ -188,6 +176,23 @@ cudaError_t launch_window_prefill_simt(const void* q, void* out, const void* k_p
                                        int max_blocks_per_seq, const int32_t* kv_lens, const int32_t* positions,
                                        int window, int sinks, const QOLayout& lay, int* err, cudaStream_t stream);
 
+// 16-bit decode with the keys as the matrix rows of the tensor cores (decode_keys.cu), for up to
+// kKeysMaxSeqs sequences: the window decode, or the sequences' own keys behind a shared prefix (rest).
+enum KeysMode { kKeysWindow = 0, kKeysRest = 1 };
+constexpr int kKeysMaxSeqs = 2048;
+constexpr int kKeysCols = 16;  // heads of a unit at most
+struct KeysPlan {
+  int grid;
+  size_t off_cut_o, off_cut_l, off_full_o, off_full_l;  // the merge's table at 0
+  size_t ws_bytes;
+};
+KeysPlan plan_keys(int num_seqs, int n_heads, int head_dim, int mode, int num_sms);
+cudaError_t launch_keys_decode(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
+                               int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
+                               int max_blocks_per_seq, const int32_t* kv_lens, int kv_cap, const DecodeExtra& ex,
+                               int mode, int dtype, const KeysPlan& plan, const QOLayout& lay, void* workspace,
+                               bool dependent, int* err, cudaStream_t stream);
+
 // Decode of sequences that share prefixes by groups (shared_prefix.cu): every group's prefix
 // is attended once for all its sequences (on the tensor cores for 16-bit types,
 // shared_prefix_tc.cu), every sequence's own keys by the split-KV kernel, and the partials
@@ -196,7 +201,9 @@ struct SharedPrefixPlan {
   int keys_per_split;  // of a prefix; 0 = no prefix to share
   int prefix_splits;   // prefix partials per (sequence, head)
   bool single_tiles;   // tensor cores: items of one query tile (small groups) instead of two
-  int target_items;    // page ranges the sequences' own keys are cut into, at most + num_seqs
+  bool keys;           // the sequences' own keys by decode_keys.cu, its workspace (kp) at 0
+  KeysPlan kp;
+  int target_items;    // else: page ranges they are cut into, at most + num_seqs
   int max_items;
   size_t off_spans, off_po, off_pl, off_ro, off_rl;  // items at 0, spans, prefix and rest partials
   size_t ws_bytes;

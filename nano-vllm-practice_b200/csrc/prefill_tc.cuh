@@ -136,17 +136,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
   using C = Cfg<D>;
   constexpr int TOK = kTileM / NREP;  // query tokens per tile
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
-  if constexpr (MODE == kTcPrefix) {
-    // Launched as a programmatic dependent of the plan kernel of the sequences' own keys, which
-    // nothing here reads.  One idle warp waits for it before it lets the next kernel start, so
-    // that kernel may read the plan without a wait of its own.
-    if ((threadIdx.x >> 5) == 3) {
-      grid_dependency_wait();
-      launch_dependents();
-    }
-  } else {
-    launch_dependents();  // decode mode: the split combine may start once every CTA is resident
-  }
+  // decode mode: the split combine may start once every CTA is resident (prefix mode: the kernel of the
+  // sequences' own keys)
+  launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
@@ -745,20 +737,12 @@ cudaError_t launch_tc(const void* q, void* out, const void* k_pool, const void* 
   if (ce != cudaSuccess) return ce;
   const int64_t ctas = plan.max_tiles * n_kv_heads * chunks * (tiles_per_split > 0 ? max_splits : 1);
   if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = MODE == kTcPrefix ? 1 : 0;
-  ce = cudaLaunchKernelEx(&cfg, kern, qmap, kmap, vmap, static_cast<T*>(out), q_len_flatten, num_seqs, n_kv_heads,
-                          num_blocks, cu_seqlens, order, cu_items, block_tables, max_blocks_per_seq, kv_lens, kv_cap,
-                          positions, lay, group, chunks, tiles_per_split, max_splits, ws_o, ws_lse, ex, err);
-  return ce != cudaSuccess ? ce : cudaGetLastError();
+  kern<<<unsigned(ctas), kThreads, C::kSmemBytes, stream>>>(qmap, kmap, vmap, static_cast<T*>(out), q_len_flatten,
+                                                            num_seqs, n_kv_heads, num_blocks, cu_seqlens, order,
+                                                            cu_items, block_tables, max_blocks_per_seq, kv_lens,
+                                                            kv_cap, positions, lay, group, chunks, tiles_per_split,
+                                                            max_splits, ws_o, ws_lse, ex, err);
+  return cudaGetLastError();
 }
 
 }  // namespace

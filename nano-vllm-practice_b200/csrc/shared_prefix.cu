@@ -6,18 +6,23 @@
 // keys: with (o_i, lse_i) of disjoint key ranges i, o = sum_i 2^(lse_i - m) o_i / sum_i
 // 2^(lse_i - m), m = max lse_i.  Here the prefix of a group is one range (or a few) that
 // all its sequences attend together, so its K and V leave HBM once per group and feed
-// 128-row tensor-core tiles of (sequence, query head) rows; the keys behind it are
-// attended per sequence by the split-KV kernel, bound by HBM.  Four launches:
+// 128-row tensor-core tiles of (sequence, query head) rows; the keys behind it are attended
+// per sequence, bound by HBM.  16-bit types, up to kKeysMaxSeqs sequences, three launches:
+//
+//   prefix   prefill_tc.cuh (kTcPrefix);
+//   rest     decode_keys.cu: the sequences' own tiles dealt evenly to one CTA per SM;
+//            starts as the prefix's CTAs leave their SMs (programmatic dependent launch);
+//   merge    one or four warps per (sequence, query head).
+//
+// fp32 and larger batches, four launches:
 //
 //   plan     one CTA: cuts the sequences' own pages into about target_items ranges of equal
 //            length, whatever their lengths are (a grid of max_splits x sequences would be
 //            mostly empty CTAs here, since the longest context bounds what every sequence
 //            may hold behind its prefix);
-//   prefix   prefill_tc.cuh (kTcPrefix), fp32: decode_split.cuh (kDecodePrefix); it reads
-//            nothing of the plan and starts beside it (programmatic dependent launch);
-//   rest     decode_split.cuh (kDecodeRest), one CTA per (range, kv head): starts as soon as
-//            the prefix's CTAs are placed and fills the SMs they leave;
-//   merge    one or four warps per (sequence, query head).
+//   prefix   fp32: decode_split.cuh (kDecodePrefix), else as above;
+//   rest     decode_split.cuh (kDecodeRest), one CTA per (range, kv head);
+//   merge    as above.
 #include "decode_split.cuh"
 
 namespace fvb {
@@ -113,14 +118,18 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const int32_t
 constexpr int kMergeThreads = 128;
 constexpr int kInFlight = 4;
 
-template <typename T, int D, int WARPS>
-__global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const float* __restrict__ po,
-                                                                     const float* __restrict__ pl,
-                                                                     const float* __restrict__ ro,
-                                                                     const float* __restrict__ rl,
-                                                                     const int4* __restrict__ spans,
-                                                                     T* __restrict__ out, int num_seqs, int n_heads,
-                                                                     int prefix_slots, const QOLayout lay) {
+// Where a row's partials are.  KEYS: decode_keys.cu's (whole units by row, cut ones by CTA); else the ranges'.
+struct MergeArgs {
+  const float *po, *pl;  // prefix: [row][prefix_slots]
+  const float *ro, *rl;  // ranges: [range][head]
+  const int4* spans;
+  const float *full_o, *full_l, *cut_o, *cut_l;
+  int num_seqs, n_heads, prefix_slots, keys_per_split, group, units, grid;
+};
+
+template <typename T, int D, int WARPS, bool KEYS>
+__global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const MergeArgs a, T* __restrict__ out,
+                                                                     const QOLayout lay) {
   constexpr int kDims = D / 32;
   constexpr int kRows = kMergeThreads / 32 / WARPS;
   __shared__ float sh_acc[WARPS > 1 ? WARPS : 1][WARPS > 1 ? D : 1];
@@ -128,10 +137,28 @@ __global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const float
   grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t row = int64_t(blockIdx.x) * kRows + (WARPS > 1 ? 0 : warp);  // (sequence, head), head fastest
-  if (row >= int64_t(num_seqs) * n_heads) return;
-  const int b = int(row / n_heads), head = int(row % n_heads);
-  const int4 span = __ldcg(spans + b);
-  const int n = span.x + span.z, w = WARPS > 1 ? warp : 0;
+  if (row >= int64_t(a.num_seqs) * a.n_heads) return;
+  const int b = int(row / a.n_heads), head = int(row % a.n_heads);
+  const int4 span = __ldcg(a.spans + b);
+  // prefix partials, then those of the sequence's own keys: own_n of them from own_0 on
+  int np = span.x, own_0 = span.y, own_n = span.z;
+  bool whole = false;
+  int column = 0;
+  if constexpr (KEYS) {
+    np = a.keys_per_split > 0 ? (span.x + a.keys_per_split - 1) / a.keys_per_split : 0;
+    const int in_group = head % a.group, chunks = (a.group + kKeysCols - 1) / kKeysCols;
+    const int unit = head / a.group * chunks + in_group / kKeysCols;
+    column = in_group % kKeysCols;
+    own_n = 0;
+    if (span.y > 0) {
+      const int64_t total = int64_t(span.w) * a.units, begin = int64_t(span.z) * a.units + int64_t(unit) * span.y;
+      const int grid = int(min(int64_t(a.grid), total));
+      own_0 = keys_cta_of(begin, total, grid);
+      own_n = keys_cta_of(begin + span.y - 1, total, grid) - own_0 + 1;
+      whole = own_n == 1;
+    }
+  }
+  const int n = np + own_n, w = WARPS > 1 ? warp : 0;
   float m = -INFINITY, l = 0.f, acc[kDims];
 #pragma unroll
   for (int d = 0; d < kDims; ++d) acc[d] = 0.f;
@@ -140,13 +167,20 @@ __global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const float
 #pragma unroll
     for (int u = 0; u < kInFlight; ++u) {
       const int i = i0 + u * WARPS;
-      const bool prefix = i < span.x;
-      const int64_t at = prefix ? row * prefix_slots + i : int64_t(span.y + i - span.x) * n_heads + head;
-      ls[u] = i < n ? __ldcg((prefix ? pl : rl) + at) : -INFINITY;
+      const bool prefix = i < np;
+      const int k = own_0 + i - np;
+      int64_t at = prefix ? row * a.prefix_slots + i : int64_t(k) * a.n_heads + head;
+      const float *po = prefix ? a.po : a.ro, *pl = prefix ? a.pl : a.rl;
+      if (KEYS && !prefix) {
+        at = whole ? row : (int64_t(k) * 2 + (k == own_0 ? 1 : 0)) * kKeysCols + column;
+        po = whole ? a.full_o : a.cut_o;
+        pl = whole ? a.full_l : a.cut_l;
+      }
+      ls[u] = i < n ? __ldcg(pl + at) : -INFINITY;
 #pragma unroll
       for (int d = 0; d < kDims; ++d) o[u][d] = 0.f;
       if (i < n) {
-        const float* src = (prefix ? po : ro) + at * D + lane * kDims;
+        const float* src = po + at * D + lane * kDims;
         if constexpr (kDims == 4) {
           const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
           o[u][0] = v.x, o[u][1] = v.y, o[u][2] = v.z, o[u][3] = v.w;
@@ -225,7 +259,7 @@ struct SharedArgs {
   SharedPrefixPlan plan;
   QOLayout lay;
   float *po, *pl, *ro, *rl;
-  const int4* spans;
+  void* ws;
   DecodeExtra ex;
   int* err;
   cudaStream_t stream;
@@ -268,28 +302,32 @@ cudaError_t launch_split(const SharedArgs& a, dim3 grid, int pages_per_split, in
 template <typename T, int D, int NREP>
 cudaError_t launch_rest(const SharedArgs& a) {
   const int chunks = (a.n_heads / a.n_kv_heads + NREP - 1) / NREP;
-  // A dependent of the prefix kernel, which waits for the plan; without one an ordinary launch.
+  // A dependent of the prefix kernel, which starts behind the plan; without one an ordinary launch.
   return launch_split<T, D, NREP, kDecodeRest>(a, dim3(a.plan.max_items, a.n_kv_heads * chunks), 0, 1, a.ro, a.rl,
                                                a.plan.keys_per_split > 0);
 }
 
-template <typename T, int D, int WARPS>
-cudaError_t launch_merge(const SharedArgs& a) {
+template <typename T, int D, int WARPS, bool KEYS>
+cudaError_t launch_merge(const SharedArgs& a, const MergeArgs& m) {
   constexpr int kRows = kMergeThreads / 32 / WARPS;
   const int64_t ctas = (int64_t(a.num_seqs) * a.n_heads + kRows - 1) / kRows;
   if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = config(dim3(unsigned(ctas)), kMergeThreads, 0, a.stream, attr);
-  return cudaLaunchKernelEx(&cfg, shared_merge_kernel<T, D, WARPS>, static_cast<const float*>(a.po),
-                            static_cast<const float*>(a.pl), static_cast<const float*>(a.ro),
-                            static_cast<const float*>(a.rl), a.spans, static_cast<T*>(a.out), a.num_seqs, a.n_heads,
-                            a.plan.prefix_splits, a.lay);
+  return cudaLaunchKernelEx(&cfg, shared_merge_kernel<T, D, WARPS, KEYS>, m, static_cast<T*>(a.out), a.lay);
 }
 
 template <typename T, int D>
-cudaError_t run(const SharedArgs& a, int head_dim, int dtype) {
+cudaError_t run(const SharedArgs& a, const MergeArgs& m, int head_dim, int dtype) {
   const int group = a.n_heads / a.n_kv_heads;
   cudaError_t ce = cudaSuccess;
+  if (!a.plan.keys) {
+    shared_plan_kernel<<<1, kPlanThreads, 0, a.stream>>>(
+        a.kv_lens, a.kv_cap, a.num_seqs, a.plan.keys_per_split, a.plan.target_items, a.plan.max_items, a.ex,
+        const_cast<int4*>(a.ex.items), const_cast<int4*>(m.spans), a.err);
+    ce = cudaGetLastError();
+    if (ce != cudaSuccess) return ce;
+  }
   if (a.plan.keys_per_split > 0) {
     if constexpr (sizeof(T) == 4) {
       // Rows are (sequence, head) pairs of a group, eight a CTA.
@@ -305,23 +343,32 @@ cudaError_t run(const SharedArgs& a, int head_dim, int dtype) {
     }
     if (ce != cudaSuccess) return ce;
   }
-  switch (decode_tile_heads(group)) {
-    case 1:
-      ce = launch_rest<T, D, 1>(a);
-      break;
-    case 2:
-      ce = launch_rest<T, D, 2>(a);
-      break;
-    case 4:
-      ce = launch_rest<T, D, 4>(a);
-      break;
-    default:
-      ce = launch_rest<T, D, 8>(a);
+  if (a.plan.keys) {
+    ce = launch_keys_decode(a.q, a.out, a.k_pool, a.v_pool, a.num_blocks, a.n_heads, a.n_kv_heads, head_dim,
+                            a.num_seqs, a.block_tables, a.max_blocks_per_seq, a.kv_lens, a.kv_cap, a.ex, kKeysRest,
+                            dtype, a.plan.kp, a.lay, a.ws, a.plan.keys_per_split > 0, a.err, a.stream);
+  } else {
+    switch (decode_tile_heads(group)) {
+      case 1:
+        ce = launch_rest<T, D, 1>(a);
+        break;
+      case 2:
+        ce = launch_rest<T, D, 2>(a);
+        break;
+      case 4:
+        ce = launch_rest<T, D, 4>(a);
+        break;
+      default:
+        ce = launch_rest<T, D, 8>(a);
+    }
   }
   if (ce != cudaSuccess) return ce;
-  // Partials a row merges on average: prefix splits and its share of the ranges.
-  const int64_t partials = a.plan.prefix_splits + a.plan.max_items / a.num_seqs;
-  ce = partials > 8 ? launch_merge<T, D, 4>(a) : launch_merge<T, D, 1>(a);
+  // Partials a row merges on average: prefix splits and its share of the ranges (of the CTAs).
+  const int64_t own = a.plan.keys ? int64_t(a.plan.kp.grid) / (int64_t(a.num_seqs) * m.units) + 1
+                                  : a.plan.max_items / a.num_seqs;
+  const bool many = a.plan.prefix_splits + own > 8;
+  if (a.plan.keys) ce = many ? launch_merge<T, D, 4, true>(a, m) : launch_merge<T, D, 1, true>(a, m);
+  else ce = many ? launch_merge<T, D, 4, false>(a, m) : launch_merge<T, D, 1, false>(a, m);
   return ce != cudaSuccess ? ce : cudaGetLastError();
 }
 
@@ -352,20 +399,26 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     p.keys_per_split = per * unit;
     p.prefix_splits = (prefix + p.keys_per_split - 1) / p.keys_per_split;
   }
-  // About four waves of three resident split-KV CTAs per SM, as plan_decode.
-  const int tile_heads = decode_tile_heads(group);
-  const int units = n_kv_heads * ((group + tile_heads - 1) / tile_heads);
-  p.target_items = std::max(1, (num_sms * 12 + units - 1) / units);
-  p.max_items = p.target_items + num_seqs;
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   const size_t rows = size_t(num_seqs) * n_heads * p.prefix_splits;
-  const size_t rest = size_t(p.max_items) * n_heads;
-  p.off_spans = up(size_t(p.max_items) * 16);
-  p.off_po = p.off_spans + up(size_t(num_seqs) * 16);
+  p.keys = dtype != FVB_DTYPE_F32 && num_seqs <= kKeysMaxSeqs;
+  if (p.keys) {
+    p.kp = plan_keys(num_seqs, n_heads, head_dim, kKeysRest, num_sms);
+    p.off_po = up(p.kp.ws_bytes);
+  } else {
+    // About four waves of three resident split-KV CTAs per SM, as plan_decode.
+    const int tile_heads = decode_tile_heads(group);
+    const int units = n_kv_heads * ((group + tile_heads - 1) / tile_heads);
+    p.target_items = std::max(1, (num_sms * 12 + units - 1) / units);
+    p.max_items = p.target_items + num_seqs;
+    const size_t rest = size_t(p.max_items) * n_heads;
+    p.off_spans = up(size_t(p.max_items) * 16);
+    p.off_ro = p.off_spans + up(size_t(num_seqs) * 16);
+    p.off_rl = p.off_ro + up(rest * head_dim * 4);
+    p.off_po = p.off_rl + up(rest * 4);
+  }
   p.off_pl = p.off_po + up(rows * head_dim * 4);
-  p.off_ro = p.off_pl + up(rows * 4);
-  p.off_rl = p.off_ro + up(rest * head_dim * 4);
-  p.ws_bytes = p.off_rl + up(rest * 4);
+  p.ws_bytes = p.off_pl + up(rows * 4);
   return p;
 }
 
@@ -396,7 +449,7 @@ cudaError_t launch_shared_prefix(const void* q, void* out, const void* k_pool, c
   a.pl = reinterpret_cast<float*>(ws + plan.off_pl);
   a.ro = reinterpret_cast<float*>(ws + plan.off_ro);
   a.rl = reinterpret_cast<float*>(ws + plan.off_rl);
-  a.spans = reinterpret_cast<const int4*>(ws + plan.off_spans);
+  a.ws = ws;
   a.ex.cu_groups = cu_groups;
   a.ex.prefix_lens = prefix_lens;
   a.ex.num_groups = num_groups;
@@ -405,17 +458,30 @@ cudaError_t launch_shared_prefix(const void* q, void* out, const void* k_pool, c
   a.ex.items = reinterpret_cast<const int4*>(ws);
   a.err = err;
   a.stream = stream;
-  shared_plan_kernel<<<1, kPlanThreads, 0, stream>>>(kv_lens, a.kv_cap, num_seqs, plan.keys_per_split,
-                                                     plan.target_items, plan.max_items, a.ex,
-                                                     reinterpret_cast<int4*>(ws),
-                                                     reinterpret_cast<int4*>(ws + plan.off_spans), err);
-  cudaError_t ce = cudaGetLastError();
-  if (ce != cudaSuccess) return ce;
+  MergeArgs m{};
+  m.po = a.po;
+  m.pl = a.pl;
+  m.ro = a.ro;
+  m.rl = a.rl;
+  m.spans = reinterpret_cast<const int4*>(ws + plan.off_spans);  // (keys: at 0)
+  m.num_seqs = num_seqs;
+  m.n_heads = n_heads;
+  m.prefix_slots = plan.prefix_splits;
+  m.keys_per_split = plan.keys_per_split;
+  m.group = n_heads / n_kv_heads;
+  if (plan.keys) {
+    m.full_o = reinterpret_cast<const float*>(ws + plan.kp.off_full_o);
+    m.full_l = reinterpret_cast<const float*>(ws + plan.kp.off_full_l);
+    m.cut_o = reinterpret_cast<const float*>(ws + plan.kp.off_cut_o);
+    m.cut_l = reinterpret_cast<const float*>(ws + plan.kp.off_cut_l);
+    m.units = n_kv_heads * ((m.group + kKeysCols - 1) / kKeysCols);
+    m.grid = plan.kp.grid;
+  }
   if (dtype == FVB_DTYPE_BF16)
-    return head_dim == 128 ? run<__nv_bfloat16, 128>(a, head_dim, dtype) : run<__nv_bfloat16, 64>(a, head_dim, dtype);
+    return head_dim == 128 ? run<__nv_bfloat16, 128>(a, m, head_dim, dtype) : run<__nv_bfloat16, 64>(a, m, head_dim, dtype);
   if (dtype == FVB_DTYPE_F16)
-    return head_dim == 128 ? run<__half, 128>(a, head_dim, dtype) : run<__half, 64>(a, head_dim, dtype);
-  return head_dim == 128 ? run<float, 128>(a, head_dim, dtype) : run<float, 64>(a, head_dim, dtype);
+    return head_dim == 128 ? run<__half, 128>(a, m, head_dim, dtype) : run<__half, 64>(a, m, head_dim, dtype);
+  return head_dim == 128 ? run<float, 128>(a, m, head_dim, dtype) : run<float, 64>(a, m, head_dim, dtype);
 }
 
 }  // namespace fvb

@@ -57,6 +57,7 @@ CU_SOURCES = [
     "beam_search.cu",
     "beam_reorder.cu",
     "decode.cu",
+    "decode_keys.cu",
     "decode_window.cu",
     "decode_noalloc.cu",
     "prefill_simt.cu",
