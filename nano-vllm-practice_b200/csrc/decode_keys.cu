@@ -60,8 +60,10 @@ struct Cfg {
   // k_full, k_empty, v_full, v_empty [kStages]; s_full, p_full, pv_done, q_full, q_empty, o_empty [2]
   static constexpr int kNumBars = 4 * kStages + 12;
   static constexpr int kOffRed = kOffBar + kNumBars * 8 + 16;   // float[4][kCols]
-  static constexpr int kOffSeqs = kOffRed + 4 * kCols * 4;      // int[num_seqs + 1] tiles before, int[num_seqs] skip
-  static_assert(kOffSeqs + (2 * kKeysMaxSeqs + 1) * 4 + 1024 <= 227 * 1024, "shared memory budget");
+  // int[num_seqs + 1] tiles before each sequence, int[num_seqs] its length, int[num_seqs] keys skipped (rest)
+  static constexpr int kOffSeqs = kOffRed + 4 * kCols * 4;
+  static constexpr int smem_bytes(int num_seqs) { return kOffSeqs + (3 * num_seqs + 1) * 4 + 1024; }
+  static_assert(smem_bytes(kKeysMaxSeqs) <= 227 * 1024, "shared memory budget");
 };
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int site) {
@@ -168,7 +170,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
   float* red = reinterpret_cast<float*>(smem + C::kOffRed);
   int32_t* cum = reinterpret_cast<int32_t*>(smem + C::kOffSeqs);
-  int32_t* skips = cum + a.num_seqs + 1;
+  int32_t* lens = cum + a.num_seqs + 1;
+  int32_t* skips = lens + a.num_seqs;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_heads = a.n_kv_heads * a.group;
   const int units = a.n_kv_heads * a.chunks;
@@ -197,7 +200,6 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
   }
 
   // ---- tiles of every sequence, and their running sum ----
-  auto seq_len = [&](int b) { return min(max(__ldg(a.kv_lens + b), 0), a.kv_cap); };
   {
     int32_t* warp_sum = reinterpret_cast<int32_t*>(red);
     int carry = 0;
@@ -219,8 +221,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
           }
           skips[b] = skip;
         }
-        if (blockIdx.x == 0 && __ldg(a.kv_lens + b) > a.kv_cap) record_error(a.err, FVB_ERR_INVALID_ARGUMENT, b);
-        n = (unit_span<MODE>(a, seq_len(b), skip).count + kTilePages - 1) / kTilePages;
+        const int kv = __ldg(a.kv_lens + b);
+        if (blockIdx.x == 0 && kv > a.kv_cap) record_error(a.err, FVB_ERR_INVALID_ARGUMENT, b);
+        lens[b] = min(max(kv, 0), a.kv_cap);
+        n = (unit_span<MODE>(a, lens[b], skip).count + kTilePages - 1) / kTilePages;
       }
       int upto = n;
 #pragma unroll
@@ -287,47 +291,56 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
       uint64_t* empty = warp == 0 ? k_empty : v_empty;
       uint8_t* ring = smem + (warp == 0 ? C::kOffK : C::kOffV);
       if (lane == 0) prefetch_tensormap(map);
-      // Row of this lane's page (lanes 0 .. 7) of tile t in the pool, -1: none.
+      // Page id of this lane's page (lanes 0 .. 7) of tile t, -1 past the unit; read one tile ahead and looked
+      // at only when its turn comes.
       KeySpan span{};
       int span_of = -1;
-      auto page_row = [&](const Walk& w, int t) {
+      auto page_id = [&](const Walk& w, int t, bool& in) {
         if (w.b != span_of) {
           span_of = w.b;
-          span = unit_span<MODE>(a, seq_len(w.b), MODE == kKeysRest ? skips[w.b] : 0);
+          span = unit_span<MODE>(a, lens[w.b], MODE == kKeysRest ? skips[w.b] : 0);
         }
         const int c = t * kTilePages + lane;
-        if (lane >= kTilePages || c >= span.count) return -1;
-        int blk = __ldg(a.block_tables + int64_t(w.b) * a.max_blocks_per_seq + (c < span.head ? c : c + span.gap));
-        if (blk < 0 || blk >= a.num_blocks) {
-          record_error(a.err, FVB_ERR_BAD_PAGE, w.b);
-          blk = 0;
-        }
-        return (blk * a.n_kv_heads + w.u / a.chunks) * kPageSize;
+        in = lane < kTilePages && c < span.count;
+        return in ? __ldg(a.block_tables + int64_t(w.b) * a.max_blocks_per_seq + (c < span.head ? c : c + span.gap)) : 0;
       };
-      int row = page_row(walk, walk.t0);
+      bool in = false;
+      int id = page_id(walk, walk.t0, in);
       int j = 0;
       bool ok = true;
       for (; walk.more() && ok; walk.next()) {
+        const int kvh = walk.u / a.chunks;
         for (int t = walk.t0; t < walk.t1; ++t, ++j) {
-          const int now = row;
-          // the next tile's page ids, in flight while this one waits for its slot
-          if (t + 1 < walk.t1) {
-            row = page_row(walk, t + 1);
-          } else {
-            Walk ahead = walk;
-            ahead.next();
-            if (ahead.more()) row = page_row(ahead, ahead.t0);
-          }
           const int st = j % kS;
           if (j >= kS) ok = warp_wait(&empty[st], (j / kS - 1) & 1, a.err, 0x400 + warp);
           if (!ok) break;
-          const int pages = __popc(__ballot_sync(0xffffffffu, now >= 0));
-          if (lane == 0) mbar_arrive_expect_tx(&full[st], uint32_t(pages) * kPageSize * D * 2);
-          __syncwarp();
-          if (now >= 0) {
+          if (in && (id < 0 || id >= a.num_blocks)) {
+            record_error(a.err, FVB_ERR_BAD_PAGE, walk.b);
+            id = 0;
+          }
+          const int now = (id * a.n_kv_heads + kvh) * kPageSize;
+          const int pages = __popc(__ballot_sync(0xffffffffu, in));
+          int rows[kTilePages];
 #pragma unroll
-            for (int h = 0; h < C::kHalves; ++h)
-              tma_load_2d(ring + st * C::kTileBytes + h * kHalf + lane * kPageSize * 128, map, h * 64, now, &full[st]);
+          for (int i = 0; i < kTilePages; ++i) rows[i] = __shfl_sync(0xffffffffu, now, i);
+          if (t + 1 < walk.t1) {
+            id = page_id(walk, t + 1, in);
+          } else {
+            Walk ahead = walk;
+            ahead.next();
+            if (ahead.more()) id = page_id(ahead, ahead.t0, in);
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&full[st], uint32_t(pages) * kPageSize * D * 2);
+            uint8_t* dst = ring + st * C::kTileBytes;
+#pragma unroll
+            for (int i = 0; i < kTilePages; ++i) {
+              if (i < pages) {  // a tile's pages are its first ones
+#pragma unroll
+                for (int h = 0; h < C::kHalves; ++h)
+                  tma_load_2d(dst + h * kHalf + i * kPageSize * 128, map, h * 64, rows[i], &full[st]);
+              }
+            }
           }
           __syncwarp();
         }
@@ -421,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
         const int b = walk.b;
         const int kvh = walk.u / a.chunks, chunk = walk.u % a.chunks;
         const int head0 = kvh * a.group + chunk * kCols, nvh = min(kCols, a.group - chunk * kCols);
-        const int kv_len = seq_len(b);
+        const int kv_len = lens[b];
         const KeySpan span = unit_span<MODE>(a, kv_len, MODE == kKeysRest ? skips[b] : 0);
         float m[HV], l[HV];
 #pragma unroll
@@ -622,13 +635,12 @@ cudaError_t launch_t(const KeysArgs& a, const void* k_pool, const void* v_pool, 
   const uint64_t rows = uint64_t(a.num_blocks) * a.n_kv_heads * kPageSize;
   cudaError_t ce = make_tma_2d(&kmap, k_pool, tdt, D, rows, D * 2, 64, kPageSize, true);
   if (ce == cudaSuccess) ce = make_tma_2d(&vmap, v_pool, tdt, D, rows, D * 2, 64, kPageSize, true);
-  constexpr int kMaxSmem = C::kOffSeqs + (2 * kKeysMaxSeqs + 1) * 4 + 1024;
-  if (ce == cudaSuccess) ce = set_smem_once<decode_keys_kernel<T, D, HV, MODE>>(kMaxSmem);
+  if (ce == cudaSuccess) ce = set_smem_once<decode_keys_kernel<T, D, HV, MODE>>(C::smem_bytes(kKeysMaxSeqs));
   if (ce != cudaSuccess) return ce;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kOffSeqs + (2 * a.num_seqs + 1) * 4 + 1024;
+  cfg.dynamicSmemBytes = C::smem_bytes(a.num_seqs);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

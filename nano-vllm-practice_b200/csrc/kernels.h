@@ -179,7 +179,7 @@ cudaError_t launch_window_prefill_simt(const void* q, void* out, const void* k_p
 // 16-bit decode with the keys as the matrix rows of the tensor cores (decode_keys.cu), for up to
 // kKeysMaxSeqs sequences: the window decode, or the sequences' own keys behind a shared prefix (rest).
 enum KeysMode { kKeysWindow = 0, kKeysRest = 1 };
-constexpr int kKeysMaxSeqs = 2048;
+constexpr int kKeysMaxSeqs = 1024;
 constexpr int kKeysCols = 16;  // heads of a unit at most
 struct KeysPlan {
   int grid;
