@@ -71,6 +71,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, ok);
 }
 
+// Maximum over the warp in one instruction (sm_100).
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
@@ -430,13 +437,66 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
       // failed goes on without waiting or touching TMEM, and the others fail or finish in their own time.
       bool ok = true;
       int j = 0;
+      // The unit whose last P V is under way: its result is taken when the next unit's first P is out, so that
+      // product never holds up the softmax.
+      struct Done {
+        int item, tile, head0, nvh, b;
+        int64_t at;      // partial's row, or -1: the unit goes to `out`
+        float *o, *l;
+      } done{};
+      done.item = -1;
+      float m[HV], l[HV], m_done[HV], l_done[HV];
+      auto finish = [&]() {
+        // Sums over the 128 keys: lanes trade halves of the heads until each holds one, then warps meet in `red`.
+        float s[HV];
+#pragma unroll
+        for (int h = 0; h < HV; ++h) s[h] = l_done[h];
+        int mine = 0;
+#pragma unroll
+        for (int n = HV / 2, o = 16; n >= 1; n /= 2, o /= 2) {
+          const bool upper = lane & o;
+#pragma unroll
+          for (int h = 0; h < n; ++h) {
+            const float give = upper ? s[h] : s[h + n], keep = upper ? s[h + n] : s[h];
+            s[h] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+          mine += upper ? n : 0;
+        }
+#pragma unroll
+        for (int o = 16 / HV; o > 0; o >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+        if (lane % (32 / HV) == 0) red[(warp & 3) * kCols + mine] = s[0];
+        named_barrier(1, kKeys);
+        ok = ok && warp_wait(&pv_done[done.tile & 1], (done.tile >> 1) & 1, a.err, 0x434);
+        uint32_t o[16] = {};
+        if (ok) {
+          tc_fence_after();
+          tmem_ld_16cols(col_o(done.item) + t_row, o);
+          tc_fence_before();
+        }
+        mbar_arrive(&o_empty[done.item & 1]);
+        // thread = head dim
+#pragma unroll
+        for (int h = 0; h < HV; ++h) {
+          const float L = (red[h] + red[kCols + h]) + (red[2 * kCols + h] + red[3 * kCols + h]);
+          const float v = __uint_as_float(o[h]) / L;
+          if (h >= done.nvh || key_t >= D) continue;
+          if (MODE == kKeysWindow && done.at < 0) {
+            static_cast<T*>(a.out)[int64_t(done.b) * a.lay.o_ts + int64_t(done.head0 + h) * a.lay.o_hs + key_t] =
+                Elem<T>::from_f(v);
+          } else {
+            done.o[(done.at + h) * D + key_t] = v;
+            if (key_t == 0) done.l[done.at + h] = m_done[h] + __log2f(L);
+          }
+        }
+        named_barrier(1, kKeys);  // red is read before its next use
+        done.item = -1;
+      };
       for (int item = 0; walk.more(); walk.next(), ++item) {
         const int b = walk.b;
         const int kvh = walk.u / a.chunks, chunk = walk.u % a.chunks;
         const int head0 = kvh * a.group + chunk * kCols, nvh = min(kCols, a.group - chunk * kCols);
         const int kv_len = lens[b];
         const KeySpan span = unit_span<MODE>(a, kv_len, MODE == kKeysRest ? skips[b] : 0);
-        float m[HV], l[HV];
 #pragma unroll
         for (int h = 0; h < HV; ++h) {
           m[h] = -INFINITY;
@@ -463,14 +523,12 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
             x[h] = valid && ok ? __uint_as_float(sr[h]) * scale : -INFINITY;
             if (h < nvh) grow = grow || x[h] > m[h] + kGrowLog2;
           }
-          if (named_barrier_or(1, kKeys, grow)) {
+          if (t == walk.t0 || named_barrier_or(1, kKeys, grow)) {
             // New reference maxima: those of the tile where they exceed the old by more than 2^8 (at the
             // unit's first tile always; a tile holds a visible key).
 #pragma unroll
             for (int h = 0; h < HV; ++h) {
-              float mx = x[h];
-#pragma unroll
-              for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              const float mx = warp_max(x[h]);
               if (lane == 0) red[(warp & 3) * kCols + h] = mx;
             }
             named_barrier(1, kKeys);
@@ -495,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
               tmem_st_16cols(col_o(item) + t_row, o);
               tmem_wait_st();
             }
-            named_barrier(1, kKeys);  // red is read before the next use
+            named_barrier(1, kKeys);  // red is read before its next use
           }
           // P of tile j - 2 has been read
           if (j >= 2) ok = ok && warp_wait(&pv_done[j & 1], ((j >> 1) - 1) & 1, a.err, 0x432);
@@ -526,42 +584,30 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
           fence_proxy_async_smem();
           tc_fence_before();
           mbar_arrive(&p_full[j & 1]);
+          if (done.item >= 0) finish();
         }
-        // ---- the unit's (or its part's) O / l: thread = head dim ----
-#pragma unroll
-        for (int h = 0; h < HV; ++h) {
-          float s = l[h];
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if (lane == 0) red[(warp & 3) * kCols + h] = s;
-        }
-        named_barrier(1, kKeys);
-        ok = ok && warp_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, a.err, 0x434);
-        uint32_t o[16] = {};
-        if (ok) {
-          tc_fence_after();
-          tmem_ld_16cols(col_o(item) + t_row, o);
-          tc_fence_before();
-        }
-        mbar_arrive(&o_empty[item & 1]);
         const bool whole = walk.t0 == 0 && walk.t1 == walk.n;
-        const int slot = int(blockIdx.x) * 2 + (walk.t0 > 0 ? 0 : 1);
+        done.item = item;
+        done.tile = j - 1;
+        done.head0 = head0;
+        done.nvh = nvh;
+        done.b = b;
+        if (whole) {
+          done.at = MODE == kKeysWindow ? -1 : int64_t(b) * n_heads + head0;
+          done.o = a.full_o;
+          done.l = a.full_l;
+        } else {
+          done.at = (int64_t(blockIdx.x) * 2 + (walk.t0 > 0 ? 0 : 1)) * kCols;
+          done.o = a.cut_o;
+          done.l = a.cut_l;
+        }
 #pragma unroll
         for (int h = 0; h < HV; ++h) {
-          const float L = (red[h] + red[kCols + h]) + (red[2 * kCols + h] + red[3 * kCols + h]);
-          const float v = __uint_as_float(o[h]) / L;
-          if (h >= nvh || key_t >= D) continue;
-          const int head = head0 + h;
-          if (MODE == kKeysWindow && whole) {
-            static_cast<T*>(a.out)[int64_t(b) * a.lay.o_ts + int64_t(head) * a.lay.o_hs + key_t] = Elem<T>::from_f(v);
-            continue;
-          }
-          const int64_t at = whole ? int64_t(b) * n_heads + head : int64_t(slot) * kCols + h;
-          (whole ? a.full_o : a.cut_o)[at * D + key_t] = v;
-          if (key_t == 0) (whole ? a.full_l : a.cut_l)[at] = m[h] + __log2f(L);
+          m_done[h] = m[h];
+          l_done[h] = l[h];
         }
-        named_barrier(1, kKeys);  // red is read before the next unit's use
       }
+      if (done.item >= 0) finish();
     }
   }
   tc_fence_before();

@@ -113,9 +113,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
 
 // Which keys a launch's queries see (compile time; the plain form carries none of the rest):
 //   plain    the causal prefix of each query;
-//   window   of that the last ex.window keys and the first ex.sinks: the KV tiles that hold
-//            a visible key of the item are numbered without the gap between sinks and window,
-//            and inside a tile only the pages that hold one are loaded;
+//   window   of that the last ex.window keys and the first ex.sinks: the pages that hold a
+//            visible key of the item are numbered without the gap between sinks and window,
+//            and the KV tiles are eight of those each, so a few sinks cost a page, not a tile;
+//            keys are then counted in these pages ("columns");
 //   prefix   the prefix shared by a group of sequences, one query each: "sequence" g of the
 //            plain form is group g, its query tokens the group's sequences, its pages those of
 //            the group's first sequence, and query i sees keys below min(kv_lens[i], prefix).
@@ -230,22 +231,29 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
     p_last[i] = (live && kv_len > 0) ? max(min(p_tok, kv_len - 1), 0) : -1;
     nkv[i] = p_last[i] >= 0 ? p_last[i] / kTileN + 1 : 0;
   }
-  // KV tile c of the item's list is tile c of the context for c < span.head, c + span.gap behind.
+  // Window mode: page c of the item is table page c for c < span.head, c + span.gap behind; `column` of a key.
   KeySpan span{0, 0, 0, 0};
-  int sink_pages = 0;
+  auto column = [&](int key) {
+    const int head = span.head * kPageSize, gap = span.gap * kPageSize;
+    return key >= head + gap ? key - gap : min(key, head - 1);
+  };
   if constexpr (MODE == kTcWindow) {
     const int last = max(p_last[0], p_last[1]);
     // positions ascend within a sequence
     const int first = positions ? min(max(__ldg(positions + t0[0]), 0), 0x7ffffffe) : last;
-    span = window_span(first + 1, last + 1, ex.window, ex.sinks, kTileN);
-    sink_pages = (min(ex.sinks, last + 1) + kPageSize - 1) / kPageSize;
+    span = window_span(first + 1, last + 1, ex.window, ex.sinks, kPageSize);
+    const int tiles = (span.count + kTileN / kPageSize - 1) / (kTileN / kPageSize);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) nkv[i] = min(nkv[i], span.head) + max(nkv[i] - span.head - span.gap, 0);
+    for (int i = 0; i < 2; ++i) nkv[i] = nkv[i] > 0 ? min(tiles, column(p_last[i]) / kTileN + 1) : 0;
   }
-  auto kv_tile = [&](int c) { return MODE == kTcWindow && c >= span.head ? c + span.gap : c; };
   int n_kv = max(nkv[0], nkv[1]);
-  const int pos_max = max(p_last[0], p_last[1]);  // last key visible to any row of the item
-  const int need_pages = pos_max / kPageSize + 1;  // pages holding every visible key
+  int pos_max = max(p_last[0], p_last[1]);  // last key visible to any row of the item
+  const int need_pages = MODE == kTcWindow ? span.count : pos_max / kPageSize + 1;  // pages holding every visible key
+  int lo_min = 0;  // window mode: first column of the earliest window (past every column: no window key exists)
+  if constexpr (MODE == kTcWindow) {
+    lo_min = span.lo > pos_max ? 0x7fffffff : column(span.lo);
+    pos_max = column(pos_max);
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (MODE == kTcPrefix && n_kv == 0) return;  // no shared page: the merge counts no partial
@@ -308,7 +316,67 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
   const int wg = threadIdx.x / kWgThreads;
 
   if (wg == 0) {
-    if ((warp == 0 || warp == 2) && lane == 0) {
+    if (MODE != kTcPlain && (warp == 0 || warp == 2)) {
+      // ======================= TMA producers: warp 0 = Q + K, warp 2 = V =======================
+      // As below, by the whole warp: eight lanes read the page ids of a tile while the one before it is
+      // issued, so neither their latency nor their check holds up the copies.
+      const bool is_k = warp == 0;
+      if (lane == 0) {
+        prefetch_tensormap(is_k ? &kmap : &vmap);
+        if (is_k) {
+          mbar_arrive_expect_tx(q_full, (has1 ? 2 : 1) * C::kQTileBytes);
+          for (int i = 0; i < (has1 ? 2 : 1); ++i) {
+#pragma unroll
+            for (int g = 0; g < NREP; ++g) {
+#pragma unroll
+              for (int h = 0; h < C::kHalves; ++h)
+                tma_load_3d(smem + C::kOffQ + i * C::kQTileBytes + h * kHalfBytes + g * TOK * 128, &qmap, h * 64, t0[i],
+                            head0 + min(g, nvh - 1), q_full);
+            }
+          }
+        }
+      }
+      constexpr int kPages = kTileN / kPageSize;
+      const int nst_ring = is_k ? C::kKStages : kVS;
+      uint64_t* full = is_k ? k_full : v_full;
+      uint64_t* empty = is_k ? k_empty : v_empty;
+      const CUtensorMap* map = is_k ? &kmap : &vmap;
+      const int32_t* table = block_tables + int64_t(MODE == kTcPrefix ? q_begin : s) * max_blocks_per_seq;
+      bool in = false;
+      auto page_id = [&](int j) {
+        const int c = (j0 + j) * kPages + lane;
+        in = lane < kPages && c < need_pages;
+        return in ? __ldg(table + (MODE == kTcWindow && c >= span.head ? c + span.gap : c)) : 0;
+      };
+      int id = page_id(0);
+      for (int j = 0; j < n_kv; ++j) {
+        const int st = j % nst_ring, use = j / nst_ring;
+        if (use > 0 && !warp_wait(&empty[st], (use - 1) & 1, err, is_k ? 0x300 : 0x301)) break;
+        if (in && (id < 0 || id >= num_blocks)) {
+          record_error(err, FVB_ERR_BAD_PAGE, s);
+          id = 0;
+        }
+        const int now = (id * n_kv_heads + kvh) * kPageSize;
+        const int np = __popc(__ballot_sync(0xffffffffu, in));
+        int rows[kPages];
+#pragma unroll
+        for (int i = 0; i < kPages; ++i) rows[i] = __shfl_sync(0xffffffffu, now, i);
+        if (j + 1 < n_kv) id = page_id(j + 1);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&full[st], uint32_t(np) * kPageSize * D * 2);
+          uint8_t* stage = smem + (is_k ? C::kOffK + st * C::kKVBytes : v_off(st));
+#pragma unroll
+          for (int i = 0; i < kPages; ++i) {
+            if (i < np) {
+#pragma unroll
+              for (int h = 0; h < C::kHalves; ++h)
+                tma_load_2d(stage + h * kHalfBytes + i * kPageSize * 128, map, h * 64, rows[i], &full[st]);
+            }
+          }
+        }
+        __syncwarp();
+      }
+    } else if (MODE == kTcPlain && (warp == 0 || warp == 2) && lane == 0) {
       // ======================= TMA producers: warp 0 = Q + K, warp 2 = V =======================
       const bool is_k = warp == 0;
       prefetch_tensormap(is_k ? &kmap : &vmap);
@@ -332,19 +400,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
       uint64_t* empty = is_k ? k_empty : v_empty;
       uint8_t* ring = smem + (is_k ? C::kOffK : C::kOffV);
       const CUtensorMap* map = is_k ? &kmap : &vmap;
-      const int32_t* table = block_tables + int64_t(MODE == kTcPrefix ? q_begin : s) * max_blocks_per_seq;
+      const int32_t* table = block_tables + int64_t(s) * max_blocks_per_seq;
       for (int j = 0; j < n_kv; ++j) {
         const int st = j % nst_ring, use = j / nst_ring;
-        const int p0 = kv_tile(j0 + j) * (kTileN / kPageSize);
+        const int p0 = (j0 + j) * (kTileN / kPageSize);
         const int np = min(kTileN / kPageSize, need_pages - p0);
-        // window mode: pages from a on hold a window key, those below b a sink; the rest are not read
-        const int a = MODE == kTcWindow ? span.lo / kPageSize - p0 : 0, b = MODE == kTcWindow ? sink_pages - p0 : 0;
-        auto skipped = [&](int pi) { return MODE == kTcWindow && pi < a && pi >= b; };
         int rows[kTileN / kPageSize];
-        int loaded = 0;
         for (int pi = 0; pi < np; ++pi) {
-          if (skipped(pi)) continue;
-          ++loaded;
           int blk = __ldg(table + p0 + pi);
           if (blk < 0 || blk >= num_blocks) {
             record_error(err, FVB_ERR_BAD_PAGE, s);
@@ -353,9 +415,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
           rows[pi] = (blk * n_kv_heads + kvh) * kPageSize;
         }
         if (use > 0 && !mbar_wait(&empty[st], (use - 1) & 1, err, is_k ? 0x300 : 0x301)) break;
-        mbar_arrive_expect_tx(&full[st], uint32_t(MODE == kTcWindow ? loaded : np) * kPageSize * D * 2);
+        mbar_arrive_expect_tx(&full[st], uint32_t(np) * kPageSize * D * 2);
         for (int pi = 0; pi < np; ++pi) {
-          if (skipped(pi)) continue;
 #pragma unroll
           for (int h = 0; h < C::kHalves; ++h) {
             uint8_t* stage = is_k ? ring + st * C::kKVBytes : smem + v_off(st);
@@ -492,9 +553,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
     const bool row_valid = tok <= t_last[qi] && g < nvh;
     const int head = head0 + g;
     int pos = (row_valid && positions) ? __ldg(positions + tok) : p_last[qi];
-    // window mode: first key of this row's window (its position may lie past kv_len)
-    const int row_lo = MODE == kTcWindow && max(pos, 0) >= ex.window ? max(pos, 0) - ex.window + 1 : 0;
+    // window mode: first column of this row's window (its position may lie past kv_len, then also its window)
+    int row_lo = MODE == kTcWindow && max(pos, 0) >= ex.window ? max(pos, 0) - ex.window + 1 : 0;
     pos = max(min(pos, kv_len - 1), 0);
+    if constexpr (MODE == kTcWindow) {
+      row_lo = row_lo >= kv_len ? 0x7fffffff : column(row_lo);
+      pos = column(pos);
+    }
     // prefix mode: a sequence shorter than the prefix sees its own keys only, possibly none (-1)
     if (MODE == kTcPrefix && row_valid) pos = min(max(__ldg(kv_lens + tok), 0), kv_len) - 1;
     const float scale = kLog2e * rsqrtf(float(D));
@@ -511,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
       tc_fence_after();
       uint32_t sr[128];
       tmem_ld_128cols(t_row + col_s(i), sr);
-      const int kbase = kv_tile(j0 + j) * kTileN;
+      const int kbase = (j0 + j) * kTileN;
       if (kbase + kTileN - 1 > pos) {
 #pragma unroll
         for (int c = 0; c < 128; ++c) {
@@ -593,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
       tmem_wait_st();
       bool dead = j == n_kv - 1 && kbase + kTileN - 1 > pos_max;
       // window mode: also keys that lie before every row's window and past the sinks
-      if (MODE == kTcWindow) dead = dead || (kbase < span.lo && kbase + kTileN > ex.sinks);
+      if (MODE == kTcWindow) dead = dead || (kbase < lo_min && kbase + kTileN > ex.sinks);
       if (dead) {
         // Keys past the last visible one (pos_max) in the final KV tile are either
         // not loaded (stale shared memory) or uninitialised pool slots: P is 0
@@ -602,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
         ok = warp_wait(&v_full[st], (j / kVS) & 1, err, 0x324 + i);
         if (!ok) break;
         const int key = kbase + r;
-        if (key > pos_max || (MODE == kTcWindow && key < span.lo && key >= ex.sinks)) {
+        if (key > pos_max || (MODE == kTcWindow && key < lo_min && key >= ex.sinks)) {
 #pragma unroll
           for (int h = 0; h < C::kHalves; ++h) {
 #pragma unroll
