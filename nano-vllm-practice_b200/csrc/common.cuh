@@ -62,12 +62,12 @@ __device__ __forceinline__ int keys_cta_of(int64_t g, int64_t total, int grid) {
 
 // Sequences of group g, inside [0, num_seqs) whatever cu_groups holds.
 __device__ __forceinline__ int2 group_rows(const DecodeExtra& ex, int g, int num_seqs) {
-  const int lo = min(max(__ldg(ex.cu_groups + g), 0), num_seqs);
-  return make_int2(lo, min(max(__ldg(ex.cu_groups + g + 1), lo), num_seqs));
+  const int lo = min(max(ex.cu_groups[g], 0), num_seqs);
+  return make_int2(lo, min(max(ex.cu_groups[g + 1], lo), num_seqs));
 }
 // Keys of group g's shared prefix, in whole pages; a sequence alone in its group shares nothing.
 __device__ __forceinline__ int group_prefix(const DecodeExtra& ex, int g, int2 rows) {
-  return rows.y - rows.x < 2 ? 0 : min(max(__ldg(ex.prefix_lens + g), 0), ex.prefix_cap) / kPageSize * kPageSize;
+  return rows.y - rows.x < 2 ? 0 : min(max(ex.prefix_lens[g], 0), ex.prefix_cap) / kPageSize * kPageSize;
 }
 // ---------------------------------------------------------------------------
 // Element types

@@ -209,6 +209,22 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
   // ---- tiles of every sequence, and their running sum ----
   {
     int32_t* warp_sum = reinterpret_cast<int32_t*>(red);
+    // The groups' table in the K ring, which is still empty, where it fits (it may hold empty groups).
+    int32_t* groups = reinterpret_cast<int32_t*>(smem + C::kOffK);
+    const int G = a.ex.num_groups;
+    const bool staged = MODE == kKeysRest && (2 * G + 1) * 4 <= kS * C::kTileBytes;
+    if (staged) {
+      for (int g = threadIdx.x; g <= G; g += kThreads) {
+        groups[g] = __ldg(a.ex.cu_groups + g);
+        if (g < G) groups[G + 1 + g] = __ldg(a.ex.prefix_lens + g);
+      }
+      __syncthreads();
+    }
+    DecodeExtra gx = a.ex;
+    if (staged) {
+      gx.cu_groups = groups;
+      gx.prefix_lens = groups + G + 1;
+    }
     int carry = 0;
     if (threadIdx.x == 0) cum[0] = 0;
     for (int base = 0; base < B; base += kThreads) {
@@ -217,14 +233,14 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
       if (b < B) {
         int skip = 0;
         if constexpr (MODE == kKeysRest) {
-          int lo = 0, hi = a.ex.num_groups;  // first group whose end lies behind b
+          int lo = 0, hi = G;  // first group whose end lies behind b
           while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (__ldg(a.ex.cu_groups + mid + 1) > b) hi = mid; else lo = mid + 1;
+            if (gx.cu_groups[mid + 1] > b) hi = mid; else lo = mid + 1;
           }
-          if (a.ex.prefix_cap > 0 && lo < a.ex.num_groups) {
-            const int2 rows = group_rows(a.ex, lo, B);
-            if (b >= rows.x) skip = group_prefix(a.ex, lo, rows);
+          if (gx.prefix_cap > 0 && lo < G) {
+            const int2 rows = group_rows(gx, lo, B);
+            if (b >= rows.x) skip = group_prefix(gx, lo, rows);
           }
           skips[b] = skip;
         }

@@ -39,7 +39,17 @@ int window_max_units(int max_kv_len, int window, int sinks, int unit) {
 DecodePlan plan_window_decode(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int max_kv_len, int window,
                               int sinks, int num_sms) {
   const int pages = window_max_units(max_kv_len, window, sinks, kPageSize);
-  return plan_decode(num_seqs, n_heads, n_kv_heads, head_dim, pages * kPageSize, num_sms);
+  DecodePlan p = plan_decode(num_seqs, n_heads, n_kv_heads, head_dim, pages * kPageSize, num_sms);
+  // Eight pages are one stage for each consumer warp: a shorter split saves no time and may cost the combine
+  // (4 short fp32 sequences, window 64: 6.6 us with splits of 4 pages and a combine, XX without).
+  constexpr int kOneRound = 8;
+  if (p.pages_per_split < kOneRound) {
+    p.pages_per_split = kOneRound;
+    p.max_splits = (pages + kOneRound - 1) / kOneRound;
+    const size_t rows = size_t(num_seqs) * n_heads * p.max_splits;
+    p.ws_bytes = p.max_splits > 1 ? ((rows * head_dim * 4 + 255) & ~size_t(255)) + rows * 4 : 0;
+  }
+  return p;
 }
 
 cudaError_t launch_window_decode(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,

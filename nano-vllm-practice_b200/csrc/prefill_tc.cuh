@@ -121,8 +121,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
 //            plain form is group g, its query tokens the group's sequences, its pages those of
 //            the group's first sequence, and query i sees keys below min(kv_lens[i], prefix).
 //            Always a partial (O / l and log2-sum-exp) per split, merged with the partials of
-//            each sequence's own keys.  Items are found by a scan of cu_groups in the CTA, so
-//            there is no plan kernel in front.
+//            each sequence's own keys.
+// Window and prefix launches have no plan kernel in front: each CTA finds its item itself.
 enum TcMode { kTcPlain = 0, kTcWindow = 1, kTcPrefix = 2 };
 
 template <typename T, int D, int NREP, bool kIlv, int MODE = kTcPlain>
@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
   // head's q and are never written.
   // With split-KV (decode mode, tiles_per_split > 0) each such CTA is further one of
   // max_splits ranges of 128-key tiles.
+  // (window mode: tiles_per_split < 0 leaves single-token sequences to the split-KV kernel)
   const int nsp = tiles_per_split > 0 ? max_splits : 1;
   const int split = int(blockIdx.x) % nsp, cta = int(blockIdx.x) / nsp;
   const int units = n_kv_heads * chunks;
@@ -173,31 +174,59 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
   const int head0 = kvh * group + chunk * NREP;     // query head of tile slot g = head0 + g
   const int nvh = min(NREP, group - chunk * NREP);  // slots that are real heads
   int s = 0, q_begin = 0, q_end = 0, tile0 = 0;
-  if constexpr (MODE == kTcPrefix) {
-    // Item -> (group, query tiles): a warp scans 32 groups' item counts at a time.
-    constexpr int kItemTok = kIlv ? TOK : 2 * TOK;  // interleaved KV: one query tile an item
-    int before = 0, found = 0;
-    for (int base = 0; base < ex.num_groups && !found; base += 32) {
-      const int g = base + (threadIdx.x & 31);
-      const int2 rows = g < ex.num_groups ? group_rows(ex, g, num_seqs) : make_int2(0, 0);
-      const int n = (rows.y - rows.x + kItemTok - 1) / kItemTok;
-      int upto = n;
+  if constexpr (MODE != kTcPlain) {
+    // Item -> (sequence or group, query tiles) by a scan of their item counts, kThreads at a time: two
+    // dependent loads where the search below takes log2(sequences) of them behind a plan kernel.  (A window
+    // bounds every item's work, so there is no longest-first order to keep.)
+    constexpr int kItemTok = MODE == kTcPrefix && kIlv ? TOK : 2 * TOK;  // interleaved KV: one query tile an item
+    __shared__ int sh_sum[kThreads / 32], sh_item[4];
+    const int n = MODE == kTcPrefix ? ex.num_groups : num_seqs;
+    const int wid = threadIdx.x >> 5, l = threadIdx.x & 31;
+    int before = 0;
+    bool found = false;
+    for (int base = 0; base < n && !found; base += kThreads) {
+      const int g = base + threadIdx.x;
+      int2 rows = make_int2(0, 0);
+      if (g < n) {
+        if constexpr (MODE == kTcPrefix) {
+          rows = group_rows(ex, g, num_seqs);
+        } else {
+          rows = make_int2(__ldg(cu_seqlens + g), __ldg(cu_seqlens + g + 1));
+        }
+      }
+      const int len = rows.y - rows.x;
+      const int count =
+          len > 0 && !(MODE == kTcWindow && tiles_per_split < 0 && len == 1) ? (len + kItemTok - 1) / kItemTok : 0;
+      int upto = count;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);
-        if ((threadIdx.x & 31) >= o) upto += y;
+        if (l >= o) upto += y;
       }
-      const uint32_t past = __ballot_sync(0xffffffffu, item < before + upto);
-      const int src = past ? __ffs(past) - 1 : 31;
-      const int at = __shfl_sync(0xffffffffu, upto - n, src);
-      s = base + src;
-      q_begin = __shfl_sync(0xffffffffu, rows.x, src);
-      q_end = __shfl_sync(0xffffffffu, rows.y, src);
-      tile0 = (item - before - at) * (kIlv ? 1 : 2);
-      before += __shfl_sync(0xffffffffu, upto, 31);
-      found = past != 0;
+      if (l == 31) sh_sum[wid] = upto;
+      __syncthreads();
+      int sum = before;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < wid) upto += sh_sum[w];
+        sum += sh_sum[w];
+      }
+      upto += before;
+      if (count > 0 && item >= upto - count && item < upto) {
+        sh_item[0] = g;
+        sh_item[1] = rows.x;
+        sh_item[2] = rows.y;
+        sh_item[3] = (item - (upto - count)) * (kItemTok / TOK);
+      }
+      __syncthreads();
+      found = item < sum;
+      before = sum;
     }
     if (!found) return;
+    s = sh_item[0];
+    q_begin = sh_item[1];
+    q_end = sh_item[2];
+    tile0 = sh_item[3];
   } else {
     if (item >= __ldg(cu_items + num_seqs)) return;
     int lo = 0, hi = num_seqs - 1;
@@ -790,7 +819,7 @@ cudaError_t launch_tc(const void* q, void* out, const void* k_pool, const void* 
   if (ce != cudaSuccess) return ce;
   int32_t* order = nullptr;
   int32_t* cu_items = nullptr;
-  if (MODE != kTcPrefix) {
+  if (MODE == kTcPlain) {
     order = static_cast<int32_t*>(workspace);
     cu_items = order + ((num_seqs + 63) & ~63);
     ce = launch_prefill_plan(cu_seqlens, kv_lens, num_seqs, TOK, 2, order, cu_items, stream,
