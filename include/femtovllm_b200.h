@@ -326,8 +326,8 @@ FVB_API int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_st
  * max_kv_len at most fvb_max_kv_len(); workspace 256-byte aligned.
  */
 FVB_API size_t fvb_paged_attention_shared_prefix_workspace_size(int num_seqs, int n_heads, int n_kv_heads,
-                                                                int head_dim, int num_groups, int max_prefix_len,
-                                                                int dtype);
+                                                                int head_dim, int max_kv_len, int num_groups,
+                                                                int max_prefix_len, int dtype);
 FVB_API int fvb_paged_attention_shared_prefix_decode(
     const void* q, int64_t q_token_stride, int64_t q_head_stride, void* out, int64_t out_token_stride,
     int64_t out_head_stride, const void* k_pool, const void* v_pool, int64_t num_blocks, int n_heads, int n_kv_heads,

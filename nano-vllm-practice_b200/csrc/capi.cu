@@ -599,9 +599,11 @@ int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_stride, in
 }
 
 size_t fvb_paged_attention_shared_prefix_workspace_size(int num_seqs, int n_heads, int n_kv_heads, int head_dim,
-                                                        int num_groups, int max_prefix_len, int dtype) {
-  if (num_seqs <= 0 || num_groups < 0 || !gqa_ok(n_heads, n_kv_heads) || esize_of(dtype) == 0) return 0;
-  return plan_shared_prefix(num_seqs, n_heads, n_kv_heads, head_dim, num_groups, max_prefix_len, dtype,
+                                                        int max_kv_len, int num_groups, int max_prefix_len,
+                                                        int dtype) {
+  if (num_seqs <= 0 || num_groups < 0 || max_kv_len < 0 || !gqa_ok(n_heads, n_kv_heads) || esize_of(dtype) == 0)
+    return 0;
+  return plan_shared_prefix(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, num_groups, max_prefix_len, dtype,
                             device_sm_count())
       .ws_bytes;
 }
@@ -626,7 +628,7 @@ int fvb_paged_attention_shared_prefix_decode(
       int64_t(max_kv_len) > int64_t(max_blocks_per_seq) * kPageSize)
     return FVB_ERR_INVALID_ARGUMENT;
   if (num_groups > kMaxGridYZ || int64_t(n_heads) > kMaxGridYZ) return FVB_ERR_UNSUPPORTED;
-  const SharedPrefixPlan plan = plan_shared_prefix(num_seqs, n_heads, n_kv_heads, head_dim, num_groups,
+  const SharedPrefixPlan plan = plan_shared_prefix(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, num_groups,
                                                    max_prefix_len, dtype, device_sm_count());
   if (!workspace || workspace_bytes < plan.ws_bytes) return FVB_ERR_WORKSPACE_TOO_SMALL;
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;

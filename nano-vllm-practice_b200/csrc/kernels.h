@@ -180,13 +180,14 @@ cudaError_t launch_window_prefill_simt(const void* q, void* out, const void* k_p
 // kKeysMaxSeqs sequences: the window decode, or the sequences' own keys behind a shared prefix (rest).
 enum KeysMode { kKeysWindow = 0, kKeysRest = 1 };
 constexpr int kKeysMaxSeqs = 1024;
-constexpr int kKeysCols = 16;  // heads of a unit at most
+constexpr int kKeysCols = 16;   // heads of a unit at most
+constexpr int kKeysTile = 128;  // keys of a tile
 struct KeysPlan {
   int grid;
   size_t off_cut_o, off_cut_l, off_full_o, off_full_l;  // the merge's table at 0
   size_t ws_bytes;
 };
-KeysPlan plan_keys(int num_seqs, int n_heads, int head_dim, int mode, int num_sms);
+KeysPlan plan_keys(int num_seqs, int n_heads, int head_dim, int mode, int grid);
 cudaError_t launch_keys_decode(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
                                int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
                                int max_blocks_per_seq, const int32_t* kv_lens, int kv_cap, const DecodeExtra& ex,
@@ -208,8 +209,8 @@ struct SharedPrefixPlan {
   size_t off_spans, off_po, off_pl, off_ro, off_rl;  // items at 0, spans, prefix and rest partials
   size_t ws_bytes;
 };
-SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int num_groups,
-                                    int max_prefix_len, int dtype, int num_sms);
+SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int max_kv_len,
+                                    int num_groups, int max_prefix_len, int dtype, int num_sms);
 cudaError_t launch_shared_prefix(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
                                  int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
                                  int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len,

@@ -613,10 +613,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
         }
       }
       if (MODE == kTcWindow && kbase < row_lo) {
-        const int a = ex.sinks - kbase, b = row_lo - kbase;  // columns [a, b) lie between sinks and window
+        // columns [a, b) lie between sinks and window; bits first, then one test a score (2 % over comparisons)
+        const int a = ex.sinks - kbase, b = row_lo - kbase;
+        auto below = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
+        uint32_t hidden[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) hidden[k] = below(b - 32 * k) & ~below(a - 32 * k);
 #pragma unroll
         for (int c = 0; c < 128; ++c) {
-          if (c >= a && c < b) sr[c] = __float_as_uint(-INFINITY);
+          if ((hidden[c / 32] >> (c % 32)) & 1u) sr[c] = __float_as_uint(-INFINITY);
         }
       }
       float mx[8];

@@ -10,8 +10,9 @@
 // per sequence, bound by HBM.  16-bit types, up to kKeysMaxSeqs sequences, three launches:
 //
 //   prefix   prefill_tc.cuh (kTcPrefix);
-//   rest     decode_keys.cu: the sequences' own tiles dealt evenly to one CTA per SM;
-//            starts as the prefix's CTAs leave their SMs (programmatic dependent launch);
+//   rest     decode_keys.cu: the sequences' own tiles dealt evenly to the SMs that the
+//            prefix kernel leaves it, beside which it runs (programmatic dependent launch):
+//            one is bound by the tensor cores and L2, the other by HBM;
 //   merge    one or four warps per (sequence, query head).
 //
 // fp32 and larger batches, four launches:
@@ -374,36 +375,49 @@ cudaError_t run(const SharedArgs& a, const MergeArgs& m, int head_dim, int dtype
 
 }  // namespace
 
-SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int num_groups,
-                                    int max_prefix_len, int dtype, int num_sms) {
+SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, int head_dim, int max_kv_len,
+                                    int num_groups, int max_prefix_len, int dtype, int num_sms) {
   SharedPrefixPlan p{};
   if (num_seqs <= 0 || n_kv_heads <= 0) return p;
   const int group = n_heads / n_kv_heads;
-  const int prefix = std::max(0, max_prefix_len) / kPageSize * kPageSize;
+  const int prefix = std::max(0, std::min(max_prefix_len, max_kv_len)) / kPageSize * kPageSize;
+  p.keys = dtype != FVB_DTYPE_F32 && num_seqs <= kKeysMaxSeqs;
+  int taken = 0;  // SMs that the prefix kernel holds
   if (prefix > 0 && num_groups > 0) {
-    // The prefix is split until its CTAs fill the SMs once; a group's rows are cut into
-    // tensor-core tiles (fp32: chunks of eight rows).  Groups of the average size that fit one
-    // query tile take items of one tile, whose two softmax groups share it.
+    // A group's rows are cut into tensor-core tiles (fp32: chunks of eight rows), its prefix into splits until
+    // the CTAs fill the SMs that are the prefixes' share.  Groups of the average size that fit one query tile
+    // take items of one tile, whose two softmax groups share it.
     const bool tc = dtype != FVB_DTYPE_F32;
     const int unit = tc ? 128 : kPageSize * 4;
     const int tile = tc ? 128 / tc_tile_heads(group) : 1;  // sequences of a query tile
     const int average = (num_seqs + num_groups - 1) / num_groups;
     p.single_tiles = tc && average <= tile;
-    const int64_t per_group = tc ? (average + tile * (p.single_tiles ? 1 : 2) - 1) / (tile * (p.single_tiles ? 1 : 2))
-                                 : (int64_t(average) * group + 7) / 8;
+    const int item = tile * (p.single_tiles ? 1 : 2);
+    const int64_t per_group = tc ? (average + item - 1) / item : (int64_t(average) * group + 7) / 8;
     const int heads = tc ? n_kv_heads * ((group + tc_tile_heads(group) - 1) / tc_tile_heads(group)) : n_kv_heads;
     const int64_t ctas = std::max<int64_t>(1, per_group * num_groups * heads);
     const int units = (prefix + unit - 1) / unit;
-    const int64_t wanted = std::max<int64_t>(1, (tc ? num_sms : num_sms * 6) / ctas);
-    const int per = int((units + std::min<int64_t>(wanted, units) - 1) / std::min<int64_t>(wanted, units));
+    int64_t room = tc ? num_sms : num_sms * 6;
+    if (p.keys) {
+      // Both kernels hold an SM's shared memory alone, so they share the SMs out: a prefix tile (twice the work
+      // in items of two) takes about 1.45 us of an SM from L2, a tile of the sequences' own keys 1.64 us from
+      // HBM.  The contexts behind the prefixes are taken for half of what max_kv_len leaves.
+      const int own = std::max(0, max_kv_len - prefix) / 2;
+      const double first = double(ctas) * units * (p.single_tiles ? 1.45 : 2.5);
+      const double rest = double(num_seqs) * n_kv_heads * ((group + kKeysCols - 1) / kKeysCols) *
+                          ((own + kKeysTile - 1) / kKeysTile) * 1.64;
+      room = std::max<int64_t>(num_sms / 8, std::min<int64_t>(num_sms * 7 / 8, int64_t(num_sms * first / (first + rest))));
+    }
+    const int64_t wanted = std::min<int64_t>(std::max<int64_t>(1, room / ctas), units);
+    const int per = int((units + wanted - 1) / wanted);
     p.keys_per_split = per * unit;
     p.prefix_splits = (prefix + p.keys_per_split - 1) / p.keys_per_split;
+    taken = int(std::min<int64_t>(num_sms * 7 / 8, ctas * p.prefix_splits));
   }
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   const size_t rows = size_t(num_seqs) * n_heads * p.prefix_splits;
-  p.keys = dtype != FVB_DTYPE_F32 && num_seqs <= kKeysMaxSeqs;
   if (p.keys) {
-    p.kp = plan_keys(num_seqs, n_heads, head_dim, kKeysRest, num_sms);
+    p.kp = plan_keys(num_seqs, n_heads, head_dim, kKeysRest, num_sms - taken);
     p.off_po = up(p.kp.ws_bytes);
   } else {
     // About four waves of three resident split-KV CTAs per SM, as plan_decode.

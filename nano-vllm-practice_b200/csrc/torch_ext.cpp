@@ -413,7 +413,7 @@ torch::Tensor PagedAttentionSharedPrefixGemvCuda(torch::Tensor q, torch::Tensor 
   c10::cuda::CUDAGuard guard(q.device());
   auto out = new_out(q, out_token_major);
   const size_t ws_bytes = fvb_paged_attention_shared_prefix_workspace_size(num_seqs, n_heads, int(k_pool.size(1)),
-                                                                           head_dim, groups, prefix, dt);
+                                                                           head_dim, kv, groups, prefix, dt);
   torch::Tensor ws = new_workspace(ws_bytes, q);
   check_status(fvb_paged_attention_shared_prefix_decode(
                    q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), out.stride(1), out.stride(0),

@@ -98,7 +98,7 @@ _SIGNATURES = {
          c_size_t, c_void_p],
     ),
     "fvb_paged_attention_shared_prefix_workspace_size": (
-        c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]
+        c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]
     ),
     "fvb_paged_attention_shared_prefix_decode": (
         c_int,
