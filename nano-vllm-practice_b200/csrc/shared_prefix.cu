@@ -10,9 +10,9 @@
 // per sequence, bound by HBM.  16-bit types, up to kKeysMaxSeqs sequences, three launches:
 //
 //   prefix   prefill_tc.cuh (kTcPrefix);
-//   rest     decode_keys.cu: the sequences' own tiles dealt evenly to the SMs that the
-//            prefix kernel leaves it, beside which it runs (programmatic dependent launch):
-//            one is bound by the tensor cores and L2, the other by HBM;
+//   rest     decode_keys.cu: the sequences' own tiles dealt evenly to one CTA per SM, as the
+//            prefix's CTAs leave them (programmatic dependent launch), or with one group to
+//            the SMs that the prefix kernel does not take, beside which it then runs;
 //   merge    one or four warps per (sequence, query head).
 //
 // fp32 and larger batches, four launches:
@@ -398,10 +398,13 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     const int64_t ctas = std::max<int64_t>(1, per_group * num_groups * heads);
     const int units = (prefix + unit - 1) / unit;
     int64_t room = tc ? num_sms : num_sms * 6;
-    if (p.keys) {
+    if (p.keys && num_groups == 1) {
       // Both kernels hold an SM's shared memory alone, so they share the SMs out: a prefix tile (twice the work
       // in items of two) takes about 1.45 us of an SM from L2, a tile of the sequences' own keys 1.64 us from
-      // HBM.  The contexts behind the prefixes are taken for half of what max_kv_len leaves.
+      // HBM.  The contexts behind the prefix are taken for half of what max_kv_len leaves.  (8 beams: 17.2 us
+      // one kernel after the other on all SMs, 12.7 beside each other; 32 requests behind 4096 tokens: 39.6,
+      // 32.2.)  With several groups the number of prefix CTAs is not known here, and a CTA too many holds up
+      // a whole share of the rest (128 sequences in 4 groups: 100 us after each other, 113 beside).
       const int own = std::max(0, max_kv_len - prefix) / 2;
       const double first = double(ctas) * units * (p.single_tiles ? 1.45 : 2.5);
       const double rest = double(num_seqs) * n_kv_heads * ((group + kKeysCols - 1) / kKeysCols) *
@@ -412,7 +415,7 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     const int per = int((units + wanted - 1) / wanted);
     p.keys_per_split = per * unit;
     p.prefix_splits = (prefix + p.keys_per_split - 1) / p.keys_per_split;
-    taken = int(std::min<int64_t>(num_sms * 7 / 8, ctas * p.prefix_splits));
+    if (num_groups == 1) taken = int(std::min<int64_t>(num_sms * 7 / 8, ctas * p.prefix_splits));
   }
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   const size_t rows = size_t(num_seqs) * n_heads * p.prefix_splits;
