@@ -359,10 +359,6 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
 #pragma unroll
             for (int i = 0; i < kTilePages; ++i) {
               if (i < pages) {  // a tile's pages are its first ones
-                if (warp == 2) {  // V: both halves of a page in one box
-                  tma_load_3d(dst + i * kPageSize * D * 2, map, 0, rows[i], 0, &full[st]);
-                  continue;
-                }
 #pragma unroll
                 for (int h = 0; h < C::kHalves; ++h)
                   tma_load_2d(dst + h * kHalf + i * kPageSize * 128, map, h * 64, rows[i], &full[st]);
@@ -379,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
         constexpr uint32_t idesc_o = umma_idesc_f16(kBF16, 128, kCols, false, true);
         const uint64_t dk = umma_sdesc_sw128(smem_u32(smem + C::kOffK), 16, 1024);
         // At D 64 both halves of the 128 rows read the same 64 dims; rows 64 .. 127 of O are not used.
-        const uint64_t dv = umma_sdesc_sw128(smem_u32(smem + C::kOffV), D == 128 ? kPageSize * 128 : 0, 1024);
+        const uint64_t dv = umma_sdesc_sw128(smem_u32(smem + C::kOffV), D == 128 ? kHalf : 0, 1024);
         const uint64_t dq = umma_sdesc_sw128(smem_u32(smem + C::kOffQ), 16, 1024);
         const uint64_t dp = umma_sdesc_sw128(smem_u32(smem + C::kOffP), 16, 1024);
         bool ok = true;
@@ -394,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
           const uint64_t pd = dp + uint64_t(((j & 1) * 2 * kBHalf) >> 4);
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk)
-            umma_f16_ss(col_o(item), vd + uint64_t((kk * kPageSize * D * 2) >> 4),
+            umma_f16_ss(col_o(item), vd + uint64_t((kk * 16 * 128) >> 4),
                         pd + uint64_t(((kk >> 2) * kBHalf + (kk & 3) * 32) >> 4), idesc_o, first && kk == 0 ? 0u : 1u);
           umma_commit(&v_empty[st]);
           umma_commit(&pv_done[j & 1]);
@@ -596,8 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
               for (int h = 0; h < C::kHalves; ++h) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                  sts_v4(smem_u32(smem + C::kOffV + st * C::kTileBytes + (key_t >> 4) * kPageSize * D * 2 +
-                                  h * kPageSize * 128 + (key_t & 15) * 128 + i * 16),
+                  sts_v4(smem_u32(smem + C::kOffV + st * C::kTileBytes + h * kHalf + key_t * 128 + i * 16),
                          make_uint4(0, 0, 0, 0));
               }
             }
@@ -701,11 +696,7 @@ cudaError_t launch_t(const KeysArgs& a, const void* k_pool, const void* v_pool, 
   CUtensorMap kmap, vmap;
   const uint64_t rows = uint64_t(a.num_blocks) * a.n_kv_heads * kPageSize;
   cudaError_t ce = make_tma_2d(&kmap, k_pool, tdt, D, rows, D * 2, 64, kPageSize, true);
-  // V: boxes of a whole page, [D / 64 halves][16 keys][128 bytes] in shared memory
-  const uint64_t vdims[3] = {64, rows, uint64_t(C::kHalves)};
-  const uint64_t vstrides[2] = {D * 2, 128};
-  const uint32_t vbox[3] = {64, kPageSize, uint32_t(C::kHalves)};
-  if (ce == cudaSuccess) ce = make_tma_3d(&vmap, v_pool, tdt, vdims, vstrides, vbox, true);
+  if (ce == cudaSuccess) ce = make_tma_2d(&vmap, v_pool, tdt, D, rows, D * 2, 64, kPageSize, true);
   if (ce == cudaSuccess) ce = set_smem_once<decode_keys_kernel<T, D, HV, MODE>>(C::smem_bytes(kKeysMaxSeqs));
   if (ce != cudaSuccess) return ce;
   cudaLaunchConfig_t cfg = {};
