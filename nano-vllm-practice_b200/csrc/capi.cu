@@ -121,8 +121,16 @@ int check_layout(const QOLayout& lay, int dtype) {
 }  // namespace
 
 int device_sm_count() {
+  // asked once per device: every call plans with it, some twice
+  static std::atomic<int> known[kMaxDevices] = {};
   int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (cudaGetDevice(&dev) != cudaSuccess) return sms;
+  if (dev >= 0 && dev < kMaxDevices) {
+    const int n = known[dev].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+  }
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < kMaxDevices) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
 }
 

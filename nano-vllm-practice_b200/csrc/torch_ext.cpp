@@ -12,6 +12,7 @@
 // workspace) with the caching allocator, and calls the C ABI on the current
 // CUDA stream.  The same functions are also registered as torch.ops.femtovllm_b200.*.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime_api.h>
 #include <torch/extension.h>
@@ -330,9 +331,27 @@ int checked_int(int64_t x, const char* name) {
   return int(x);
 }
 
-torch::Tensor new_workspace(size_t bytes, const at::Tensor& like) {
-  return torch::empty({int64_t(bytes > 0 ? bytes : 1)}, like.options().dtype(torch::kUInt8));
+// Straight from the caching allocator: the small calls here are bound by the host, and the dispatcher's part of
+// torch::empty is a tenth of one.
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
+
+// As new_out above.
+at::Tensor new_attention_out(const at::Tensor& q, bool token_major) {
+  if (!token_major) return new_tensor(q.sizes(), q.scalar_type(), q);
+  return new_tensor({q.size(1), q.size(0), q.size(2)}, q.scalar_type(), q).transpose(0, 1);
+}
+
+// A workspace of `bytes`, nothing (and a null pointer) for 0.
+struct Workspace {
+  at::Tensor tensor;
+  size_t bytes;
+  Workspace(size_t n, const at::Tensor& like) : bytes(n) {
+    if (n > 0) tensor = new_tensor({int64_t(n)}, at::kByte, like);
+  }
+  void* data() const { return bytes > 0 ? tensor.data_ptr() : nullptr; }
+};
 
 }  // namespace
 
@@ -346,15 +365,15 @@ torch::Tensor PagedAttentionWindowGemvCuda(torch::Tensor q, torch::Tensor k_pool
   const int kv = checked_int(max_kv_len, "max_kv_len"), win = checked_int(window, "window"),
             sinks = checked_int(num_sinks, "num_sinks");
   c10::cuda::CUDAGuard guard(q.device());
-  auto out = new_out(q, out_token_major);
-  const size_t ws_bytes = fvb_paged_attention_window_decode_workspace_size(num_seqs, n_heads, int(k_pool.size(1)),
-                                                                           head_dim, kv, win, sinks);
-  torch::Tensor ws = new_workspace(ws_bytes, q);
+  auto out = new_attention_out(q, out_token_major);
+  const Workspace ws(fvb_paged_attention_window_decode_workspace_size(num_seqs, n_heads, int(k_pool.size(1)), head_dim,
+                                                                      kv, win, sinks),
+                     q);
   check_status(fvb_paged_attention_window_decode(
                    q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), out.stride(1), out.stride(0),
                    k_pool.data_ptr(), v_pool.data_ptr(), k_pool.size(0), n_heads, int(k_pool.size(1)), head_dim,
                    int(k_pool.size(2)), num_seqs, kv_page_tables.data_ptr<int32_t>(), int(kv_page_tables.size(1)),
-                   kv_lens.data_ptr<int32_t>(), kv, win, sinks, dtype_code(q.scalar_type()), ws.data_ptr(), ws_bytes,
+                   kv_lens.data_ptr<int32_t>(), kv, win, sinks, dtype_code(q.scalar_type()), ws.data(), ws.bytes,
                    stream_of(q)),
                "PagedAttentionWindowGemvCuda");
   return out;
@@ -379,16 +398,16 @@ torch::Tensor PagedAttentionWindowGemmCuda(torch::Tensor q, torch::Tensor k_pool
   const int max_q = checked_int(max_q_len, "max_q_len"), win = checked_int(window, "window"),
             sinks = checked_int(num_sinks, "num_sinks");
   c10::cuda::CUDAGuard guard(q.device());
-  auto out = new_out(q, out_token_major);
-  const size_t ws_bytes = fvb_paged_attention_prefill_workspace_size(num_seqs, n_heads, int(k_pool.size(1)), head_dim,
-                                                                     q_len_flatten, max_q);
-  torch::Tensor ws = new_workspace(ws_bytes, q);
+  auto out = new_attention_out(q, out_token_major);
+  const Workspace ws(fvb_paged_attention_prefill_workspace_size(num_seqs, n_heads, int(k_pool.size(1)), head_dim,
+                                                                q_len_flatten, max_q),
+                     q);
   check_status(fvb_paged_attention_window_prefill(
                    q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), out.stride(1), out.stride(0),
                    k_pool.data_ptr(), v_pool.data_ptr(), k_pool.size(0), n_heads, int(k_pool.size(1)), head_dim,
                    int(k_pool.size(2)), num_seqs, q_len_flatten, cu_seqlens.data_ptr<int32_t>(), max_q,
                    kv_page_tables.data_ptr<int32_t>(), int(kv_page_tables.size(1)), kv_lens.data_ptr<int32_t>(),
-                   positions.data_ptr<int32_t>(), win, sinks, dtype_code(q.scalar_type()), ws.data_ptr(), ws_bytes,
+                   positions.data_ptr<int32_t>(), win, sinks, dtype_code(q.scalar_type()), ws.data(), ws.bytes,
                    stream_of(q)),
                "PagedAttentionWindowGemmCuda");
   return out;
@@ -411,16 +430,16 @@ torch::Tensor PagedAttentionSharedPrefixGemvCuda(torch::Tensor q, torch::Tensor 
   const int groups = int(prefix_lens.numel()), dt = dtype_code(q.scalar_type());
   const int kv = checked_int(max_kv_len, "max_kv_len"), prefix = checked_int(max_prefix_len, "max_prefix_len");
   c10::cuda::CUDAGuard guard(q.device());
-  auto out = new_out(q, out_token_major);
-  const size_t ws_bytes = fvb_paged_attention_shared_prefix_workspace_size(num_seqs, n_heads, int(k_pool.size(1)),
-                                                                           head_dim, kv, groups, prefix, dt);
-  torch::Tensor ws = new_workspace(ws_bytes, q);
+  auto out = new_attention_out(q, out_token_major);
+  const Workspace ws(fvb_paged_attention_shared_prefix_workspace_size(num_seqs, n_heads, int(k_pool.size(1)), head_dim,
+                                                                      kv, groups, prefix, dt),
+                     q);
   check_status(fvb_paged_attention_shared_prefix_decode(
                    q.data_ptr(), q.stride(1), q.stride(0), out.data_ptr(), out.stride(1), out.stride(0),
                    k_pool.data_ptr(), v_pool.data_ptr(), k_pool.size(0), n_heads, int(k_pool.size(1)), head_dim,
                    int(k_pool.size(2)), num_seqs, kv_page_tables.data_ptr<int32_t>(), int(kv_page_tables.size(1)),
                    kv_lens.data_ptr<int32_t>(), kv, cu_groups.data_ptr<int32_t>(), groups,
-                   prefix_lens.data_ptr<int32_t>(), prefix, dt, ws.data_ptr(), ws_bytes, stream_of(q)),
+                   prefix_lens.data_ptr<int32_t>(), prefix, dt, ws.data(), ws.bytes, stream_of(q)),
                "PagedAttentionSharedPrefixGemvCuda");
   return out;
 }
@@ -447,16 +466,15 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> BeamSearchSelectCuda(tor
   }
   const int K = checked_int(num_select, "num_select"), dt = dtype_code(logits.scalar_type());
   c10::cuda::CUDAGuard guard(logits.device());
-  auto tokens = torch::empty({N, K}, logits.options().dtype(torch::kInt64));
-  auto parents = torch::empty({N, K}, logits.options().dtype(torch::kInt64));
-  auto out = torch::empty({N, K}, scores.options());
-  const size_t ws_bytes = fvb_beam_search_workspace_size(int(N), int(W), V, K, dt);
-  torch::Tensor ws = new_workspace(ws_bytes, logits);
+  auto tokens = new_tensor({N, K}, at::kLong, logits);
+  auto parents = new_tensor({N, K}, at::kLong, logits);
+  auto out = new_tensor({N, K}, at::kFloat, logits);
+  const Workspace ws(fvb_beam_search_workspace_size(int(N), int(W), V, K, dt), logits);
   // A single row's stride is free: torch leaves any value there.
   const int64_t stride = logits.size(0) > 1 ? logits.stride(0) : V;
   check_status(fvb_beam_search_select(logits.data_ptr(), stride, int(N), int(W), V, dt, scores.data_ptr<float>(), done,
                                       eos_token_id, K, tokens.data_ptr<int64_t>(), parents.data_ptr<int64_t>(),
-                                      out.data_ptr<float>(), ws.data_ptr(), ws_bytes, stream_of(logits)),
+                                      out.data_ptr<float>(), ws.data(), ws.bytes, stream_of(logits)),
                "BeamSearchSelectCuda");
   return {tokens, parents, out};
 }
@@ -490,7 +508,7 @@ torch::Tensor BeamReorderKVCacheCuda(std::vector<torch::Tensor> k_pools, std::ve
   TORCH_CHECK(block_tables.size(0) == N * W && kv_lens.numel() == N * W, "one block table row and one kv_len per beam");
   TORCH_CHECK(N <= 0x7fffffff && W <= 0x7fffffff, "too many beams");
   c10::cuda::CUDAGuard guard(pool.device());
-  auto out = torch::empty_like(block_tables);
+  auto out = new_tensor(block_tables.sizes(), at::kInt, block_tables);
   check_status(fvb_beam_reorder_kvcache(k.data(), v.data(), int(k.size()), pool.size(0), int(pool.size(1)),
                                         int(pool.size(3)), int(pool.size(2)), dtype_code(pool.scalar_type()),
                                         block_tables.data_ptr<int32_t>(), out.data_ptr<int32_t>(),

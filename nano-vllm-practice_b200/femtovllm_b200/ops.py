@@ -160,7 +160,8 @@ def paged_attention_window_gemv(
     back.  ``window >= 1``; ``max_kv_len`` still bounds ``kv_lens``, not the window.
     """
     q = _q_view(q)
-    _require_cuda(k_pool=k_pool, v_pool=v_pool, kv_page_tables=kv_page_tables, kv_lens=kv_lens)
+    if not (k_pool.is_cuda and v_pool.is_cuda and kv_page_tables.is_cuda and kv_lens.is_cuda):
+        _require_cuda(k_pool=k_pool, v_pool=v_pool, kv_page_tables=kv_page_tables, kv_lens=kv_lens)
     return _cuda_backend.PagedAttentionWindowGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens, int(max_kv_len),
                                                       int(window), int(num_sinks), bool(out_token_major))
 
@@ -186,8 +187,10 @@ def paged_attention_window_gemm(
     whose mask leaves nothing gives zeros.
     """
     q = _q_view(q)
-    _require_cuda(k_pool=k_pool, v_pool=v_pool, cu_seqlens=cu_seqlens, kv_page_tables=kv_page_tables,
-                  kv_lens=kv_lens, positions=positions)
+    if not (k_pool.is_cuda and v_pool.is_cuda and cu_seqlens.is_cuda and kv_page_tables.is_cuda
+            and kv_lens.is_cuda and positions.is_cuda):
+        _require_cuda(k_pool=k_pool, v_pool=v_pool, cu_seqlens=cu_seqlens, kv_page_tables=kv_page_tables,
+                      kv_lens=kv_lens, positions=positions)
     return _cuda_backend.PagedAttentionWindowGemmCuda(q, k_pool, v_pool, cu_seqlens, int(max_q_len), kv_page_tables,
                                                       kv_lens, positions, int(window), int(num_sinks),
                                                       bool(out_token_major))
@@ -214,8 +217,10 @@ def paged_attention_shared_prefix_gemv(
     ``max_prefix_len`` bounds ``prefix_lens``; keys past it are read per sequence.
     """
     q = _q_view(q)
-    _require_cuda(k_pool=k_pool, v_pool=v_pool, kv_page_tables=kv_page_tables, kv_lens=kv_lens, cu_groups=cu_groups,
-                  prefix_lens=prefix_lens)
+    if not (k_pool.is_cuda and v_pool.is_cuda and kv_page_tables.is_cuda and kv_lens.is_cuda and cu_groups.is_cuda
+            and prefix_lens.is_cuda):
+        _require_cuda(k_pool=k_pool, v_pool=v_pool, kv_page_tables=kv_page_tables, kv_lens=kv_lens,
+                      cu_groups=cu_groups, prefix_lens=prefix_lens)
     return _cuda_backend.PagedAttentionSharedPrefixGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens,
                                                             int(max_kv_len), cu_groups, prefix_lens,
                                                             int(max_prefix_len), bool(out_token_major))
@@ -395,7 +400,8 @@ def beam_search_select(
     ``eos_token_id`` at its own score only.  W and ``num_select`` up to 64; the first step after a
     prompt gives every beam but one a score of ``-inf``.
     """
-    _require_cuda(logits=logits, scores=scores)
+    if not (logits.is_cuda and scores.is_cuda):
+        _require_cuda(logits=logits, scores=scores)
     if logits.dim() == 2 and logits.stride(-1) != 1:
         logits = logits.contiguous()
     if finished is not None:
@@ -427,7 +433,8 @@ def beam_reorder_kvcache(
         for t in pools:
             if not t.is_cuda:
                 raise ValueError(f"Argument '{n}' must be CUDA tensors. Got device={t.device}")
-    _require_cuda(block_tables=block_tables, kv_lens=kv_lens, parents=parents)
+    if not (block_tables.is_cuda and kv_lens.is_cuda and parents.is_cuda):
+        _require_cuda(block_tables=block_tables, kv_lens=kv_lens, parents=parents)
     return _cuda_backend.BeamReorderKVCacheCuda(k_pools, v_pools, block_tables.contiguous(), kv_lens.contiguous(),
                                                 parents.contiguous())
 
