@@ -142,9 +142,10 @@ constexpr int kFinishWarps = kFinishThreads / 32;
 constexpr int kSegment = 32;           // logits
 constexpr int kMaxSegments = 4096;     // of a part: their maxima fill 16 KB of shared memory
 constexpr int kVecs = 4;               // vectors per lane and tile
+constexpr int kFewSegments = 128;      // of a part whose segments are ranked one by one
 constexpr int kListSegs = 1024, kListLogits = 1024;  // segments and logits at or above the bound that are ranked
 
-// The k-th largest (from 0) of `groups` values (64 or 128) into *bound; whole CTAs of WARPS warps.
+// The k-th largest (from 0) of `groups` <= 128 values into *bound, where there are so many; whole CTAs of WARPS warps.
 template <int WARPS>
 __device__ __forceinline__ void kth_largest(const uint32_t* values, int groups, int k, uint32_t* bound) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kThreads) beam_partials_kernel(const BeamArgs 
   const int n_vecs = int(max(min(r.vecs() - part_begin, a.part_vecs), int64_t(0)));
   const int n_segs = (n_vecs + kSegVecs - 1) / kSegVecs;
 
-  if (threadIdx.x == 0) n_list = n_cand = 0;
+  if (threadIdx.x == 0) n_list = n_cand = bound = 0;
   float m = -INFINITY;
   uint32_t run = 0;  // of segments of this thread alone; 0: none
   float2 s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -301,8 +302,11 @@ __global__ void __launch_bounds__(kThreads) beam_partials_kernel(const BeamArgs 
     for (int o = kWarps / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (lane == 0) a.sums[out] = make_float2(mm, ss);
   }
-  // ---- bound: the K-th largest group (0, every logit, where fewer than K groups have one) ----
-  kth_largest<kWarps>(sh_runs, groups, K - 1, &bound);
+  // ---- bound: the K-th largest group (0, every logit, where fewer than K groups have one).  A part of few segments
+  // leaves most groups without one, and its segments are groups themselves (the last 107 vectors of a row of 50001
+  // 16-bit logits, K 10: all 856 logits reached the bound, and ranking them took 22 us). ----
+  const bool few = n_segs <= kFewSegments;
+  kth_largest<kWarps>(few ? sh : sh_runs, few ? n_segs : groups, K - 1, &bound);
   __syncthreads();
   const uint32_t least = bound;
   // ---- segments that reach it, and their logits that do ----
@@ -724,15 +728,18 @@ cudaError_t launch_t(const BeamArgs& a, int num_requests, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, beam_finish_kernel<T>, a);
 }
 
-// Vectors of a part, in whole tiles of a CTA's warps: enough CTAs for the device, at most kMaxSegments
-// segments, and no more lists a request than the finish kernel's threads merge where that allows.
+// Vectors of a part, in whole tiles of a warp and even over the parts: enough CTAs for the device, no part below one
+// tile of each of its warps, at most kMaxSegments segments, and no more lists a request than the finish kernel's
+// threads merge where that allows.
 int64_t beam_part_vecs(int num_requests, int num_beams, int64_t vocab, int esize) {
   const int64_t vecs = (vocab * esize + 15) / 16 + 1;  // a row may straddle one vector more
-  const int64_t rows = int64_t(num_requests) * num_beams, tile = 32 * kVecs * kWarps;
+  const int64_t rows = int64_t(num_requests) * num_beams, warp_tile = 32 * kVecs, tile = warp_tile * kWarps;
   const int64_t wanted = std::min<int64_t>((int64_t(device_sm_count()) * kCtasPerSm + rows - 1) / rows,
                                            kLists * kFinishThreads / num_beams);
-  const int64_t per = ((vecs + wanted - 1) / wanted + tile - 1) / tile * tile;
-  return std::min<int64_t>(per, int64_t(kMaxSegments) * kSegment * esize / 16);
+  const int64_t most = std::min<int64_t>(((vecs + wanted - 1) / wanted + tile - 1) / tile * tile,
+                                         int64_t(kMaxSegments) * kSegment * esize / 16);
+  const int64_t parts = (vecs + most - 1) / most;
+  return ((vecs + parts - 1) / parts + warp_tile - 1) / warp_tile * warp_tile;
 }
 int64_t beam_parts(int num_requests, int num_beams, int64_t vocab, int esize) {
   const int64_t vecs = (vocab * esize + 15) / 16 + 1, per = beam_part_vecs(num_requests, num_beams, vocab, esize);
