@@ -515,7 +515,8 @@ size_t fvb_paged_attention_window_decode_workspace_size(int num_seqs, int n_head
   const int sms = device_sm_count();
   const size_t split_ws =
       plan_window_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, window, num_sinks, sms).ws_bytes;
-  if (num_seqs > kKeysMaxSeqs) return split_ws;
+  if (!window_decode_on_keys(num_seqs, n_heads, n_kv_heads, max_kv_len, window, num_sinks, FVB_DTYPE_BF16, sms))
+    return split_ws;
   const size_t keys_ws = plan_keys(num_seqs, n_heads, head_dim, kKeysWindow, sms).ws_bytes;
   return split_ws > keys_ws ? split_ws : keys_ws;  // fp32, 16-bit
 }
@@ -542,9 +543,7 @@ int fvb_paged_attention_window_decode(const void* q, int64_t q_token_stride, int
   if (num_seqs > kMaxGridYZ || int64_t(n_heads) > kMaxGridYZ) return FVB_ERR_UNSUPPORTED;
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;
   const int sms = device_sm_count();
-  // 16-bit: the tensor-core kernel, whose table of sequences fits its shared memory; fp32 and larger batches
-  // the split-KV kernel.
-  const bool tc = dtype != FVB_DTYPE_F32 && num_seqs <= kKeysMaxSeqs;
+  const bool tc = window_decode_on_keys(num_seqs, n_heads, n_kv_heads, max_kv_len, window, num_sinks, dtype, sms);
   DecodePlan plan{};
   KeysPlan kp{};
   if (tc) kp = plan_keys(num_seqs, n_heads, head_dim, kKeysWindow, sms);
@@ -593,10 +592,10 @@ int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_stride, in
   if (!err) return cuda_status(e);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == FVB_DTYPE_F32)
-    return cuda_status(launch_window_prefill_simt(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim,
-                                                  num_seqs, q_len_flatten, cu_seqlens, block_tables,
-                                                  max_blocks_per_seq, kv_lens, positions, window, num_sinks, lay, err,
-                                                  s));
+    return cuda_status(launch_window_prefill_f32(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim,
+                                                 num_seqs, q_len_flatten, max_q_len, cu_seqlens, block_tables,
+                                                 max_blocks_per_seq, kv_lens, positions, window, num_sinks, lay, err,
+                                                 s));
   const PrefillPlan plan = plan_prefill(num_seqs, n_heads, n_kv_heads, head_dim, q_len_flatten, max_q_len, dtype);
   if (!workspace || workspace_bytes < plan.ws_bytes) return FVB_ERR_WORKSPACE_TOO_SMALL;
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;

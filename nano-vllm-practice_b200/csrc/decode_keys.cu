@@ -729,6 +729,21 @@ cudaError_t dispatch(const KeysArgs& a, const void* k_pool, const void* v_pool, 
 
 }  // namespace
 
+bool window_decode_on_keys(int num_seqs, int n_heads, int n_kv_heads, int max_kv_len, int window, int sinks, int dtype,
+                           int num_sms) {
+  if (dtype == FVB_DTYPE_F32 || num_seqs > kKeysMaxSeqs) return false;  // (the sequence table fills shared memory)
+  // A call of this kernel costs 8 us before its first tile and 3 us a unit that has only one tile, and its tiles then
+  // stream at HBM's rate whatever the group is.  The split-KV kernel starts in 4 us, but what a page costs it grows with
+  // the group's heads, and from five on it is bound by its lanes.  Over 320 calls of random shapes the pages an SM
+  // gets at most are what tells them apart; with these limits the choice is 2 % off the better kernel on average.
+  // (201 sequences x 8 heads, window 5: 29.7 us here, 8.1 there; 256 x 8, group 2, window 1024: 165.5 and 189;
+  // 190 x 2, group 16, window 1512: 67.5 and 157.)
+  const int group = n_heads / n_kv_heads;
+  const int64_t limit = group <= 4 ? 128 : group <= 8 ? 32 : 16;
+  const int64_t pages = window_max_units(max_kv_len, window, sinks, kPageSize);
+  return int64_t(num_seqs) * n_kv_heads * pages > limit * num_sms;
+}
+
 KeysPlan plan_keys(int num_seqs, int n_heads, int head_dim, int mode, int grid) {
   KeysPlan p{};
   p.grid = grid;

@@ -169,12 +169,13 @@ cudaError_t launch_window_prefill(const void* q, void* out, const void* k_pool, 
                                   const int32_t* kv_lens, const int32_t* positions, int window, int sinks, int dtype,
                                   const PrefillPlan& plan, const QOLayout& lay, void* workspace, int* err,
                                   cudaStream_t stream);
-// fp32 (prefill_simt.cu).
-cudaError_t launch_window_prefill_simt(const void* q, void* out, const void* k_pool, const void* v_pool,
-                                       int64_t num_blocks, int n_heads, int n_kv_heads, int head_dim, int num_seqs,
-                                       int64_t q_len_flatten, const int32_t* cu_seqlens, const int32_t* block_tables,
-                                       int max_blocks_per_seq, const int32_t* kv_lens, const int32_t* positions,
-                                       int window, int sinks, const QOLayout& lay, int* err, cudaStream_t stream);
+// fp32 (prefill_f32.cu).
+cudaError_t launch_window_prefill_f32(const void* q, void* out, const void* k_pool, const void* v_pool,
+                                      int64_t num_blocks, int n_heads, int n_kv_heads, int head_dim, int num_seqs,
+                                      int64_t q_len_flatten, int max_q_len, const int32_t* cu_seqlens,
+                                      const int32_t* block_tables, int max_blocks_per_seq, const int32_t* kv_lens,
+                                      const int32_t* positions, int window, int sinks, const QOLayout& lay, int* err,
+                                      cudaStream_t stream);
 
 // 16-bit decode with the keys as the matrix rows of the tensor cores (decode_keys.cu), for up to
 // kKeysMaxSeqs sequences: the window decode, or the sequences' own keys behind a shared prefix (rest).
@@ -187,6 +188,9 @@ struct KeysPlan {
   size_t off_cut_o, off_cut_l, off_full_o, off_full_l;  // the merge's table at 0
   size_t ws_bytes;
 };
+// Whether a window decode runs on it (16-bit types, enough pages) or on the split-KV kernel.
+bool window_decode_on_keys(int num_seqs, int n_heads, int n_kv_heads, int max_kv_len, int window, int sinks, int dtype,
+                           int num_sms);
 KeysPlan plan_keys(int num_seqs, int n_heads, int head_dim, int mode, int grid);
 cudaError_t launch_keys_decode(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
                                int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,

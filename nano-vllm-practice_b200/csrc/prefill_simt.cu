@@ -31,13 +31,13 @@ __device__ __forceinline__ float warp_sum_s(float v) {
   return v;
 }
 
-template <typename T, int D, bool kWindow = false>
+template <typename T, int D>
 __global__ void __launch_bounds__(32 * kWarpsPerCta) prefill_simt_kernel(
     const T* __restrict__ q, T* __restrict__ out, const T* __restrict__ k_pool, const T* __restrict__ v_pool,
     int64_t num_blocks, int n_heads, int n_kv_heads, int num_seqs, int64_t q_len_flatten,
     const int32_t* __restrict__ cu_seqlens, const int32_t* __restrict__ block_tables, int max_blocks_per_seq,
     const int32_t* __restrict__ kv_lens, const int32_t* __restrict__ positions, const QOLayout lay,
-    int* __restrict__ err, int window = 0, int sinks = 0) {
+    int* __restrict__ err) {
   constexpr int kDPL = D / 32;
   __shared__ float qsh[kWarpsPerCta][D];
   __shared__ float psh[kWarpsPerCta][32];
@@ -60,17 +60,7 @@ __global__ void __launch_bounds__(32 * kWarpsPerCta) prefill_simt_kernel(
     kv_len = max_blocks_per_seq * kPageSize;
   }
   const int pos = __ldg(positions + tok);
-  int n_keys = min(kv_len, pos + 1);
-  // Window: the visible keys are the first `front` and those from front + gap on; c-th visible key -> key.
-  int front = 0, gap = 0;
-  if constexpr (kWindow) {
-    n_keys = max(n_keys, 0);
-    front = min(sinks, n_keys);
-    const int near = pos >= window ? pos - window + 1 : 0;
-    gap = min(max(near, front), n_keys) - front;
-    n_keys -= gap;
-  }
-  auto key_of = [&](int c) { return kWindow && c >= front ? c + gap : c; };
+  const int n_keys = min(kv_len, pos + 1);
   const float scale = kLog2e * rsqrtf(float(D));
   const T* qrow = q + tok * lay.q_ts + int64_t(head) * lay.q_hs;
   for (int d = lane; d < D; d += 32) qsh[warp][d] = Elem<T>::to_f(qrow[d]) * scale;
@@ -80,9 +70,9 @@ __global__ void __launch_bounds__(32 * kWarpsPerCta) prefill_simt_kernel(
 #pragma unroll
   for (int i = 0; i < kDPL; ++i) acc[i] = 0.f;
   for (int j0 = 0; j0 < n_keys; j0 += 32) {
-    const int j = key_of(j0 + lane);
+    const int j = j0 + lane;
     float sc = -INFINITY;
-    if (j0 + lane < n_keys) {
+    if (j < n_keys) {
       int blk = __ldg(table + j / kPageSize);
       if (blk < 0 || blk >= num_blocks) {
         record_error(err, FVB_ERR_BAD_PAGE, s);
@@ -105,7 +95,7 @@ __global__ void __launch_bounds__(32 * kWarpsPerCta) prefill_simt_kernel(
     __syncwarp();
     const int nk = min(32, n_keys - j0);
     for (int t = 0; t < nk; ++t) {
-      const int jj = key_of(j0 + t);
+      const int jj = j0 + t;
       int blk = __ldg(table + jj / kPageSize);
       if (blk < 0 || blk >= num_blocks) blk = 0;
       const T* vr = v_pool + ((int64_t(blk) * n_kv_heads + kvh) * kPageSize + (jj % kPageSize)) * D;
@@ -134,7 +124,7 @@ cudaError_t launch_simt_t(const void* q, void* out, const void* k_pool, const vo
     kern<<<unsigned(blocks), 32 * kWarpsPerCta, 0, stream>>>(
         static_cast<const T*>(q), static_cast<T*>(out), static_cast<const T*>(k_pool),
         static_cast<const T*>(v_pool), num_blocks, n_heads, n_kv_heads, num_seqs, q_len_flatten, cu_seqlens,
-        block_tables, max_blocks_per_seq, kv_lens, positions, lay, err, 0, 0);
+        block_tables, max_blocks_per_seq, kv_lens, positions, lay, err);
   };
   if (head_dim == 128) args(prefill_simt_kernel<T, 128>);
   else args(prefill_simt_kernel<T, 64>);
@@ -142,25 +132,6 @@ cudaError_t launch_simt_t(const void* q, void* out, const void* k_pool, const vo
 }
 
 }  // namespace
-
-cudaError_t launch_window_prefill_simt(const void* q, void* out, const void* k_pool, const void* v_pool,
-                                       int64_t num_blocks, int n_heads, int n_kv_heads, int head_dim, int num_seqs,
-                                       int64_t q_len_flatten, const int32_t* cu_seqlens, const int32_t* block_tables,
-                                       int max_blocks_per_seq, const int32_t* kv_lens, const int32_t* positions,
-                                       int window, int sinks, const QOLayout& lay, int* err, cudaStream_t stream) {
-  if (q_len_flatten == 0 || num_seqs == 0) return cudaSuccess;
-  const int64_t blocks = (int64_t(n_heads) * q_len_flatten + kWarpsPerCta - 1) / kWarpsPerCta;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-  auto launch = [&](auto kern) {
-    kern<<<unsigned(blocks), 32 * kWarpsPerCta, 0, stream>>>(
-        static_cast<const float*>(q), static_cast<float*>(out), static_cast<const float*>(k_pool),
-        static_cast<const float*>(v_pool), num_blocks, n_heads, n_kv_heads, num_seqs, q_len_flatten, cu_seqlens,
-        block_tables, max_blocks_per_seq, kv_lens, positions, lay, err, window, sinks);
-  };
-  if (head_dim == 128) launch(prefill_simt_kernel<float, 128, true>);
-  else launch(prefill_simt_kernel<float, 64, true>);
-  return cudaGetLastError();
-}
 
 cudaError_t launch_prefill_simt(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
                                 int n_heads, int n_kv_heads, int head_dim, int num_seqs, int64_t q_len_flatten,

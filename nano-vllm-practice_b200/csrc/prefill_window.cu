@@ -11,7 +11,9 @@ cudaError_t dispatch(int nrep, const void* q, void* out, const void* k_pool, con
                      const int32_t* block_tables, int max_blocks_per_seq, const int32_t* kv_lens, int kv_cap,
                      const int32_t* positions, const PrefillPlan& plan, const QOLayout& lay, void* ws, int* err,
                      cudaStream_t stream, const DecodeExtra& ex) {
-#define FVB_TW_ARGS q, out, k_pool, v_pool, num_blocks, n_kv_heads, num_seqs, q_len_flatten, cu_seqlens, block_tables,                     max_blocks_per_seq, kv_lens, kv_cap, positions, plan, lay, nrep, 0, 1, nullptr, nullptr, ws, err,                     stream, ex
+#define FVB_TW_ARGS q, out, k_pool, v_pool, num_blocks, n_kv_heads, num_seqs, q_len_flatten, cu_seqlens, block_tables, \
+                    max_blocks_per_seq, kv_lens, kv_cap, positions, plan, lay, nrep, 0, 1, nullptr, nullptr, ws, err, \
+                    stream, ex
   switch (tc_tile_heads(nrep)) {
     case 1:
       return launch_tc<T, D, 1, false, kTcWindow>(FVB_TW_ARGS);

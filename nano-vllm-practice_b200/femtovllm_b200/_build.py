@@ -63,6 +63,7 @@ CU_SOURCES = [
     "prefill_simt.cu",
     "prefill_sm100.cu",
     "prefill_window.cu",
+    "prefill_f32.cu",
     "shared_prefix.cu",
     "shared_prefix_tc.cu",
 ]
