@@ -33,8 +33,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 128;
-constexpr int kRows = 64;   // query rows of a tile
+constexpr int kThreads = 256;
 constexpr int kKeys = 64;   // keys of a tile, four pages
 constexpr int kPagesPerTile = kKeys / kPageSize;
 constexpr int kFewRows = 16;
@@ -51,14 +50,15 @@ struct F32Args {
   int* err;
 };
 
-template <int D>
+// ROWS: query rows of a tile, 64 or 32.
+template <int D, int ROWS>
 struct Smem {
-  static constexpr int kQ = 0;                          // [64][D], 16-byte chunk c of row r at c ^ (r & 1)
-  static constexpr int kK = kQ + kRows * D;             // [64][D], at c ^ (r & 7); at the end the split's O
+  static constexpr int kQ = 0;                          // [ROWS][D], 16-byte chunk c of row r at c ^ (r & 1)
+  static constexpr int kK = kQ + ROWS * D;              // [64][D], at c ^ (r & 7); at the end the split's O
   static constexpr int kV = kK + kKeys * D;             // [64][D]
-  static constexpr int kP = kV + kKeys * D;             // [64][64], at c ^ 4 (r & 1)
-  static constexpr int kStats = kP + kRows * kKeys;     // (m, l) of the split's rows
-  static constexpr int kMeta = kStats + 2 * kRows;      // sequence, first row, rows, earliest and latest position
+  static constexpr int kP = kV + kKeys * D;             // [ROWS][64], at c ^ 4 (r & 1)
+  static constexpr int kStats = kP + ROWS * kKeys;      // (m, l) of the split's rows
+  static constexpr int kMeta = kStats + 2 * ROWS;       // sequence, first row, rows, earliest and latest position
   static constexpr int kFloats = kMeta + 16;
   static constexpr int kBytes = kFloats * 4;
 };
@@ -70,14 +70,14 @@ __device__ __forceinline__ void copy16(float* dst, const float* src, bool live) 
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void wait_copies_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 
-// The tile of one CTA: R rows a thread (R = kRows / 8, or 2 for at most kFewRows rows).
-template <int D, int R>
+// The tile of one CTA, R rows a thread: ROWS / 16, or 1 for at most kFewRows rows.
+template <int D, int ROWS, int R>
 __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq, int kvh, int64_t tok0, int row0,
                                             int n_rows, int kv_len, const KeySpan span, int first_seen, int split,
                                             int splits) {
   constexpr int kChunks = D / 4;    // 16-byte chunks of a row
   constexpr int kVC = D / 64;       // chunks of V (and O) a thread holds
-  using S = Smem<D>;
+  using S = Smem<D, ROWS>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, col = lane & 15;
   const int my_row = warp * 2 * R + half;  // its rows: my_row + 2 i
   const int32_t* table = a.block_tables + int64_t(seq) * a.max_blocks_per_seq;
@@ -89,7 +89,7 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
     pos[i] = row < n_rows ? __ldg(a.positions + tok0 + (row0 + row) / a.group) : -1;
   }
   const float scale = kLog2e * rsqrtf(float(D));
-  for (int x = threadIdx.x; x < 8 * R * kChunks; x += kThreads) {
+  for (int x = threadIdx.x; x < kThreads / 16 * R * kChunks; x += kThreads) {
     const int row = x / kChunks, c = x % kChunks;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (row < n_rows) {
@@ -139,13 +139,14 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
     }
   };
 
-  float m[R], l[R], o[R][4 * kVC];
+  float m[R], l[R];
+  float2 o[R][2 * kVC];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int d = 0; d < 4 * kVC; ++d) o[i][d] = 0.f;
+    for (int d = 0; d < 2 * kVC; ++d) o[i][d] = make_float2(0.f, 0.f);
   }
   int id[kPagesPerTile];
   read_ids(t_begin);
@@ -163,11 +164,11 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
     wait_copies_but_one();
     __syncthreads();  // K (and, the first time, Q) is there
     // ---- S: keys col + 16 j ----
-    float s[R][4];
+    float2 s2[R][4];  // even and odd dims
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+      for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
     for (int c = 0; c < kChunks; ++c) {
       float4 kv[4];
@@ -179,13 +180,16 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
         const float4 qv = *reinterpret_cast<const float4*>(qp + 2 * i * D + ((c ^ (my_row & 1)) << 2));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[i][j] = fmaf(qv.x, kv[j].x, s[i][j]);
-          s[i][j] = fmaf(qv.y, kv[j].y, s[i][j]);
-          s[i][j] = fmaf(qv.z, kv[j].z, s[i][j]);
-          s[i][j] = fmaf(qv.w, kv[j].w, s[i][j]);
+          s2[i][j] = __ffma2_rn(make_float2(qv.x, qv.y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
+          s2[i][j] = __ffma2_rn(make_float2(qv.z, qv.w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
         }
       }
     }
+    float s[R][4];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
     __syncthreads();  // K is read
     check_ids(id);
     if (t + 1 < t_end) copy_tile(a.k_pool, sm + S::kK, id, t + 1, true);
@@ -212,7 +216,7 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
       m[i] = next;
       l[i] *= f;
 #pragma unroll
-      for (int d = 0; d < 4 * kVC; ++d) o[i][d] *= f;
+      for (int d = 0; d < 2 * kVC; ++d) o[i][d] = __fmul2_rn(o[i][d], make_float2(f, f));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float p = fast_exp2(s[i][j] - ref);
@@ -239,10 +243,8 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
 #pragma unroll
           for (int i = 0; i < R; ++i) {
             const float p = kk == 0 ? pv[i].x : kk == 1 ? pv[i].y : kk == 2 ? pv[i].z : pv[i].w;
-            o[i][4 * x + 0] = fmaf(p, vv.x, o[i][4 * x + 0]);
-            o[i][4 * x + 1] = fmaf(p, vv.y, o[i][4 * x + 1]);
-            o[i][4 * x + 2] = fmaf(p, vv.z, o[i][4 * x + 2]);
-            o[i][4 * x + 3] = fmaf(p, vv.w, o[i][4 * x + 3]);
+            o[i][2 * x] = __ffma2_rn(make_float2(p, p), make_float2(vv.x, vv.y), o[i][2 * x]);
+            o[i][2 * x + 1] = __ffma2_rn(make_float2(p, p), make_float2(vv.z, vv.w), o[i][2 * x + 1]);
           }
         }
       }
@@ -262,7 +264,7 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
 #pragma unroll
       for (int x = 0; x < kVC; ++x)
         *reinterpret_cast<float4*>(sm + S::kK + row * D + 4 * col + 64 * x) =
-            make_float4(o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]);
+            make_float4(o[i][2 * x].x, o[i][2 * x].y, o[i][2 * x + 1].x, o[i][2 * x + 1].y);
       if (col == 0) *reinterpret_cast<float2*>(sm + S::kStats + 2 * row) = make_float2(m[i], l[i]);
     } else if (row < n_rows) {
       const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];  // (a NaN stays one)
@@ -272,15 +274,15 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
 #pragma unroll
       for (int x = 0; x < kVC; ++x)
         *reinterpret_cast<float4*>(dst + 4 * col + 64 * x) = make_float4(
-            o[i][4 * x] * inv, o[i][4 * x + 1] * inv, o[i][4 * x + 2] * inv, o[i][4 * x + 3] * inv);
+            o[i][2 * x].x * inv, o[i][2 * x].y * inv, o[i][2 * x + 1].x * inv, o[i][2 * x + 1].y * inv);
     }
   }
 }
 
-template <int D>
+template <int D, int ROWS>
 __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) window_prefill_f32_kernel(const F32Args a) {
   extern __shared__ __align__(16) float sm[];
-  using S = Smem<D>;
+  using S = Smem<D, ROWS>;
   int* meta = reinterpret_cast<int*>(sm + S::kMeta);
   const cg::cluster_group cluster = cg::this_cluster();
   const int splits = int(cluster.num_blocks()), split = int(cluster.block_rank());
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) window_prefill_f32
         hi = min(max(int64_t(__ldg(a.cu_seqlens + s + 1)), lo), a.q_len_flatten);
       }
       const int64_t n = (hi - lo) * a.group;
-      const int64_t mine = (n + kRows - 1) / kRows;
+      const int64_t mine = (n + ROWS - 1) / ROWS;
       int64_t sum = mine;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
@@ -312,11 +314,11 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) window_prefill_f32
       const unsigned found = __ballot_sync(0xffffffffu, here);
       if (found != 0) {
         const int src = __ffs(found) - 1;
-        const int64_t row = (tile - begin) * kRows;
+        const int64_t row = (tile - begin) * ROWS;
         seq = s0 + src;
         // (its place inside the sequence: a row takes 256 bytes or more, so fewer than 2^31 of them fit a device)
         first = __shfl_sync(0xffffffffu, int(row), src);
-        rows = __shfl_sync(0xffffffffu, int(min(n - row, int64_t(kRows))), src);
+        rows = __shfl_sync(0xffffffffu, int(min(n - row, int64_t(ROWS))), src);
         if (lane == src) {
           meta[0] = seq;
           meta[1] = int(lo);
@@ -359,9 +361,9 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) window_prefill_f32
   kv_len = max(0, high < kv_len ? high + 1 : kv_len);  // keys that some row sees end here
   const KeySpan span = window_span(low + 1, kv_len, a.window, a.sinks, kPageSize);
   if (n_rows <= kFewRows)
-    attend_tile<D, 2>(a, sm, seq, kvh, tok0, row0, n_rows, kv_len, span, span.lo, split, splits);
+    attend_tile<D, ROWS, kFewRows * 16 / kThreads>(a, sm, seq, kvh, tok0, row0, n_rows, kv_len, span, span.lo, split, splits);
   else
-    attend_tile<D, kRows / 8>(a, sm, seq, kvh, tok0, row0, n_rows, kv_len, span, span.lo, split, splits);
+    attend_tile<D, ROWS, ROWS * 16 / kThreads>(a, sm, seq, kvh, tok0, row0, n_rows, kv_len, span, span.lo, split, splits);
   if (splits == 1) return;
   // ---- join: CTA r of the cluster takes rows r, r + splits, ... ----
   cluster.sync();
@@ -396,16 +398,17 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) window_prefill_f32
   cluster.sync();  // no CTA leaves while another reads its shared memory
 }
 
-template <int D>
+template <int D, int ROWS>
 cudaError_t launch_t(const F32Args& a, int64_t tiles, int splits, cudaStream_t stream) {
-  const cudaError_t ce = set_smem_once<window_prefill_f32_kernel<D>>(Smem<D>::kBytes);
+  using S = Smem<D, ROWS>;
+  const cudaError_t ce = set_smem_once<window_prefill_f32_kernel<D, ROWS>>(S::kBytes);
   if (ce != cudaSuccess) return ce;
   const int64_t ctas = tiles * a.n_kv_heads * splits;
   if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ctas));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Smem<D>::kBytes;
+  cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -414,7 +417,7 @@ cudaError_t launch_t(const F32Args& a, int64_t tiles, int splits, cudaStream_t s
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, window_prefill_f32_kernel<D>, a);
+  return cudaLaunchKernelEx(&cfg, window_prefill_f32_kernel<D, ROWS>, a);
 }
 
 }  // namespace
@@ -445,17 +448,22 @@ cudaError_t launch_window_prefill_f32(const void* q, void* out, const void* k_po
   a.positions = positions;
   a.lay = lay;
   a.err = err;
-  // A sequence's last tile is ragged, so the batch has at most this many.
-  const int64_t tiles = q_len_flatten * a.group / kRows + num_seqs;
+  // A sequence's last tile is ragged, so the batch has at most this many.  Tiles of 32 rows where the SMs hold those of
+  // 64 at once: what one tile takes is then the call's time (about 2 / 3 of it).
+  const int places = device_sm_count() * (head_dim == 128 ? 2 : 3);
+  auto tiles_of = [&](int rows) { return q_len_flatten * a.group / rows + num_seqs; };
+  const int rows = tiles_of(64) * n_kv_heads > device_sm_count() ? 64 : 32;
+  const int64_t tiles = tiles_of(rows);
   // As many CTAs share a tile's keys as leave each two tiles of them and fill the SMs' places once.
   const int64_t kv_cap = std::min<int64_t>(int64_t(max_blocks_per_seq) * kPageSize, 0x7fffffff);
-  const int tokens = std::min(max_q_len, (kRows + a.group - 2) / a.group + 1);  // of a tile at most
+  const int tokens = std::min(max_q_len, (rows + a.group - 2) / a.group + 1);  // of a tile at most
   const int64_t keys = std::min<int64_t>(kv_cap, int64_t(window) + tokens - 1);
   const int key_tiles = window_max_units(int(kv_cap), int(std::max<int64_t>(1, keys)), sinks, kPageSize) / kPagesPerTile;
-  const int places = device_sm_count() * (head_dim == 128 ? 2 : 3);
   int splits = 1;
   while (splits < kMaxSplits && tiles * n_kv_heads * splits * 2 <= places && key_tiles >= splits * 4) splits *= 2;
-  return head_dim == 128 ? launch_t<128>(a, tiles, splits, stream) : launch_t<64>(a, tiles, splits, stream);
+  if (rows == 64)
+    return head_dim == 128 ? launch_t<128, 64>(a, tiles, splits, stream) : launch_t<64, 64>(a, tiles, splits, stream);
+  return head_dim == 128 ? launch_t<128, 32>(a, tiles, splits, stream) : launch_t<64, 32>(a, tiles, splits, stream);
 }
 
 }  // namespace fvb
