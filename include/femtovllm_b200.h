@@ -344,7 +344,8 @@ FVB_API int fvb_paged_attention_shared_prefix_decode(
  * last, in the same order.  finished (one byte per row, may be NULL): a beam with a nonzero entry has the
  * single continuation eos_token_id at scores[r], and its logits are not read.
  * num_beams and num_select 1 to 64, num_select <= num_beams * vocab, at most 1024 parts of 131072 logits a
- * request (num_beams * ceil(vocab / 131072)), rows at any element alignment.  Sums in fp32, the order of the beams' candidates decided in fp64.
+ * request (num_beams * ceil(vocab / 131072)), rows at any element alignment.  Sums in fp32, the order of the
+ * beams' candidates decided in fp64.
  * workspace: fvb_beam_search_workspace_size bytes, 256-byte aligned, no initial value.  Two launches.
  */
 FVB_API size_t fvb_beam_search_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select,

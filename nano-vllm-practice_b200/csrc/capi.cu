@@ -587,6 +587,11 @@ int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_stride, in
   if (!cu_seqlens || !positions) return FVB_ERR_INVALID_ARGUMENT;
   if (q_len_flatten > int64_t(0x7fffffff) || int64_t(max_blocks_per_seq) * kPageSize > fvb_max_kv_len())
     return FVB_ERR_UNSUPPORTED;
+  const PrefillPlan plan = plan_prefill(num_seqs, n_heads, n_kv_heads, head_dim, q_len_flatten, max_q_len, dtype);
+  if (dtype != FVB_DTYPE_F32) {  // (fp32 keeps nothing outside shared memory)
+    if (!workspace || workspace_bytes < plan.ws_bytes) return FVB_ERR_WORKSPACE_TOO_SMALL;
+    if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;
+  }
   cudaError_t e;
   int* err = device_error_ptr(&e);
   if (!err) return cuda_status(e);
@@ -596,9 +601,6 @@ int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_stride, in
                                                  num_seqs, q_len_flatten, max_q_len, cu_seqlens, block_tables,
                                                  max_blocks_per_seq, kv_lens, positions, window, num_sinks, lay, err,
                                                  s));
-  const PrefillPlan plan = plan_prefill(num_seqs, n_heads, n_kv_heads, head_dim, q_len_flatten, max_q_len, dtype);
-  if (!workspace || workspace_bytes < plan.ws_bytes) return FVB_ERR_WORKSPACE_TOO_SMALL;
-  if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;
   return cuda_status(launch_window_prefill(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim,
                                            num_seqs, q_len_flatten, cu_seqlens, block_tables, max_blocks_per_seq,
                                            kv_lens, positions, window, num_sinks, dtype, plan, lay, workspace, err,

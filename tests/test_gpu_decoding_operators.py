@@ -1,0 +1,204 @@
+"""The window and beam operators where another kernel, tile or path takes over, against the plain forms in 64 bits."""
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import cabi
+import ref64
+from femtovllm_b200 import capi, ops, workloads
+from test_gpu_beam import check as check_select
+from test_gpu_window import GQA, _decode, _prefill
+
+pytestmark = pytest.mark.gpu
+
+
+def _workspace(b, window, sinks):
+    return cabi.lib().fvb_paged_attention_window_decode_workspace_size(
+        len(b.kv_lens), b.q.shape[0], b.k_pool.shape[1], b.q.shape[2], b.max_kv_len, window, sinks)
+
+
+@pytest.mark.parametrize("n_rep", GQA)
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_window_decode_of_a_crowd(head_dim, n_rep, cuda_device):
+    """Enough pages an SM for the tensor-core kernel, units of one tile to three, cut wherever the SMs' shares end."""
+    dtype = torch.float16 if n_rep % 2 else torch.bfloat16
+    lens = np.random.default_rng(n_rep).integers(1, 260, size=1024)
+    lens[:20] = [1, 2, 15, 16, 17, 31, 32, 33, 127, 128, 129, 130, 255, 256, 257, 1, 1, 1, 259, 259]
+    b = workloads.custom(lens, np.ones(1024), 8 * n_rep, 8, head_dim, dtype, seed=n_rep).materialize(cuda_device)
+    for i, (window, sinks) in enumerate([(33, 1), (17, 20), (1 << 30, 0)]):
+        assert _workspace(b, window, sinks) > 0  # (the split-KV kernel would take one split and keep no partials)
+        _decode(b, window, sinks, drop=i % 2 == 0)
+
+
+@pytest.mark.parametrize("n_rep", [1, 8])
+def test_window_decode_at_the_border_between_the_kernels(n_rep, cuda_device):
+    """The same sequences in batches on either side of the rule, and of the largest table."""
+    for n in (290, 1024, 1025, 1100):
+        lens = np.random.default_rng(n).integers(1, 90, size=n)
+        b = workloads.custom(lens, np.ones(n), 8 * n_rep, 8, 64, torch.bfloat16, seed=n).materialize(cuda_device)
+        _decode(b, 20, 3)
+
+
+def test_window_decode_with_empty_sequences_in_a_crowd(cuda_device):
+    lens = np.random.default_rng(5).integers(1, 400, size=600)
+    b = workloads.custom(lens, np.ones(600), 16, 8, 128, torch.bfloat16, seed=5).materialize(cuda_device)
+    tables = torch.from_numpy(b.block_tables).to(cuda_device)
+    kv = torch.from_numpy(b.kv_lens).to(cuda_device)
+    kv[::7] = 0
+    got = ops.paged_attention_window_gemv(b.q, b.k_pool, b.v_pool, tables, kv, 400, 300, 2)
+    ref64.check_attention(got, ref64.attention(b.q, b.k_pool, b.v_pool, tables, kv, window=300, sinks=2))
+    assert (got[:, ::7] == 0).all()
+
+
+# ------------------------------------------------------------------ fp32 prefill
+
+
+@pytest.mark.parametrize("n_rep", [1, 3, 8, 16])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_fp32_prefill_keys_shared_by_a_cluster(head_dim, n_rep, cuda_device):
+    b = workloads.custom([9000, 700, 5003], [40, 1, 16], n_rep, 1, head_dim, torch.float32, seed=1).materialize(cuda_device)
+    for window, sinks in [(1 << 30, 0), (4096, 130), (33, 7000), (600, 0), (1, 0)]:
+        _prefill(b, window, sinks)
+
+
+@pytest.mark.parametrize("n_rep", [1, 5])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_fp32_prefill_large_tiles(head_dim, n_rep, cuda_device):
+    q_lens = np.array([900, 1, 64, 63, 65, 450, 16, 17, 2])
+    kv = q_lens + np.array([300, 800, 0, 64, 1, 0, 15, 100, 31])
+    b = workloads.custom(kv, q_lens, 8 * n_rep, 8, head_dim, torch.float32, seed=2).materialize(cuda_device)
+    for window, sinks in [(200, 4), (1000, 0), (15, 70)]:
+        _prefill(b, window, sinks, drop=False)
+
+
+def test_fp32_prefill_scores_far_apart_and_infinite(cuda_device):
+    """Rows whose running maximum moves by thousands, keys whose score is -inf, and one whose score is +inf (NaN out)."""
+    b = workloads.custom([300, 90], [200, 1], 4, 2, 64, torch.float32, seed=3).materialize(cuda_device)
+    b.q.mul_(40)
+    _prefill(b, 128, 4)
+    md = b.device_metadata(cuda_device)
+    k = b.k_pool.clone()
+    page = int(b.block_tables[0, 3])
+    k[page, :, 5] = -math.inf  # key 53 of the first sequence: scores of -inf, +inf or NaN, by the query
+    q = b.q.abs()              # here -inf for every query
+    got = ops.paged_attention_window_gemm(q, k, b.v_pool, md["cu_seqlens"], 200, md["block_tables"], md["kv_lens"],
+                                          md["positions"], 128, 0)
+    small = k.clone()
+    small[page, :, 5] = -3e30  # below every other score by far: the same weights
+    same = ops.paged_attention_window_gemm(q, small, b.v_pool, md["cu_seqlens"], 200, md["block_tables"],
+                                           md["kv_lens"], md["positions"], 128, 0)
+    assert torch.equal(got, same) and torch.isfinite(got).all()
+    k[page, :, 5] = math.inf
+    got = ops.paged_attention_window_gemm(q, k, b.v_pool, md["cu_seqlens"], 200, md["block_tables"], md["kv_lens"],
+                                          md["positions"], 128, 0)
+    sees = (md["positions"][:200] >= 53) & (md["positions"][:200] < 53 + 128)
+    assert torch.isnan(got[:, :200][:, sees]).all() and torch.isfinite(got[:, :200][:, ~sees]).all()
+    assert torch.isfinite(got[:, 200:]).all()
+
+
+@pytest.mark.parametrize("dtype,n_rep", [(torch.float32, 2), (torch.bfloat16, 2), (torch.bfloat16, 8)])
+def test_window_prefill_leaves_rows_behind_the_last_sequence(dtype, n_rep, cuda_device):
+    b = workloads.custom([100, 30, 40], [60, 1, 7], 2 * n_rep, 2, 64, dtype, seed=4).materialize(cuda_device)
+    md = b.device_metadata(cuda_device)
+    hq, t, d = b.q.shape
+    q = torch.cat([b.q, b.q[:, :5]], 1).contiguous()
+    out = torch.full_like(q, 7.0)
+    lib = cabi.lib()
+    need = lib.fvb_paged_attention_prefill_workspace_size(3, hq, 2, d, t + 5, 60)
+    ws = torch.empty(max(need, 256), dtype=torch.uint8, device=cuda_device)
+    capi.check(lib.fvb_paged_attention_window_prefill(
+        q.data_ptr(), d, (t + 5) * d, out.data_ptr(), d, (t + 5) * d, b.k_pool.data_ptr(), b.v_pool.data_ptr(),
+        b.k_pool.shape[0], hq, 2, d, 16, 3, t + 5, md["cu_seqlens"].data_ptr(), 60, md["block_tables"].data_ptr(),
+        md["block_tables"].shape[1], md["kv_lens"].data_ptr(), md["positions"].data_ptr(), 50, 3,
+        capi.dtype_code(dtype), ws.data_ptr(), need, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)), "window")
+    ref64.check_attention(out[:, :t], ref64.attention(b.q, b.k_pool, b.v_pool, md["block_tables"], md["kv_lens"],
+                                                      md["cu_seqlens"], md["positions"], 50, 3))
+    assert (out[:, t:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_window_prefill_reports_bad_pages_and_long_contexts(dtype, cuda_device):
+    b = workloads.custom([100, 50], [20, 50], 4, 2, 64, dtype, seed=6).materialize(cuda_device)
+    md = b.device_metadata(cuda_device)
+
+    def run(tables, lens):
+        ops.paged_attention_window_gemm(b.q, b.k_pool, b.v_pool, md["cu_seqlens"], 50, tables, lens, md["positions"],
+                                        30, 0)
+        return ops.read_device_error()
+
+    assert run(md["block_tables"], md["kv_lens"]) == (0, 0)
+    for bad in (-1, -2, b.k_pool.shape[0], 1 << 30):
+        tables = md["block_tables"].clone()
+        tables[0, 5] = bad
+        assert run(tables, md["kv_lens"]) == (7, 0)
+        tables = md["block_tables"].clone()
+        tables[0, 1] = bad  # keys 16 to 31: behind every query's window
+        assert run(tables, md["kv_lens"]) == (0, 0)
+    longer = md["kv_lens"].clone()
+    longer[1] = 16 * md["block_tables"].shape[1] + 1
+    assert run(md["block_tables"], longer) == (1, 1)
+
+
+def test_fp32_window_prefill_in_two_graphs_and_beside_them(cuda_device):
+    b = workloads.custom([900, 300], [100, 40], 8, 2, 128, torch.float32, seed=7).materialize(cuda_device)
+    md = b.device_metadata(cuda_device)
+
+    def run(window):
+        return ops.paged_attention_window_gemm(b.q, b.k_pool, b.v_pool, md["cu_seqlens"], 100, md["block_tables"],
+                                               md["kv_lens"], md["positions"], window, 2)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(64)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for window in (64, 700):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run(window)
+        graphs.append((g, out, window))
+    for _ in range(2):
+        b.q.normal_()
+        torch.cuda.synchronize()
+        for g, _, _ in graphs:
+            g.replay()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            beside = run(700)
+        torch.cuda.synchronize()
+        for _, out, window in graphs:
+            assert torch.equal(out, run(window))
+        assert torch.equal(beside, run(700))
+    graphs.clear()
+
+
+# ------------------------------------------------------------------ beam selection
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_select_with_the_largest_logits_in_few_threads(dtype, cuda_device):
+    """Rows of one part each whose thousands of largest logits lie with a few lanes: the bound misses them."""
+    n, w, v = 150, 4, 100000
+    gen = torch.Generator(device=cuda_device).manual_seed(3)
+    logits = torch.randn(n * w, v, generator=gen, device=cuda_device)
+    per = 128 // torch.finfo(dtype).bits  # logits of a vector
+    high = (torch.arange(v, device=cuda_device) // per) % 128 < 7
+    logits[:, high] += 12
+    scores = -torch.rand(n, w, generator=gen, device=cuda_device)
+    check_select(logits.to(dtype), scores, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("v", [1420, 8200, 16500, 17823, 50001])
+def test_select_with_short_last_parts(dtype, v, cuda_device):
+    """Vocabularies whose parts end in a few vectors, at every alignment of the rows and for many and few of them."""
+    gen = torch.Generator(device=cuda_device).manual_seed(v)
+    for n, w, k in [(1, 10, 10), (3, 16, 32), (25, 10, 20), (1, 1, 64), (60, 10, 33)]:
+        logits = (torch.randn(n * w, v, generator=gen, device=cuda_device) * 2.5).to(dtype)
+        logits[:, v - 40:] += 3  # the short part holds some of the best
+        check_select(logits, -torch.rand(n, w, generator=gen, device=cuda_device) * 5, k)
