@@ -320,7 +320,7 @@ FVB_API int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_st
  * Group g is sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int32, num_groups + 1 ascending entries within
  * [0, num_seqs]; sequences outside every group share nothing).  The caller says that the table rows of a
  * group agree in their first prefix_lens[g] / 16 pages; those pages are read through the row of the group's
- * first sequence, whatever its kv_len.  prefix_lens[g] need not be a multiple of 16 nor below every
+ * first sequence, whatever its kv_len, or, by calls too small to gain from sharing, through each one's own.  prefix_lens[g] need not be a multiple of 16 nor below every
  * kv_len of the group; max_prefix_len bounds it (keys past it are read per sequence).
  * Malformed groups are recorded in the device error word and never read out of bounds.
  * max_kv_len at most fvb_max_kv_len(); workspace 256-byte aligned.

@@ -639,7 +639,7 @@ int fvb_paged_attention_shared_prefix_decode(
   if (num_groups > kMaxGridYZ || int64_t(n_heads) > kMaxGridYZ) return FVB_ERR_UNSUPPORTED;
   const SharedPrefixPlan plan = plan_shared_prefix(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, num_groups,
                                                    max_prefix_len, dtype, device_sm_count());
-  if (!workspace || workspace_bytes < plan.ws_bytes) return FVB_ERR_WORKSPACE_TOO_SMALL;
+  if (plan.ws_bytes > 0 && (!workspace || workspace_bytes < plan.ws_bytes)) return FVB_ERR_WORKSPACE_TOO_SMALL;
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return FVB_ERR_MISALIGNED;
   cudaError_t e;
   int* err = device_error_ptr(&e);

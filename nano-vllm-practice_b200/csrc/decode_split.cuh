@@ -160,6 +160,14 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_split_kernel(
   const int2 members = kPre ? group_rows(ex, blockIdx.z, num_seqs) : make_int2(0, 0);
   const int split = kPre ? blockIdx.x % max_splits : blockIdx.x, kvh = kPre ? blockIdx.y : blockIdx.y / chunks,
             chunk = kPre ? blockIdx.x / max_splits : blockIdx.y % chunks;
+  if (MODE == kDecodeWindow && ex.num_groups > 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
+    // A shared-prefix call that shares nothing (shared_prefix.cu) still tells of malformed groups.
+    for (int g = threadIdx.x; g < ex.num_groups; g += blockDim.x) {
+      const int lo = __ldg(ex.cu_groups + g), hi = __ldg(ex.cu_groups + g + 1);
+      if (lo < 0 || hi < lo || hi > num_seqs || __ldg(ex.prefix_lens + g) < 0)
+        record_error(err, FVB_ERR_INVALID_ARGUMENT, g);
+    }
+  }
   const int4 range = MODE == kDecodeRest ? __ldcg(ex.items + blockIdx.x) : make_int4(0, 0, 0, 0);
   if (MODE == kDecodeRest && range.x < 0) return;
   const int b = kPre ? members.x : MODE == kDecodeRest ? range.x : int(blockIdx.z);

@@ -56,10 +56,9 @@ cudaError_t launch_window_decode(const void* q, void* out, const void* k_pool, c
                                  int n_heads, int n_kv_heads, int head_dim, int num_seqs, const int32_t* block_tables,
                                  int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len, int window, int sinks,
                                  int dtype, const DecodePlan& plan, const QOLayout& lay, void* workspace, int* err,
-                                 cudaStream_t stream, const int32_t* q_index, const int32_t* q_pos) {
+                                 cudaStream_t stream, const int32_t* q_index, const int32_t* q_pos, DecodeExtra ex) {
   if (num_seqs == 0) return cudaSuccess;
   const int nrep = n_heads / n_kv_heads;
-  DecodeExtra ex;
   ex.window = window;
   ex.sinks = sinks;
 #define FVB_DW_ARGS nrep, q, out, k_pool, v_pool, num_blocks, n_kv_heads, num_seqs, block_tables, \

@@ -162,7 +162,7 @@ cudaError_t launch_window_decode(const void* q, void* out, const void* k_pool, c
                                  int max_blocks_per_seq, const int32_t* kv_lens, int max_kv_len, int window, int sinks,
                                  int dtype, const DecodePlan& plan, const QOLayout& lay, void* workspace, int* err,
                                  cudaStream_t stream, const int32_t* q_index = nullptr,
-                                 const int32_t* q_pos = nullptr);
+                                 const int32_t* q_pos = nullptr, DecodeExtra ex = DecodeExtra{});
 cudaError_t launch_window_prefill(const void* q, void* out, const void* k_pool, const void* v_pool, int64_t num_blocks,
                                   int n_heads, int n_kv_heads, int head_dim, int num_seqs, int64_t q_len_flatten,
                                   const int32_t* cu_seqlens, const int32_t* block_tables, int max_blocks_per_seq,
@@ -203,6 +203,8 @@ cudaError_t launch_keys_decode(const void* q, void* out, const void* k_pool, con
 // shared_prefix_tc.cu), every sequence's own keys by the split-KV kernel, and the partials
 // of both are merged.
 struct SharedPrefixPlan {
+  bool direct;         // every sequence reads all its keys itself (dp, the split-KV kernel), nothing is shared
+  DecodePlan dp;
   int keys_per_split;  // of a prefix; 0 = no prefix to share
   int prefix_splits;   // prefix partials per (sequence, head)
   bool single_tiles;   // tensor cores: items of one query tile (small groups) instead of two

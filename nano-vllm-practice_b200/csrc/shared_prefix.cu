@@ -7,7 +7,8 @@
 // 2^(lse_i - m), m = max lse_i.  Here the prefix of a group is one range (or a few) that
 // all its sequences attend together, so its K and V leave HBM once per group and feed
 // 128-row tensor-core tiles of (sequence, query head) rows; the keys behind it are attended
-// per sequence, bound by HBM.  16-bit types, up to kKeysMaxSeqs sequences, three launches:
+// per sequence, bound by HBM.  Calls that are too small for that share nothing (plan_shared_prefix says where).  Else,
+// for 16-bit types and up to kKeysMaxSeqs sequences, three launches:
 //
 //   prefix   prefill_tc.cuh (kTcPrefix);
 //   rest     decode_keys.cu: the sequences' own tiles dealt evenly to one CTA per SM, as the
@@ -24,6 +25,8 @@
 //   prefix   fp32: decode_split.cuh (kDecodePrefix), else as above;
 //   rest     decode_split.cuh (kDecodeRest), one CTA per (range, kv head);
 //   merge    as above.
+#include <climits>
+
 #include "decode_split.cuh"
 
 namespace fvb {
@@ -381,6 +384,26 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
   if (num_seqs <= 0 || n_kv_heads <= 0) return p;
   const int group = n_heads / n_kv_heads;
   const int prefix = std::max(0, std::min(max_prefix_len, max_kv_len)) / kPageSize * kPageSize;
+  // Sharing takes three launches (fp32 four) that follow on one another, 10 to 14 us (17) however little there is to
+  // read.  Where an SM has few pages to read, each sequence reading its own, out of L2 for all but one of a group, is
+  // one launch of 4 to 10 us.  Which is faster goes by the pages an SM gets at most (halves of D 128 count each), and
+  // by what a page costs the split-KV kernel: over 400 calls of random shapes the choice is 1 % off the better way on
+  // average, and sharing always 40 %.  (70 sequences x 2 heads x 128 behind up to 182 keys, group 3: 18.0 us shared,
+  // 9.9 each for itself; 8 x 8 x 128 behind 2000, group 2: 12.6 and 20.3; 32 x 8 x 128 behind 4096, group 4: 32.4 and
+  // 116.)
+  const int64_t pages = std::max<int64_t>(1, (int64_t(max_kv_len) + kPageSize - 1) / kPageSize) * (head_dim / 64);
+  const int64_t direct_pages = dtype == FVB_DTYPE_F32 ? (group <= 8 ? 128 : 64)
+                               : group <= 1           ? 256
+                               : group <= 2           ? 96
+                               : group <= 4           ? 64
+                               : group <= 8           ? 28
+                                                      : 22;
+  if (int64_t(num_seqs) * n_kv_heads * pages <= direct_pages * num_sms) {
+    p.direct = true;
+    p.dp = plan_window_decode(num_seqs, n_heads, n_kv_heads, head_dim, max_kv_len, INT_MAX, 0, num_sms);
+    p.ws_bytes = p.dp.ws_bytes;
+    return p;
+  }
   p.keys = dtype != FVB_DTYPE_F32 && num_seqs <= kKeysMaxSeqs;
   int taken = 0;  // SMs that the prefix kernel holds
   if (prefix > 0 && num_groups > 0) {
@@ -409,7 +432,8 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
       const double first = double(ctas) * units * (p.single_tiles ? 1.45 : 2.5);
       const double rest = double(num_seqs) * n_kv_heads * ((group + kKeysCols - 1) / kKeysCols) *
                           ((own + kKeysTile - 1) / kKeysTile) * 1.64;
-      room = std::max<int64_t>(num_sms / 8, std::min<int64_t>(num_sms * 7 / 8, int64_t(num_sms * first / (first + rest))));
+      const int64_t share = int64_t(num_sms * first / (first + rest));
+      room = std::max<int64_t>(num_sms / 8, std::min<int64_t>(num_sms * 7 / 8, share));
     }
     const int64_t wanted = std::min<int64_t>(std::max<int64_t>(1, room / ctas), units);
     const int per = int((units + wanted - 1) / wanted);
@@ -446,6 +470,15 @@ cudaError_t launch_shared_prefix(const void* q, void* out, const void* k_pool, c
                                  int max_prefix_len, int dtype, const SharedPrefixPlan& plan, const QOLayout& lay,
                                  void* workspace, int* err, cudaStream_t stream) {
   if (num_seqs == 0) return cudaSuccess;
+  if (plan.direct) {
+    DecodeExtra ex;
+    ex.cu_groups = cu_groups;
+    ex.prefix_lens = prefix_lens;
+    ex.num_groups = num_groups;
+    return launch_window_decode(q, out, k_pool, v_pool, num_blocks, n_heads, n_kv_heads, head_dim, num_seqs,
+                                block_tables, max_blocks_per_seq, kv_lens, max_kv_len, INT_MAX, 0, dtype, plan.dp, lay,
+                                workspace, err, stream, nullptr, nullptr, ex);
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   SharedArgs a{};
   a.q = q;
@@ -495,7 +528,8 @@ cudaError_t launch_shared_prefix(const void* q, void* out, const void* k_pool, c
     m.grid = plan.kp.grid;
   }
   if (dtype == FVB_DTYPE_BF16)
-    return head_dim == 128 ? run<__nv_bfloat16, 128>(a, m, head_dim, dtype) : run<__nv_bfloat16, 64>(a, m, head_dim, dtype);
+    return head_dim == 128 ? run<__nv_bfloat16, 128>(a, m, head_dim, dtype)
+                           : run<__nv_bfloat16, 64>(a, m, head_dim, dtype);
   if (dtype == FVB_DTYPE_F16)
     return head_dim == 128 ? run<__half, 128>(a, m, head_dim, dtype) : run<__half, 64>(a, m, head_dim, dtype);
   return head_dim == 128 ? run<float, 128>(a, m, head_dim, dtype) : run<float, 64>(a, m, head_dim, dtype);

@@ -213,7 +213,8 @@ def paged_attention_shared_prefix_gemv(
     Group ``g`` is sequences ``cu_groups[g] .. cu_groups[g + 1] - 1`` (int32, ``G + 1`` ascending entries;
     sequences outside every group share nothing); the caller says that their table rows agree in the first
     ``prefix_lens[g] // 16`` pages (int32, ``G``), which are read once for the group, through its first
-    sequence's row.  The result is that of ``paged_attention_gemv`` on the same tables.
+    sequence's row (calls too small to gain from that read them per sequence).  The result is that of
+    ``paged_attention_gemv`` on the same tables.
     ``max_prefix_len`` bounds ``prefix_lens``; keys past it are read per sequence.
     """
     q = _q_view(q)

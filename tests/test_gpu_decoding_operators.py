@@ -1,4 +1,5 @@
-"""The window and beam operators where another kernel, tile or path takes over, against the plain forms in 64 bits."""
+"""The window, shared-prefix and beam operators where another kernel, tile or path takes over, against the plain forms
+in 64 bits."""
 
 import ctypes
 import math
@@ -10,6 +11,7 @@ import torch
 import cabi
 import ref64
 from femtovllm_b200 import capi, ops, workloads
+import test_gpu_shared_prefix as shared
 from test_gpu_beam import check as check_select
 from test_gpu_window import GQA, _decode, _prefill
 
@@ -175,6 +177,94 @@ def test_fp32_window_prefill_in_two_graphs_and_beside_them(cuda_device):
             assert torch.equal(out, run(window))
         assert torch.equal(beside, run(700))
     graphs.clear()
+
+
+# ------------------------------------------------------------------ shared prefixes
+
+
+def _wide(s, columns=8192):
+    """The same call with a table and a bound on kv_lens so wide that it is worth sharing."""
+    tables = torch.full((len(s["tables"]), columns), -1, dtype=torch.int32, device=s["tables"].device)
+    tables[:, : s["tables"].shape[1]] = s["tables"]
+    dtype = capi.dtype_code(s["q"].dtype)
+    hq, b, d = s["q"].shape
+    args = (b, hq, s["kp"].shape[1], d)
+    size = cabi.lib().fvb_paged_attention_shared_prefix_workspace_size
+    s = dict(s, tables=tables, max_kv=16 * columns)
+    # partials of the shared keys for every (sequence, head): more than each one's own splits would take
+    assert size(*args, s["max_kv"], len(s["prefix"]), s["max_prefix"], dtype) > 0
+    return s
+
+
+@pytest.mark.parametrize("n_rep", [1, 2, 3, 4, 5, 8, 16])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_shared_prefix_sweep_with_sharing(dtype, head_dim, n_rep, cuda_device):
+    for i, (groups, own, loners) in enumerate(shared.SHAPES):
+        shared.check(_wide(shared.make(groups, own, loners, 2 * n_rep, 2, head_dim, dtype, cuda_device, seed=i)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_shared_prefix_of_short_empty_and_skewed_sequences_with_sharing(dtype, cuda_device):
+    for seed, shorter in enumerate([{1: 5}, {0: 20, 2: 300}, {0: 0, 3: 0}, {3: 1}, {0: 0, 1: 0, 2: 0, 3: 0}]):
+        s = shared.make([(4, 500)], [1, 30], [], 8, 2, 128, dtype, cuda_device, seed=seed, shorter=shorter)
+        got = shared.check(_wide(s))
+        for b, n in shorter.items():
+            assert n > 0 or (got[:, b] == 0).all()
+    shared.check(_wide(shared.make([(20, 320)], [1], [20000], 16, 8, 128, dtype, cuda_device, seed=7)))
+    s = shared.make([(6, 400), (3, 90)], [5, 50], [7], 8, 4, 64, dtype, cuda_device, seed=3)
+    for bound in (0, 10, 100, 399):
+        shared.check(_wide(s), max_prefix=bound)
+
+
+def test_shared_prefix_of_many_sequences_and_groups_with_sharing(cuda_device):
+    bf16 = torch.bfloat16
+    shared.check(_wide(shared.make([(700, 40), (801, 33)], [1, 20, 3], [9] * 30, 4, 2, 64, bf16, cuda_device, seed=5), 512))
+    many = [(2 + i % 3, 16 * (1 + i % 5) + i % 7) for i in range(70)]
+    shared.check(_wide(shared.make(many, [1, 20, 3], [], 8, 4, 64, bf16, cuda_device, seed=6), 2048))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_shared_prefix_with_sharing_reports_malformed_groups(dtype, cuda_device):
+    s = _wide(shared.make([(4, 100), (4, 100)], [9], [], 16, 8, 128, dtype, cuda_device, seed=9))
+    for cu in ([0, 9, 8], [-3, 4, 8], [0, 4, 100], [5, 2, 8]):
+        shared.call(dict(s, cu=torch.tensor(cu, dtype=torch.int32, device=cuda_device)))
+        assert ops.read_device_error()[0] == 1
+    shared.call(dict(s, prefix=torch.tensor([-1, 100], dtype=torch.int32, device=cuda_device)))
+    assert ops.read_device_error()[0] == 1
+    for bad in (1 << 28, -1, -2):
+        tables = s["tables"].clone()
+        tables[0, 2] = bad  # the group's first row names its shared pages
+        shared.call(dict(s, tables=tables))
+        assert ops.read_device_error()[0] == 7
+        tables = s["tables"].clone()
+        tables[1, 2] = bad  # another row's entry for a shared page is not read
+        shared.call(dict(s, tables=tables))
+        assert ops.read_device_error()[0] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_shared_prefix_with_sharing_replays_in_a_graph_and_beside_it(dtype, cuda_device):
+    s = _wide(shared.make([(12, 900), (3, 64)], [9, 100, 31], [40], 16, 8, 128, dtype, cuda_device, seed=10))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        shared.call(s)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = shared.call(s)
+    for _ in range(3):
+        s["q"].normal_()
+        torch.cuda.synchronize()
+        want = shared.call(s)
+        g.replay()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            beside = shared.call(s)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(beside, want)
+    del g
 
 
 # ------------------------------------------------------------------ beam selection

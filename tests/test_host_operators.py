@@ -103,10 +103,13 @@ def test_no_work_returns_before_the_workspace_is_looked_at(lib):
 
 def test_small_workspaces_are_refused(lib):
     small = _status(lib, "FVB_ERR_WORKSPACE_TOO_SMALL")
-    need = lib.fvb_paged_attention_shared_prefix_workspace_size(2, 8, 2, 128, 50, 1, 32, 1)
-    assert need > 0
-    assert _call(lib.fvb_paged_attention_shared_prefix_decode, SHARED, dict(ws_bytes=need - 1)) == small
-    assert _call(lib.fvb_paged_attention_shared_prefix_decode, SHARED, dict(ws=None)) == small
+    long = dict(columns=4096, max_kv=65536, max_prefix=60000)
+    for dtype in (0, 1):
+        need = lib.fvb_paged_attention_shared_prefix_workspace_size(2, 8, 2, 128, 65536, 1, 60000, dtype)
+        assert need > 0
+        assert _call(lib.fvb_paged_attention_shared_prefix_decode, SHARED,
+                     dict(long, dtype=dtype, q_ts=256, q_hs=512, ws_bytes=need - 1)) == small
+        assert _call(lib.fvb_paged_attention_shared_prefix_decode, SHARED, dict(long, dtype=dtype, ws=None)) == small
     need = lib.fvb_beam_search_workspace_size(2, 4, 1000, 4, 1)
     assert _call(lib.fvb_beam_search_select, SELECT, dict(ws_bytes=need - 1)) == small
     wide = dict(columns=4096, max_kv=65536, window=65536)  # split over the SMs, so partials are kept
@@ -132,10 +135,8 @@ def test_shared_prefix_workspace_sizes(lib):
     size = lib.fvb_paged_attention_shared_prefix_workspace_size
     assert size(0, 8, 2, 128, 50, 1, 32, 1) == 0
     for dtype in (0, 1, 2):
-        alone = size(32, 32, 8, 128, 5120, 0, 0, dtype)
-        shared = size(32, 32, 8, 128, 5120, 1, 4096, dtype)
-        assert shared >= alone + 32 * 32 * 129 * 4 or dtype == 0  # partials of every (sequence, head) and split
-        assert shared % 4 == 0
+        assert size(32, 32, 8, 128, 5120, 1, 4096, dtype) >= 32 * 32 * 129 * 4  # a partial of every (sequence, head)
+        assert size(100, 8, 2, 64, 64, 3, 48, dtype) == 0  # too small to share anything: one split, no partials
 
 
 SELECT = dict(logits=16, stride=1000, requests=2, beams=4, vocab=1000, dtype=1, scores=16, finished=None, eos=-1, select=4,
