@@ -17,6 +17,10 @@
 //
 // The matching needs only the request's parents: every CTA (row, layer) derives its own row's
 // part of it from two 64-bit masks, and CTAs of rows with nothing to copy end there.
+//
+// Bound by HBM where much is copied: 32 requests x 8 beams, 28 layers, 8 heads x 128 bf16, 173 MB read and written,
+// 32.6 us = 5.3 TB/s (open pages of 1 to 15 tokens: runs of 256 bytes to 3.75 KB a head).  One request's 4 beams, 4
+// layers: 4.1 us, which is a launch and three dependent loads.
 #include "common.cuh"
 #include "kernels.h"
 

@@ -24,6 +24,11 @@
 //             again in fp64 (about one request in a thousand), so the order does not
 //             depend on rounding.
 //
+// Measured: 32 requests x 8 beams x 151936 bf16, 16 chosen (62 MB) 23 us out of L2, 30 us out of HBM.  Of the 23: the
+// loads alone 12.5, the exponentials 3.6 (16 a clock and SM), bound and ranking 4, finish 5 (two overlap with the next
+// part's loads).  1 x 4 x 151936: 8.7 us, two launches' latency.  The first version kept sorted lists in every thread
+// and merged them serially: 110 and 19 us.
+//
 // A finished beam has one continuation, eos at its own score, and its logits are not read.
 // A score that is not a number (a NaN or +inf logit, a row of -inf) counts as -inf.
 #include <algorithm>

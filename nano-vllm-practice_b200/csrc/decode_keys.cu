@@ -29,6 +29,11 @@
 //
 // A unit that one CTA holds whole is written directly (window) or as one partial (own keys
 // behind a prefix); a cut one leaves partials by CTA, which a small dependent kernel merges.
+//
+// Bound by HBM: a tile takes 1.64 us of each of the 148 SMs' time, 5.9 TB/s; the first tile waits about 6 us for launch,
+// scan, page ids and the first bytes.  Measured: 256 sequences x 8 heads x 128, group 2, window 1024 (1.04 GB)
+// 164-173 us = 6.0-6.3 TB/s of the 6.54 a copy reaches (split-KV kernel: 189); 32 x 8 x 128, group 8, window 4096
+// (0.555 GB) 93-97 us = 5.7-5.9 TB/s (on 128-row tiles of query rows, where the softmax bounds it: 185).
 #include <algorithm>
 
 #include "common.cuh"

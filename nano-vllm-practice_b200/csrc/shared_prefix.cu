@@ -16,6 +16,10 @@
 //            the SMs that the prefix kernel does not take, beside which it then runs;
 //   merge    one or four warps per (sequence, query head).
 //
+// Measured: 32 requests behind 4096 tokens, 32/8 heads x 128, own keys U[64, 1024]: 32 us (86 MB: 2.7 TB/s; every
+// sequence reading all its keys 116); 128 sequences in four groups behind 2048 to 12288 tokens 100 us (0.41 GB: 4.1
+// TB/s; 529).  Of the 100: prefixes 36, bound by the softmax of 128-row tiles, rest 58 at HBM's rate, merge 5.
+//
 // fp32 and larger batches, four launches:
 //
 //   plan     one CTA: cuts the sequences' own pages into about target_items ranges of equal
