@@ -3,8 +3,9 @@
 //
 // The sinks' and the window's pages are packed into one line of columns, so KV tiles hold pages of both and none that
 // no row sees; each CTA finds its item by a scan of cu_seqlens, so no plan kernel runs in front.  Measured: a tile
-// pair takes 1.9 us of an SM (16.8 MFLOP: 1.3 PFLOP/s over the device), an item 9 us more for its start and end.  8 chunks of 128 to 2048 tokens, 16/8 heads x 128, window 1024 (104 GFLOP): 181 us =
-// 0.57 PFLOP/s; with a causal kernel's tiles over all keys and a mask: 216.
+// pair takes 1.9 us of an SM (16.8 MFLOP: 1.3 PFLOP/s over the device), an item 9 us more for its start and end.
+// 8 chunks of 128 to 2048 tokens, 16/8 heads x 128, window 1024 (104 GFLOP): 181 us = 0.57 PFLOP/s (216 with whole
+// tiles of sinks and window and a plan kernel in front).
 #include "prefill_tc.cuh"
 
 namespace fvb {
