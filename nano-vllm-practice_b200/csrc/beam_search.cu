@@ -24,7 +24,7 @@
 //             again in fp64 (about one request in a thousand), so the order does not
 //             depend on rounding.
 //
-// Measured: 32 requests x 8 beams x 151936 bf16, 16 chosen (62 MB) 23 us out of L2, 30 us out of HBM.  Of the 23: the
+// Measured: 32 requests x 8 beams x 151936 bf16, 16 chosen (62 MB) 24 us out of L2, 28 us out of HBM.  Of the 24: the
 // loads alone 12.5, the exponentials 3.6 (16 a clock and SM), bound and ranking 4, finish 5 (two overlap with the next
 // part's loads).  1 x 4 x 151936: 8.7 us, two launches' latency.  The first version kept sorted lists in every thread
 // and merged them serially: 110 and 19 us.
@@ -733,13 +733,15 @@ cudaError_t launch_t(const BeamArgs& a, int num_requests, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, beam_finish_kernel<T>, a);
 }
 
-// Vectors of a part, in whole tiles of a warp and even over the parts: enough CTAs for the device, no part below one
-// tile of each of its warps, at most kMaxSegments segments, and no more lists a request than the finish kernel's
-// threads merge where that allows.
+// Vectors of a part, in whole tiles of a warp and even over the parts: as many CTAs as the device holds at once, no part
+// below one tile of each of its warps, at most kMaxSegments segments, and no more lists a request than the finish
+// kernel's threads merge where that allows.  (One part more a row, a second wave of the same CTAs: 150 rows x 50001
+// bf16 15.6 us instead of 12.9, 32 x 151936 12.5 instead of 10.6; 200 x 146216, whose 400 CTAs leave a third of the
+// places empty, 19.3 instead of 20.3.)
 int64_t beam_part_vecs(int num_requests, int num_beams, int64_t vocab, int esize) {
   const int64_t vecs = (vocab * esize + 15) / 16 + 1;  // a row may straddle one vector more
   const int64_t rows = int64_t(num_requests) * num_beams, warp_tile = 32 * kVecs, tile = warp_tile * kWarps;
-  const int64_t wanted = std::min<int64_t>((int64_t(device_sm_count()) * kCtasPerSm + rows - 1) / rows,
+  const int64_t wanted = std::min<int64_t>(std::max<int64_t>(1, int64_t(device_sm_count()) * kCtasPerSm / rows),
                                            kLists * kFinishThreads / num_beams);
   const int64_t most = std::min<int64_t>(((vecs + wanted - 1) / wanted + tile - 1) / tile * tile,
                                          int64_t(kMaxSegments) * kSegment * esize / 16);
