@@ -51,6 +51,7 @@ constexpr int kHalf = kKeys * 128;  // 128 keys x one 128-byte swizzle span
 constexpr int kBHalf = kCols * 128; // 16 rows of Q or P x one span
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrowLog2 = 8.0f;
+constexpr float kLeast = -1e37f;
 
 template <int D>
 struct Cfg {
@@ -505,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
             static_cast<T*>(a.out)[int64_t(done.b) * a.lay.o_ts + int64_t(done.head0 + h) * a.lay.o_hs + key_t] =
                 Elem<T>::from_f(v);
           } else {
-            done.o[(done.at + h) * D + key_t] = v;
+            done.o[(done.at + h) * D + key_t] = L == 0.f ? 0.f : v;  // (every score was -inf)
             if (key_t == 0) done.l[done.at + h] = m_done[h] + __log2f(L);
           }
         }
@@ -558,8 +559,11 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
             for (int h = 0; h < HV; ++h) {
               const float mx = fmaxf(fmaxf(red[h], red[kCols + h]), fmaxf(red[2 * kCols + h], red[3 * kCols + h]));
               f[h] = 1.f;
-              if (mx > m[h] + kGrowLog2) {
-                f[h] = fast_exp2(m[h] - mx);  // 0 at the first tile
+              if (t == walk.t0) {
+                // finite though every score were -inf (infinite keys): P is 0 then, and the next tile's maximum larger
+                m[h] = fmaxf(mx, kLeast);
+              } else if (mx > m[h] + kGrowLog2) {
+                f[h] = fast_exp2(m[h] - mx);
                 m[h] = mx;
               }
               l[h] *= f[h];
@@ -665,7 +669,8 @@ __global__ void __launch_bounds__(kCutThreads) keys_cut_kernel(const KeysArgs a)
   for (int k = c + way; k <= last; k += kWays) {
     const int64_t at = (int64_t(k) * 2 + (k == c ? 1 : 0)) * kCols + h;
     const float ls = __ldcg(a.cut_l + at), o = __ldcg(a.cut_o + at * D + d);
-    const float mn = fmaxf(m, ls), f = fast_exp2(m - mn), w = fast_exp2(ls - mn);
+    const float mn = fmaxf(m, ls), ref = mn == -INFINITY ? 0.f : mn;
+    const float f = fast_exp2(m - ref), w = fast_exp2(ls - ref);
     l = fmaf(l, f, w);
     acc = fmaf(acc, f, w * o);
     m = mn;
@@ -684,7 +689,7 @@ __global__ void __launch_bounds__(kCutThreads) keys_cut_kernel(const KeysArgs a)
   acc = 0.f;
 #pragma unroll
   for (int k = 0; k < kWays; ++k) {
-    const float w = fast_exp2(sh_m[k] - mx);
+    const float w = fast_exp2(sh_m[k] - (mx == -INFINITY ? 0.f : mx));
     l = fmaf(sh_l[k], w, l);
     acc = fmaf(sh_o[k][d], w, acc);
   }

@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_split_kernel(
   // (prefix mode: blockIdx.x = (row chunk, split), y = kv head, z = group of sequences, whose
   // first sequence b names the pages and whose rows are sequence-major: (b, head 0), (b, head 1), ..)
   constexpr bool kPre = MODE == kDecodePrefix;
+  constexpr bool kNoKey = MODE != kDecodePlain;  // a maximum of -inf is met and weighs nothing
   const int2 members = kPre ? group_rows(ex, blockIdx.z, num_seqs) : make_int2(0, 0);
   const int split = kPre ? blockIdx.x % max_splits : blockIdx.x, kvh = kPre ? blockIdx.y : blockIdx.y / chunks,
             chunk = kPre ? blockIdx.x / max_splits : blockIdx.y % chunks;
@@ -365,8 +366,8 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_split_kernel(
       const bool valid_r = kPre ? tok0 + lane < row_kv[r] : valid;
       const float sr = valid_r ? s[r] : -INFINITY;
       const float mn = fmaxf(m[r], warp_max(sr));  // finite: a stage's first page holds a visible key
-      // (prefix mode: a sequence shorter than its group's prefix sees none of the later ones)
-      const float ms = kPre && mn == -INFINITY ? 0.f : mn;
+      // (prefix mode: a sequence shorter than its group's prefix sees none of the later ones; and infinite keys)
+      const float ms = kNoKey && mn == -INFINITY ? 0.f : mn;
       const float corr = fast_exp2(m[r] - ms);
       const float p = fast_exp2(sr - ms);
       m[r] = mn;
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_split_kernel(
     float L = 0.f, O = 0.f;
 #pragma unroll
     for (int w = 0; w < kConsumerWarps; ++w) {
-      const float f = kPre && mx == -INFINITY ? 0.f : fast_exp2(wm[w * NREP + r] - mx);
+      const float f = kNoKey && mx == -INFINITY ? 0.f : fast_exp2(wm[w * NREP + r] - mx);
       L += wl[w * NREP + r] * f;
       O += wacc[(w * NREP + r) * D + d] * f;
     }
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_split_kernel(
       const int64_t idx = kPre ? (int64_t(row_tok(r)) * n_heads + row_head(r)) * ex.slots + split
                                : int64_t(blockIdx.x) * n_heads + head0 + r;
       ws_o[idx * D + d] = O / L;
-      if (d == 0) ws_lse[idx] = L > 0.f ? mx + __log2f(L) : -INFINITY;
+      if (d == 0) ws_lse[idx] = L == 0.f ? -INFINITY : mx + __log2f(L);  // (NaN stays NaN)
       continue;
     }
     const int head = head0 + r;
@@ -474,7 +475,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_split_kernel(
       out[int64_t(tok) * lay.o_ts + int64_t(head) * lay.o_hs + d] = Elem<T>::from_f(O / L);
     } else {
       const int64_t idx = (int64_t(b) * n_heads + head) * max_splits + split;
-      ws_o[idx * D + d] = O / L;
+      ws_o[idx * D + d] = kNoKey && L == 0.f ? 0.f : O / L;
       if (d == 0) ws_lse[idx] = mx + __log2f(L);
     }
   }
@@ -561,6 +562,8 @@ __global__ void __launch_bounds__(kCmbThreads) decode_combine_kernel(const float
     float mn = m;
 #pragma unroll
     for (int u = 0; u < kCmbUnroll; ++u) mn = fmaxf(mn, ls[u]);  // finite: row s0 exists
+    const float top = mn;
+    if (MODE == kDecodeWindow && mn == -INFINITY) mn = 0.f;      // (only scores of -inf so far)
     const float corr = fast_exp2(m - mn);                        // 0 on the first pass
     l *= corr;
     acc.x *= corr;
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(kCmbThreads) decode_combine_kernel(const float
       acc.z = fmaf(w, o[u].z, acc.z);
       acc.w = fmaf(w, o[u].w, acc.w);
     }
-    m = mn;
+    m = top;
   }
   g_acc[g][c] = acc;  // groups without rows leave m = -inf, l = 0, acc = 0
   if (c == 0) {
@@ -588,6 +591,7 @@ __global__ void __launch_bounds__(kCmbThreads) decode_combine_kernel(const float
   float M = g_m[0];  // finite: group 0 holds split 0
 #pragma unroll
   for (int k = 1; k < kGroups; ++k) M = fmaxf(M, g_m[k]);
+  if (MODE == kDecodeWindow && M == -INFINITY) M = 0.f;
   float L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll

@@ -200,7 +200,10 @@ __global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const Merge
     }
     float mn = m;
 #pragma unroll
-    for (int u = 0; u < kInFlight; ++u) mn = fmaxf(mn, ls[u]);
+    for (int u = 0; u < kInFlight; ++u) {
+      mn = fmaxf(mn, ls[u]);
+      if (ls[u] != ls[u]) l = ls[u];  // a NaN among the scores: one in the row
+    }
     if (mn == -INFINITY) continue;  // no key seen so far
     const float corr = fast_exp2(m - mn);
     l *= corr;
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const Merge
       for (int d = 0; d < kDims; ++d) acc[d] = fmaf(wt, sh_acc[k][lane * kDims + d], acc[d]);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;  // an empty context gives zeros
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // an empty context gives zeros
   T* dst = out + int64_t(b) * lay.o_ts + int64_t(head) * lay.o_hs + lane * kDims;
   __align__(16) T v[kDims];
 #pragma unroll

@@ -56,6 +56,56 @@ def test_window_decode_with_empty_sequences_in_a_crowd(cuda_device):
     assert (got[:, ::7] == 0).all()
 
 
+def _special_keys(k_pool, table, keys, value):
+    """A copy of the pool with `value` in all of a sequence's `keys`."""
+    k = k_pool.clone()
+    keys = torch.as_tensor(keys, device=k.device)
+    k[table[keys // 16].long(), :, keys % 16] = value
+    return k
+
+
+@pytest.mark.parametrize("dtype,n_rep,n", [(torch.bfloat16, 2, 700), (torch.bfloat16, 8, 700), (torch.bfloat16, 2, 5),
+                                           (torch.bfloat16, 8, 5), (torch.float32, 2, 5), (torch.float32, 2, 300)])
+def test_window_decode_with_infinite_and_nan_keys(dtype, n_rep, n, cuda_device):
+    """Scores of -inf weigh nothing wherever they stand, also where they fill a tile; a NaN shows in its sequence only."""
+    lens = np.full(n, 400)
+    b = workloads.custom(lens, np.ones(n), 8 * n_rep, 8, 64, dtype, seed=8).materialize(cuda_device)
+    b.q.abs_().clamp_(min=0.01)
+    tables, kv = torch.from_numpy(b.block_tables).to(cuda_device), torch.from_numpy(b.kv_lens).to(cuda_device)
+    run = lambda k: ops.paged_attention_window_gemv(b.q, k, b.v_pool, tables, kv, 400, 390, 3)  # noqa: E731
+    k = b.k_pool
+    for s, keys in [(0, range(0, 130)), (1, range(120, 300)), (2, range(256, 400)), (3, [399])]:
+        k = _special_keys(k, tables[s], list(keys), -math.inf)
+    low = torch.where(k == -math.inf, torch.full_like(k, -1e4), k)  # far below the others' scores: the same weights
+    got, same = run(k), run(low)
+    assert torch.isfinite(got).all()
+    ref64.check_attention(got, ref64.attention(b.q, low, b.v_pool, tables, kv, window=390, sinks=3))
+    ref64.check_attention(same, ref64.attention(b.q, low, b.v_pool, tables, kv, window=390, sinks=3))
+    bad = torch.isnan(run(_special_keys(b.k_pool, tables[4], [200], math.nan)))
+    assert bad[:, 4].all() and not bad[:, :4].any() and not bad[:, 5:].any()
+
+
+@pytest.mark.parametrize("dtype,n_rep", [(torch.float32, 2), (torch.bfloat16, 2), (torch.bfloat16, 8)])
+def test_window_prefill_with_infinite_and_nan_keys(dtype, n_rep, cuda_device):
+    b = workloads.custom([400, 300], [200, 30], 4 * n_rep, 4, 64, dtype, seed=8).materialize(cuda_device)
+    md = b.device_metadata(cuda_device)
+    b.q.abs_().clamp_(min=0.01)
+    tables = md["block_tables"]
+
+    def run(k):
+        return ops.paged_attention_window_gemm(b.q, k, b.v_pool, md["cu_seqlens"], 200, tables, md["kv_lens"],
+                                               md["positions"], 150, 3)
+
+    k = _special_keys(b.k_pool, tables[0], list(range(40, 199)) + [0, 1, 2], -math.inf)
+    low = torch.where(k == -math.inf, torch.full_like(k, -1e4), k)
+    got = run(k)
+    ref64.check_attention(got, ref64.attention(b.q, low, b.v_pool, tables, md["kv_lens"], md["cu_seqlens"],
+                                               md["positions"], 150, 3))
+    bad = torch.isnan(run(_special_keys(b.k_pool, tables[0], [210], math.nan)))
+    sees = (md["positions"][:200] >= 210) & (md["positions"][:200] < 210 + 150)
+    assert bad[:, :200][:, sees].all() and not bad[:, :200][:, ~sees].any() and not bad[:, 200:].any()
+
+
 # ------------------------------------------------------------------ fp32 prefill
 
 
@@ -241,6 +291,24 @@ def test_shared_prefix_with_sharing_reports_malformed_groups(dtype, cuda_device)
         tables[1, 2] = bad  # another row's entry for a shared page is not read
         shared.call(dict(s, tables=tables))
         assert ops.read_device_error()[0] == 0
+
+
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_shared_prefix_with_infinite_and_nan_keys(dtype, wide, cuda_device):
+    s = shared.make([(6, 640)], [300], [200], 16, 8, 64, dtype, cuda_device, seed=11)
+    s = _wide(s) if wide else s
+    s["q"].abs_().clamp_(min=0.01)
+    k = _special_keys(s["kp"], s["tables"][0], list(range(100, 640)), -math.inf)  # shared: whole tiles and splits
+    k = _special_keys(k, s["tables"][1], list(range(640, 800)), -math.inf)
+    k = _special_keys(k, s["tables"][2], list(range(640, 940)), -math.inf)
+    low = torch.where(k == -math.inf, torch.full_like(k, -1e4), k)
+    got = shared.call(dict(s, kp=k))
+    ref64.check_attention(got, ref64.attention(s["q"], low, s["vp"], s["tables"], s["kv"]))
+    bad = torch.isnan(shared.call(dict(s, kp=_special_keys(s["kp"], s["tables"][3], [700], math.nan))))
+    assert bad[:, 3].all() and not bad[:, :3].any() and not bad[:, 4:].any()
+    bad = torch.isnan(shared.call(dict(s, kp=_special_keys(s["kp"], s["tables"][3], [17], math.nan))))
+    assert bad[:, :6].all() and not bad[:, 6:].any()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
