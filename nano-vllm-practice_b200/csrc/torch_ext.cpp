@@ -326,6 +326,22 @@ void check_tables(const at::Tensor& q, const at::Tensor& tables, const at::Tenso
               "one block table row and one kv_len per sequence");
 }
 
+// ops' checks and conversions (Python's take 2 us of a small call's 7): ValueError for tensors that are not on a GPU.
+void require_cuda(const at::Tensor& t, const char* name) {
+  if (!t.is_cuda())
+    throw py::value_error("Argument '" + std::string(name) + "' must be a CUDA tensor. Got device=" + t.device().str());
+}
+
+// q as the kernels can read it in place, or a copy.
+at::Tensor readable_q(const at::Tensor& q) {
+  require_cuda(q, "q");
+  const int64_t es = q.element_size();
+  if (q.dim() == 3 && q.stride(2) == 1 && (q.stride(0) * es) % 16 == 0 && (q.stride(1) * es) % 16 == 0 &&
+      (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) == 0)
+    return q;
+  return q.contiguous();
+}
+
 int checked_int(int64_t x, const char* name) {
   TORCH_CHECK(x >= 0 && x <= 0x7fffffff, name, " must be an int32 that is not negative, got ", x);
   return int(x);
@@ -359,6 +375,11 @@ struct Workspace {
 torch::Tensor PagedAttentionWindowGemvCuda(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool,
                                            torch::Tensor kv_page_tables, torch::Tensor kv_lens, int64_t max_kv_len,
                                            int64_t window, int64_t num_sinks, bool out_token_major) {
+  q = readable_q(q);
+  require_cuda(k_pool, "k_pool");
+  require_cuda(v_pool, "v_pool");
+  require_cuda(kv_page_tables, "kv_page_tables");
+  require_cuda(kv_lens, "kv_lens");
   check_pools(q, k_pool, v_pool);
   check_tables(q, kv_page_tables, kv_lens, q.size(1));
   const int n_heads = int(q.size(0)), num_seqs = int(q.size(1)), head_dim = int(q.size(2));
@@ -384,6 +405,13 @@ torch::Tensor PagedAttentionWindowGemmCuda(torch::Tensor q, torch::Tensor k_pool
                                            torch::Tensor cu_seqlens, int64_t max_q_len, torch::Tensor kv_page_tables,
                                            torch::Tensor kv_lens, torch::Tensor positions, int64_t window,
                                            int64_t num_sinks, bool out_token_major) {
+  q = readable_q(q);
+  require_cuda(k_pool, "k_pool");
+  require_cuda(v_pool, "v_pool");
+  require_cuda(cu_seqlens, "cu_seqlens");
+  require_cuda(kv_page_tables, "kv_page_tables");
+  require_cuda(kv_lens, "kv_lens");
+  require_cuda(positions, "positions");
   check_pools(q, k_pool, v_pool);
   for (const auto* t : {&cu_seqlens, &positions}) {
     TORCH_CHECK(t->scalar_type() == torch::kInt32 && t->is_contiguous() && t->get_device() == q.get_device(),
@@ -419,6 +447,13 @@ torch::Tensor PagedAttentionSharedPrefixGemvCuda(torch::Tensor q, torch::Tensor 
                                                  int64_t max_kv_len, torch::Tensor cu_groups,
                                                  torch::Tensor prefix_lens, int64_t max_prefix_len,
                                                  bool out_token_major) {
+  q = readable_q(q);
+  require_cuda(k_pool, "k_pool");
+  require_cuda(v_pool, "v_pool");
+  require_cuda(kv_page_tables, "kv_page_tables");
+  require_cuda(kv_lens, "kv_lens");
+  require_cuda(cu_groups, "cu_groups");
+  require_cuda(prefix_lens, "prefix_lens");
   check_pools(q, k_pool, v_pool);
   check_tables(q, kv_page_tables, kv_lens, q.size(1));
   for (const auto* t : {&cu_groups, &prefix_lens}) {
@@ -449,8 +484,15 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> BeamSearchSelectCuda(tor
                                                                              torch::Tensor scores, int64_t num_select,
                                                                              c10::optional<torch::Tensor> finished,
                                                                              int64_t eos_token_id) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
-              "logits must be an (N * W, vocab) CUDA tensor with contiguous rows");
+  require_cuda(logits, "logits");
+  require_cuda(scores, "scores");
+  TORCH_CHECK(logits.dim() == 2, "logits must be an (N * W, vocab) tensor");
+  if (logits.stride(1) != 1) logits = logits.contiguous();
+  scores = scores.contiguous();
+  if (finished.has_value()) {
+    require_cuda(*finished, "finished");
+    finished = finished->contiguous();
+  }
   TORCH_CHECK(scores.dim() == 2 && scores.scalar_type() == torch::kFloat32 && scores.is_contiguous() &&
                   scores.get_device() == logits.get_device(),
               "scores must be a contiguous float32 (N, W) tensor on the logits' device");
@@ -483,8 +525,16 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> BeamSearchSelectCuda(tor
 torch::Tensor BeamReorderKVCacheCuda(std::vector<torch::Tensor> k_pools, std::vector<torch::Tensor> v_pools,
                                      torch::Tensor block_tables, torch::Tensor kv_lens, torch::Tensor parents) {
   TORCH_CHECK(!k_pools.empty() && k_pools.size() == v_pools.size(), "one K and one V pool per layer");
+  for (const auto& t : k_pools) require_cuda(t, "k_pools");
+  for (const auto& t : v_pools) require_cuda(t, "v_pools");
+  require_cuda(block_tables, "block_tables");
+  require_cuda(kv_lens, "kv_lens");
+  require_cuda(parents, "parents");
+  block_tables = block_tables.contiguous();
+  kv_lens = kv_lens.contiguous();
+  parents = parents.contiguous();
   const at::Tensor& pool = k_pools[0];
-  TORCH_CHECK(pool.is_cuda() && pool.dim() == 4, "pools must be (num_blocks, n_kv_heads, block_size, d_head) CUDA tensors");
+  TORCH_CHECK(pool.dim() == 4, "pools must be (num_blocks, n_kv_heads, block_size, d_head) tensors");
   std::vector<const void*> k(k_pools.size()), v(v_pools.size());
   for (size_t i = 0; i < k_pools.size(); ++i) {
     for (const at::Tensor* t : {&k_pools[i], &v_pools[i]}) {

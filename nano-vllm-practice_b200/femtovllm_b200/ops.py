@@ -135,12 +135,6 @@ def paged_attention_gemm(
     )
 
 
-def _require_cuda(**tensors) -> None:
-    for n, t in tensors.items():
-        if not t.is_cuda:
-            raise ValueError(f"Argument '{n}' must be a CUDA tensor. Got device={t.device}")
-
-
 def paged_attention_window_gemv(
     q: torch.Tensor,
     k_pool: torch.Tensor,
@@ -159,11 +153,8 @@ def paged_attention_window_gemv(
     table entries may be ``-1`` and their contents anything (NaN included), so an engine may take them
     back.  ``window >= 1``; ``max_kv_len`` still bounds ``kv_lens``, not the window.
     """
-    q = _q_view(q)
-    if not (k_pool.is_cuda and v_pool.is_cuda and kv_page_tables.is_cuda and kv_lens.is_cuda):
-        _require_cuda(k_pool=k_pool, v_pool=v_pool, kv_page_tables=kv_page_tables, kv_lens=kv_lens)
-    return _cuda_backend.PagedAttentionWindowGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens, int(max_kv_len),
-                                                      int(window), int(num_sinks), bool(out_token_major))
+    return _cuda_backend.PagedAttentionWindowGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens, max_kv_len, window,
+                                                      num_sinks, out_token_major)
 
 
 def paged_attention_window_gemm(
@@ -186,14 +177,8 @@ def paged_attention_window_gemm(
     :func:`paged_attention_window_gemv`.  The positions of a sequence's tokens must not descend.  A query
     whose mask leaves nothing gives zeros.
     """
-    q = _q_view(q)
-    if not (k_pool.is_cuda and v_pool.is_cuda and cu_seqlens.is_cuda and kv_page_tables.is_cuda
-            and kv_lens.is_cuda and positions.is_cuda):
-        _require_cuda(k_pool=k_pool, v_pool=v_pool, cu_seqlens=cu_seqlens, kv_page_tables=kv_page_tables,
-                      kv_lens=kv_lens, positions=positions)
-    return _cuda_backend.PagedAttentionWindowGemmCuda(q, k_pool, v_pool, cu_seqlens, int(max_q_len), kv_page_tables,
-                                                      kv_lens, positions, int(window), int(num_sinks),
-                                                      bool(out_token_major))
+    return _cuda_backend.PagedAttentionWindowGemmCuda(q, k_pool, v_pool, cu_seqlens, max_q_len, kv_page_tables, kv_lens,
+                                                      positions, window, num_sinks, out_token_major)
 
 
 def paged_attention_shared_prefix_gemv(
@@ -217,14 +202,8 @@ def paged_attention_shared_prefix_gemv(
     ``paged_attention_gemv`` on the same tables.
     ``max_prefix_len`` bounds ``prefix_lens``; keys past it are read per sequence.
     """
-    q = _q_view(q)
-    if not (k_pool.is_cuda and v_pool.is_cuda and kv_page_tables.is_cuda and kv_lens.is_cuda and cu_groups.is_cuda
-            and prefix_lens.is_cuda):
-        _require_cuda(k_pool=k_pool, v_pool=v_pool, kv_page_tables=kv_page_tables, kv_lens=kv_lens,
-                      cu_groups=cu_groups, prefix_lens=prefix_lens)
-    return _cuda_backend.PagedAttentionSharedPrefixGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens,
-                                                            int(max_kv_len), cu_groups, prefix_lens,
-                                                            int(max_prefix_len), bool(out_token_major))
+    return _cuda_backend.PagedAttentionSharedPrefixGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens, max_kv_len,
+                                                            cu_groups, prefix_lens, max_prefix_len, out_token_major)
 
 
 def store_kvcache(
@@ -401,15 +380,7 @@ def beam_search_select(
     ``eos_token_id`` at its own score only.  W and ``num_select`` up to 64; the first step after a
     prompt gives every beam but one a score of ``-inf``.
     """
-    if not (logits.is_cuda and scores.is_cuda):
-        _require_cuda(logits=logits, scores=scores)
-    if logits.dim() == 2 and logits.stride(-1) != 1:
-        logits = logits.contiguous()
-    if finished is not None:
-        _require_cuda(finished=finished)
-        finished = finished.contiguous()
-    return _cuda_backend.BeamSearchSelectCuda(logits, scores.contiguous(), int(num_select), finished,
-                                              int(eos_token_id))
+    return _cuda_backend.BeamSearchSelectCuda(logits, scores, num_select, finished, eos_token_id)
 
 
 def beam_reorder_kvcache(
@@ -430,14 +401,7 @@ def beam_reorder_kvcache(
     """
     k_pools = [k_pools] if isinstance(k_pools, torch.Tensor) else list(k_pools)
     v_pools = [v_pools] if isinstance(v_pools, torch.Tensor) else list(v_pools)
-    for n, pools in (("k_pools", k_pools), ("v_pools", v_pools)):
-        for t in pools:
-            if not t.is_cuda:
-                raise ValueError(f"Argument '{n}' must be CUDA tensors. Got device={t.device}")
-    if not (block_tables.is_cuda and kv_lens.is_cuda and parents.is_cuda):
-        _require_cuda(block_tables=block_tables, kv_lens=kv_lens, parents=parents)
-    return _cuda_backend.BeamReorderKVCacheCuda(k_pools, v_pools, block_tables.contiguous(), kv_lens.contiguous(),
-                                                parents.contiguous())
+    return _cuda_backend.BeamReorderKVCacheCuda(k_pools, v_pools, block_tables, kv_lens, parents)
 
 
 def read_device_error() -> tuple[int, int]:
