@@ -733,8 +733,8 @@ cudaError_t launch_t(const BeamArgs& a, int num_requests, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, beam_finish_kernel<T>, a);
 }
 
-// Vectors of a part, in whole tiles of a warp and even over the parts: as many CTAs as the device holds at once, no part
-// below one tile of each of its warps, at most kMaxSegments segments, and no more lists a request than the finish
+// Vectors of a part, in whole tiles of a warp and even over the parts: as many CTAs as the device holds at once, no
+// part below one tile of each of its warps, at most kMaxSegments segments, and no more lists a request than the finish
 // kernel's threads merge where that allows.  (One part more a row, a second wave of the same CTAs: 150 rows x 50001
 // bf16 15.6 us instead of 12.9, 32 x 151936 12.5 instead of 10.6; 200 x 146216, whose 400 CTAs leave a third of the
 // places empty, 19.3 instead of 20.3.)

@@ -30,8 +30,8 @@
 // A unit that one CTA holds whole is written directly (window) or as one partial (own keys
 // behind a prefix); a cut one leaves partials by CTA, which a small dependent kernel merges.
 //
-// Bound by HBM: a tile takes 1.64 us of each of the 148 SMs' time, 5.9 TB/s; the first tile waits about 6 us for launch,
-// scan, page ids and the first bytes.  Measured: 256 sequences x 8 heads x 128, group 2, window 1024 (1.04 GB)
+// Bound by HBM: a tile takes 1.64 us of each of the 148 SMs' time, 5.9 TB/s; the first tile waits about 6 us for
+// launch, scan, page ids and the first bytes.  Measured: 256 sequences x 8 heads x 128, group 2, window 1024 (1.04 GB)
 // 164-173 us = 6.0-6.3 TB/s of the 6.54 a copy reaches (split-KV kernel: 189); 32 x 8 x 128, group 8, window 4096
 // (0.555 GB) 93-97 us = 5.7-5.9 TB/s (on 128-row tiles of query rows, where the softmax bounds it: 185).
 #include <algorithm>
@@ -331,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
         }
         const int c = t * kTilePages + lane;
         in = lane < kTilePages && c < span.count;
-        return in ? __ldg(a.block_tables + int64_t(w.b) * a.max_blocks_per_seq + (c < span.head ? c : c + span.gap)) : 0;
+        const int32_t* table = a.block_tables + int64_t(w.b) * a.max_blocks_per_seq;
+        return in ? __ldg(table + (c < span.head ? c : c + span.gap)) : 0;
       };
       bool in = false;
       int id = page_id(walk, walk.t0, in);
@@ -743,8 +744,8 @@ bool window_decode_on_keys(int num_seqs, int n_heads, int n_kv_heads, int max_kv
                            int num_sms) {
   if (dtype == FVB_DTYPE_F32 || num_seqs > kKeysMaxSeqs) return false;  // (the sequence table fills shared memory)
   // A call of this kernel costs 8 us before its first tile and 3 us a unit that has only one tile, and its tiles then
-  // stream at HBM's rate whatever the group is.  The split-KV kernel starts in 4 us, but what a page costs it grows with
-  // the group's heads, and from five on it is bound by its lanes.  Over 320 calls of random shapes the pages an SM
+  // stream at HBM's rate whatever the group is.  The split-KV kernel starts in 4 us, but what a page costs it grows
+  // with the group's heads, and from five on it is bound by its lanes.  Over 320 calls of random shapes the pages an SM
   // gets at most are what tells them apart; with these limits the choice is 2 % off the better kernel on average.
   // (201 sequences x 8 heads, window 5: 29.7 us here, 8.1 there; 256 x 8, group 2, window 1024: 165.5 and 189;
   // 190 x 2, group 16, window 1512: 67.5 and 157.)

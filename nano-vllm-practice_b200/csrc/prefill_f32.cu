@@ -75,8 +75,7 @@ __device__ __forceinline__ void wait_copies_but_one() { asm volatile("cp.async.w
 // The tile of one CTA, R rows a thread: ROWS / 16, or 1 for at most kFewRows rows.
 template <int D, int ROWS, int R>
 __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq, int kvh, int64_t tok0, int row0,
-                                            int n_rows, int kv_len, const KeySpan span, int first_seen, int split,
-                                            int splits) {
+                                            int n_rows, int kv_len, const KeySpan span, int split, int splits) {
   constexpr int kChunks = D / 4;    // 16-byte chunks of a row
   constexpr int kVC = D / 64;       // chunks of V (and O) a thread holds
   using S = Smem<D, ROWS>;
@@ -135,7 +134,7 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
       const int r = ld_r + i * kRowStep;
       const int p = (i * kRowStep) / kPageSize;  // (kRowStep divides a page)
       const int key = page_of(t * kPagesPerTile + p) * kPageSize + r % kPageSize;
-      const bool live = id[p] >= 0 && key < kv_len && (key >= first_seen || key < a.sinks);
+      const bool live = id[p] >= 0 && key < kv_len && (key >= span.lo || key < a.sinks);
       const float* src = pool + (live ? int64_t(id[p]) * page_step + head_off + (r % kPageSize) * D + ld_c * 4 : 0);
       copy16(dst + r * D + ((swizzle ? ld_c ^ (r & 7) : ld_c) << 2), src, live);
     }
@@ -363,9 +362,9 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) window_prefill_f32
   kv_len = max(0, high < kv_len ? high + 1 : kv_len);  // keys that some row sees end here
   const KeySpan span = window_span(low + 1, kv_len, a.window, a.sinks, kPageSize);
   if (n_rows <= kFewRows)
-    attend_tile<D, ROWS, kFewRows * 16 / kThreads>(a, sm, seq, kvh, tok0, row0, n_rows, kv_len, span, span.lo, split, splits);
+    attend_tile<D, ROWS, kFewRows * 16 / kThreads>(a, sm, seq, kvh, tok0, row0, n_rows, kv_len, span, split, splits);
   else
-    attend_tile<D, ROWS, ROWS * 16 / kThreads>(a, sm, seq, kvh, tok0, row0, n_rows, kv_len, span, span.lo, split, splits);
+    attend_tile<D, ROWS, ROWS * 16 / kThreads>(a, sm, seq, kvh, tok0, row0, n_rows, kv_len, span, split, splits);
   if (splits == 1) return;
   // ---- join: CTA r of the cluster takes rows r, r + splits, ... ----
   cluster.sync();
@@ -460,7 +459,8 @@ cudaError_t launch_window_prefill_f32(const void* q, void* out, const void* k_po
   const int64_t kv_cap = std::min<int64_t>(int64_t(max_blocks_per_seq) * kPageSize, 0x7fffffff);
   const int tokens = std::min(max_q_len, (rows + a.group - 2) / a.group + 1);  // of a tile at most
   const int64_t keys = std::min<int64_t>(kv_cap, int64_t(window) + tokens - 1);
-  const int key_tiles = window_max_units(int(kv_cap), int(std::max<int64_t>(1, keys)), sinks, kPageSize) / kPagesPerTile;
+  const int key_pages = window_max_units(int(kv_cap), int(std::max<int64_t>(1, keys)), sinks, kPageSize);
+  const int key_tiles = key_pages / kPagesPerTile;
   int splits = 1;
   while (splits < kMaxSplits && tiles * n_kv_heads * splits * 2 <= places && key_tiles >= splits * 4) splits *= 2;
   if (rows == 64)
