@@ -3,25 +3,26 @@
 // fp32 results have to hold fp32's accuracy, which the tensor cores' inputs do not, so the
 // products run on the FMA pipe (128 a clock and SM: 72 TFLOP/s), tiled for it:
 //
-//   tile   64 consecutive rows of one sequence and kv head (row = token x GQA head, so a key
-//          that is fetched serves the whole group) against 64 keys at a time, 128 threads.
-//   S      each thread 8 rows x 4 keys, 12 16-byte shared loads for 128 FMAs; the rows of a
-//          half-warp are its own, so the row maximum is four shuffles.
-//   P V    the same 8 rows x D/16 dims, P through the warp's own 16 rows of shared memory:
-//          no barrier between softmax and PV, and O, m and l never leave their registers.
+//   tile   64 (small calls 32) consecutive rows of one sequence and kv head (row = token x GQA
+//          head, so a key that is fetched serves the whole group) against 64 keys at a time,
+//          four rows a thread.
+//   S      each thread 4 rows x 4 keys, 8 16-byte shared loads for 64 FMAs (32 paired ones);
+//          the rows of a half-warp are its own, so the row maximum is four shuffles.
+//   P V    the same 4 rows x D/16 dims, P through the warp's own 8 rows of shared memory:
+//          O, m and l never leave their registers.
 //   loads  K of the next tile is copied (cp.async) while this tile's softmax and PV run, V
 //          while its S does; page ids are read a tile ahead.  Two CTAs per SM (three at D 64)
 //          fill the barriers' gaps.
 //   rows   a tile of at most 16 rows (a single token's group, the end of a chunk) takes the
-//          same code with 2 rows a thread.
+//          same code with 1 or 2 rows a thread.
 //   keys   only the pages that the tile's rows can see: the sinks' and the window's; keys of
 //          them that no row sees are stored as zeros and masked.
 //   split  with fewer tiles than the SMs hold, a cluster of 2 to 8 CTAs shares a tile's keys
 //          and joins (m, l, O) through distributed shared memory.
 //
-// Bound by the FMA pipe, which the shared-memory loads and the softmax leave 44 % of: 7 chunks of 761 to 1019 tokens,
-// 32/8 heads x 128, window 1059 (37 GFLOP) 1.21 ms = 31 TFLOP/s (one warp a query row: 38 ms).  128 threads with twice
-// the rows took 1.24 and left small calls at 25 us instead of 12.
+// Bound by the shared-memory loads (74 % of their pipe; paired FMAs take 32 % of theirs): 7 chunks of 761 to 1019
+// tokens, 32/8 heads x 128, window 1059 (37 GFLOP) 1.21 ms = 31 TFLOP/s; one warp a query row, as the causal fp32
+// kernel has it, 38 ms.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -35,7 +36,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
+// Threads of a tile of ROWS rows: four rows each.  (Two rows each in tiles of 32, 256 threads: 42.5 us where these
+// take 34.6, from the shared-memory loads, and 12.3 where these take 14.2 in calls of one tile an SM and one of keys;
+// eight each in tiles of 64, 128 threads: the largest call 5 % faster, the others up to 15 % slower.)
+template <int ROWS>
+constexpr int kThreadsOf = ROWS * 4;
 constexpr int kKeys = 64;   // keys of a tile, four pages
 constexpr int kPagesPerTile = kKeys / kPageSize;
 constexpr int kFewRows = 16;
@@ -78,6 +83,7 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
                                             int n_rows, int kv_len, const KeySpan span, int split, int splits) {
   constexpr int kChunks = D / 4;    // 16-byte chunks of a row
   constexpr int kVC = D / 64;       // chunks of V (and O) a thread holds
+  constexpr int kThreads = kThreadsOf<ROWS>;
   using S = Smem<D, ROWS>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, col = lane & 15;
   const int my_row = warp * 2 * R + half;  // its rows: my_row + 2 i
@@ -281,8 +287,9 @@ __device__ __forceinline__ void attend_tile(const F32Args& a, float* sm, int seq
 }
 
 template <int D, int ROWS>
-__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 3) window_prefill_f32_kernel(const F32Args a) {
+__global__ void __launch_bounds__(kThreadsOf<ROWS>, D == 128 ? 2 : 3) window_prefill_f32_kernel(const F32Args a) {
   extern __shared__ __align__(16) float sm[];
+  constexpr int kThreads = kThreadsOf<ROWS>;
   using S = Smem<D, ROWS>;
   int* meta = reinterpret_cast<int*>(sm + S::kMeta);
   const cg::cluster_group cluster = cg::this_cluster();
@@ -408,7 +415,7 @@ cudaError_t launch_t(const F32Args& a, int64_t tiles, int splits, cudaStream_t s
   if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ctas));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kThreadsOf<ROWS>);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
