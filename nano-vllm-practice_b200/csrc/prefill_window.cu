@@ -18,8 +18,8 @@ cudaError_t dispatch(int nrep, const void* q, void* out, const void* k_pool, con
                      const int32_t* positions, const PrefillPlan& plan, const QOLayout& lay, void* ws, int* err,
                      cudaStream_t stream, const DecodeExtra& ex) {
 #define FVB_TW_ARGS q, out, k_pool, v_pool, num_blocks, n_kv_heads, num_seqs, q_len_flatten, cu_seqlens, block_tables, \
-                    max_blocks_per_seq, kv_lens, kv_cap, positions, plan, lay, nrep, 0, 1, nullptr, nullptr, ws, err, \
-                    stream, ex
+                    max_blocks_per_seq, kv_lens, kv_cap, positions, plan, lay, nrep, \
+                    plan.single_rows_apart ? -1 : 0, 1, nullptr, nullptr, ws, err, stream, ex
   switch (tc_tile_heads(nrep)) {
     case 1:
       return launch_tc<T, D, 1, false, kTcWindow>(FVB_TW_ARGS);
@@ -50,7 +50,8 @@ cudaError_t launch_window_prefill(const void* q, void* out, const void* k_pool, 
   ex.window = window;
   ex.sinks = sinks;
 #define FVB_WP_ARGS nrep, q, out, k_pool, v_pool, num_blocks, n_kv_heads, num_seqs, q_len_flatten, cu_seqlens, \
-                    block_tables, max_blocks_per_seq, kv_lens, kv_cap, positions, plan, lay, workspace, err, stream, ex
+                    block_tables, max_blocks_per_seq, kv_lens, kv_cap, positions, plan, lay, workspace, err, \
+                    stream, ex
   cudaError_t ce;
   if (dtype == FVB_DTYPE_BF16) {
     ce = head_dim == 128 ? dispatch<__nv_bfloat16, 128>(FVB_WP_ARGS)

@@ -172,6 +172,30 @@ def test_window_prefill_leaves_rows_behind_the_last_sequence(dtype, n_rep, cuda_
     assert (out[:, t:] == 7.0).all()
 
 
+@pytest.mark.parametrize("n_rep", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("window", [60, 100])
+def test_window_prefill_single_rows_are_written_once(window, n_rep, cuda_device):
+    """Single-token rows of a mixed batch: bit for bit what they are in a batch of their own, whatever runs beside them."""
+    q_lens = np.array([1, 400, 1, 1, 700, 33, 1, 2, 1, 900])
+    kv = q_lens + np.array([700, 300, 5, 0, 900, 64, 100, 9, 333, 0])
+    b = workloads.custom(kv, q_lens, 4 * n_rep, 4, 128, torch.bfloat16, seed=9).materialize(cuda_device)
+    md = b.device_metadata(cuda_device)
+    ones = np.flatnonzero(q_lens == 1)
+    rows = torch.from_numpy(np.concatenate([[0], np.cumsum(q_lens)])[ones]).to(cuda_device)
+    pick = torch.from_numpy(ones).to(cuda_device)
+    alone = ops.paged_attention_window_gemm(
+        b.q[:, rows].contiguous(), b.k_pool, b.v_pool, torch.arange(len(ones) + 1, dtype=torch.int32, device=cuda_device),
+        1, md["block_tables"][pick].contiguous(), md["kv_lens"][pick].contiguous(),
+        md["positions"][rows].contiguous(), window, 3)
+    want = ref64.attention(b.q, b.k_pool, b.v_pool, md["block_tables"], md["kv_lens"], md["cu_seqlens"],
+                           md["positions"], window, 3)
+    for _ in range(20):
+        got = ops.paged_attention_window_gemm(b.q, b.k_pool, b.v_pool, md["cu_seqlens"], 900, md["block_tables"],
+                                              md["kv_lens"], md["positions"], window, 3)
+        assert torch.equal(got[:, rows], alone)
+    ref64.check_attention(got, want)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_window_prefill_reports_bad_pages_and_long_contexts(dtype, cuda_device):
     b = workloads.custom([100, 50], [20, 50], 4, 2, 64, dtype, seed=6).materialize(cuda_device)
