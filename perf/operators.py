@@ -14,7 +14,6 @@ Lengths, group sizes and parents come from a case's ``lens_seed`` alone, so ``wo
 contents and page numbers come from ``prepare``'s seed.
 """
 
-import functools
 import math
 
 import numpy as np
@@ -378,7 +377,6 @@ def _plain_beam_reorder(s):
 # ----------------------------------------------------------------------------------------------
 
 
-@functools.lru_cache(maxsize=None)
 def _ops():
     import sys
     from pathlib import Path
