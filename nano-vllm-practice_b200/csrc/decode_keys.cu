@@ -215,10 +215,11 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
   // ---- tiles of every sequence, and their running sum ----
   {
     int32_t* warp_sum = reinterpret_cast<int32_t*>(red);
-    // The groups' table in the K ring, which is still empty, where it fits (it may hold empty groups).
+    // The groups' table in the K ring, which is still empty, where it fits (it may hold empty groups).  Without
+    // groups there is no table to read: both pointers may be null.
     int32_t* groups = reinterpret_cast<int32_t*>(smem + C::kOffK);
     const int G = a.ex.num_groups;
-    const bool staged = MODE == kKeysRest && (2 * G + 1) * 4 <= kS * C::kTileBytes;
+    const bool staged = MODE == kKeysRest && G > 0 && (2 * G + 1) * 4 <= kS * C::kTileBytes;
     if (staged) {
       for (int g = threadIdx.x; g <= G; g += kThreads) {
         groups[g] = __ldg(a.ex.cu_groups + g);

@@ -1,0 +1,54 @@
+"""Shared-prefix calls that are large enough to share, where tests/test_gpu_shared_prefix.py's go sequence by sequence.
+
+A call shares its prefixes once sequences x kv heads x pages of max_kv_len (twice that at 128 dims) exceed a limit per SM
+that is 256 at most, so `wide` gives a call a table and a bound beyond it; `make` and the lengths are that file's.
+"""
+
+import ctypes
+
+import pytest
+import torch
+
+import cabi
+import ref64
+from femtovllm_b200 import capi, ops
+import test_gpu_shared_prefix as shared
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def wide(s, limit=256):
+    """The call `s` with a table and a max_kv_len that put it beyond `limit` pages an SM."""
+    hkv, d = s["kp"].shape[1], s["kp"].shape[3]
+    sms = torch.cuda.get_device_properties(s["q"].device).multi_processor_count
+    columns = min(limit * sms // (len(s["tables"]) * hkv * (d // 64)) + 1, capi.load().fvb_max_kv_len() // 16)
+    assert len(s["tables"]) * hkv * columns * (d // 64) > limit * sms
+    columns = max(columns, s["tables"].shape[1])
+    tables = torch.full((len(s["tables"]), columns), -1, dtype=torch.int32, device=s["tables"].device)
+    tables[:, : s["tables"].shape[1]] = s["tables"]
+    return dict(s, tables=tables, max_kv=16 * columns)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_groups_by_null_pointers(dtype, cuda_device):
+    """Zero groups need no arrays: both may be null in the C entry, also where the call could share."""
+    s = wide(shared.make([], [], [100, 1, 33, 700], 16, 8, 128, dtype, cuda_device, seed=1))
+    hq, b, d = s["q"].shape
+    lib, code = cabi.lib(), capi.dtype_code(dtype)
+    need = lib.fvb_paged_attention_shared_prefix_workspace_size(b, hq, 8, d, s["max_kv"], 0, 0, code)
+    ws = torch.empty(max(need, 256), dtype=torch.uint8, device=cuda_device)
+    out = torch.empty_like(s["q"])
+    for max_prefix in (0, 4096):
+        need = lib.fvb_paged_attention_shared_prefix_workspace_size(b, hq, 8, d, s["max_kv"], 0, max_prefix, code)
+        assert need <= ws.numel()
+        out.fill_(7.0)
+        capi.check(lib.fvb_paged_attention_shared_prefix_decode(
+            s["q"].data_ptr(), d, b * d, out.data_ptr(), d, b * d, s["kp"].data_ptr(), s["vp"].data_ptr(),
+            s["kp"].shape[0], hq, 8, d, 16, b, s["tables"].data_ptr(), s["tables"].shape[1], s["kv"].data_ptr(),
+            s["max_kv"], None, 0, None, max_prefix, code, ws.data_ptr(), ws.numel(),
+            ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)), "shared prefix")
+        ref64.check_attention(out, ref64.attention(s["q"], s["kp"], s["vp"], s["tables"], s["kv"]))
+        assert ops.read_device_error() == (0, 0)
+    shared.check(s)  # and by the tensor of one entry that the Python call takes
