@@ -272,6 +272,9 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
       if (b < B) cum[b + 1] = before + upto;
       __syncthreads();
     }
+    // The table's bytes are next written by TMA: ordinary accesses to them come first (a barrier for all threads
+    // follows before any copy is issued).
+    if (staged) fence_proxy_async_smem();
   }
   if constexpr (MODE == kKeysRest) {
     if (blockIdx.x == 0) {

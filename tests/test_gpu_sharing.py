@@ -52,3 +52,13 @@ def test_no_groups_by_null_pointers(dtype, cuda_device):
         ref64.check_attention(out, ref64.attention(s["q"], s["kp"], s["vp"], s["tables"], s["kv"]))
         assert ops.read_device_error() == (0, 0)
     shared.check(s)  # and by the tensor of one entry that the Python call takes
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_groups_again_and_again(dtype, cuda_device):
+    """The table of groups stands where the first tiles of keys go: it must have been read before they arrive."""
+    many = [(2 + i % 3, 16 * (1 + i % 5) + i % 7) for i in range(300)]
+    s = wide(shared.make(many, [1, 20, 3, 140], [], 8, 4, 64, dtype, cuda_device, seed=6))
+    want = shared.check(s)
+    for _ in range(30):
+        assert torch.equal(shared.call(s), want)
