@@ -8,6 +8,13 @@
 //   S^T[128 keys x 16]  = K [128 x D]   Q^T           (A = K tile, K-major;  B = Q, K-major)
 //   O^T[D x 16]        += V^T[D x 128]  P^T[128 x 16] (A = V tile, MN-major; B = P, K-major)
 //
+// The tensor cores take P in 16 bits, so each probability is fed as two of them, p = hi + lo with hi = p rounded and
+// lo = p - hi rounded: off by 2^-16 of itself in bf16, 2^-22 in fp16, where one of them alone (2^-8, 2^-11) adds as
+// much error as the output's own rounding (measured, 256 sequences of window 1024: 0.0023 off against 0.0017, and the
+// same 173 us).  hi and lo are rows of P, so they take columns of O that the group's
+// heads leave unused (8 + h; from nine heads on 16 + h, N = 32), and are added in fp32 when the unit ends.  fp16 has
+// no bits left below 2^-24, which long rows of small weights behind a large one reach: its lo is kept times 2^11.
+//
 // A softmax thread then owns one key: it takes its scores of the group's heads from TMEM,
 // the mask is one predicate, and the exponentials are keys x heads, as they should be.
 // What is left is the stream of K and V, 64 KB per tile of 128 keys at D 128.
@@ -48,12 +55,14 @@ constexpr int kTilePages = kKeys / kPageSize;
 constexpr int kThreads = 256;
 constexpr int kCols = kKeysCols;     // heads of a unit: columns of both products
 constexpr int kHalf = kKeys * 128;  // 128 keys x one 128-byte swizzle span
-constexpr int kBHalf = kCols * 128; // 16 rows of Q or P x one span
+constexpr int kBHalf = kCols * 128; // 16 rows of Q x one span
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrowLog2 = 8.0f;
 constexpr float kLeast = -1e37f;
+template <typename T>
+constexpr float kLoScale = std::is_same<T, __half>::value ? 2048.f : 1.f;
 
-template <int D>
+template <int D, int HV, int MODE>
 struct Cfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kHalves * kHalf;
@@ -61,14 +70,21 @@ struct Cfg {
   static constexpr int kOffK = 0;
   static constexpr int kOffV = kStages * kTileBytes;
   static constexpr int kOffQ = 2 * kStages * kTileBytes;        // two units' q
+  static constexpr int kLoCol = HV <= 8 ? 8 : kCols;            // column of head 0's lo
+  static constexpr int kPCols = 2 * kLoCol;                     // rows of P: hi and lo
+  static constexpr int kPHalf = kPCols * 128;
   static constexpr int kOffP = kOffQ + 2 * kHalves * kBHalf;    // two tiles' P
-  static constexpr int kOffBar = kOffP + 2 * 2 * kBHalf;
+  static constexpr int kOffBar = kOffP + 2 * 2 * kPHalf;
   // k_full, k_empty, v_full, v_empty [kStages]; s_full, p_full, pv_done, q_full, q_empty, o_empty [2]
   static constexpr int kNumBars = 4 * kStages + 12;
   static constexpr int kOffRed = kOffBar + kNumBars * 8 + 16;   // float[4][kCols]
-  // int[num_seqs + 1] tiles before each sequence, int[num_seqs] its length, int[num_seqs] keys skipped (rest)
+  // int[num_seqs + 1] tiles before each sequence; window: int[num_seqs] its length; rest: int[num_seqs] keys skipped,
+  // uint8_t[num_seqs] keys that its last tile lacks
   static constexpr int kOffSeqs = kOffRed + 4 * kCols * 4;
-  static constexpr int smem_bytes(int num_seqs) { return kOffSeqs + (3 * num_seqs + 1) * 4 + 1024; }
+  static constexpr int smem_bytes(int num_seqs) {
+    return kOffSeqs + (2 * num_seqs + 1) * 4 + (MODE == kKeysRest ? num_seqs : 0) + 1024;
+  }
+  static constexpr uint32_t kTmemCols = HV <= 8 ? 64 : 128;  // S twice, O twice
   static_assert(smem_bytes(kKeysMaxSeqs) <= 227 * 1024, "shared memory budget");
 };
 
@@ -82,19 +98,6 @@ __device__ __forceinline__ float warp_max(float x) {
   float r;
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
   return r;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
 }
 
 struct KeysArgs {
@@ -164,7 +167,7 @@ template <typename T, int D, int HV, int MODE>
 __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                   const __grid_constant__ CUtensorMap vmap,
                                                                   const __grid_constant__ KeysArgs a) {
-  using C = Cfg<D>;
+  using C = Cfg<D, HV, MODE>;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kS = C::kStages;
   launch_dependents();
@@ -183,8 +186,14 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
   float* red = reinterpret_cast<float*>(smem + C::kOffRed);
   int32_t* cum = reinterpret_cast<int32_t*>(smem + C::kOffSeqs);
-  int32_t* lens = cum + a.num_seqs + 1;
-  int32_t* skips = lens + a.num_seqs;
+  int32_t* lens = cum + a.num_seqs + 1;  // window
+  int32_t* skips = lens;                 // rest
+  uint8_t* tails = reinterpret_cast<uint8_t*>(skips + a.num_seqs);
+  // Length of sequence b, and the keys of it that are not this kernel's.
+  auto skip_of = [&](int b) { return MODE == kKeysRest ? skips[b] : 0; };
+  auto len_of = [&](int b) {
+    return MODE == kKeysRest ? skips[b] + (cum[b + 1] - cum[b]) * kKeys - tails[b] : lens[b];
+  };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_heads = a.n_kv_heads * a.group;
   const int units = a.n_kv_heads * a.chunks;
@@ -208,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 64);
+    tmem_alloc(tmem_slot, C::kTmemCols);
     tmem_relinquish();
   }
 
@@ -249,12 +258,17 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
             const int2 rows = group_rows(gx, lo, B);
             if (b >= rows.x) skip = group_prefix(gx, lo, rows);
           }
-          skips[b] = skip;
         }
-        const int kv = __ldg(a.kv_lens + b);
+        int kv = __ldg(a.kv_lens + b);
         if (blockIdx.x == 0 && kv > a.kv_cap) record_error(a.err, FVB_ERR_INVALID_ARGUMENT, b);
-        lens[b] = min(max(kv, 0), a.kv_cap);
-        n = (unit_span<MODE>(a, lens[b], skip).count + kTilePages - 1) / kTilePages;
+        kv = min(max(kv, 0), a.kv_cap);
+        n = (unit_span<MODE>(a, kv, skip).count + kTilePages - 1) / kTilePages;
+        if constexpr (MODE == kKeysRest) {
+          skips[b] = skip;
+          tails[b] = uint8_t(n > 0 ? skip + n * kKeys - kv : 0);
+        } else {
+          lens[b] = kv;
+        }
       }
       int upto = n;
 #pragma unroll
@@ -301,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   auto col_s = [&](int j) { return tmem + uint32_t(j & 1) * kCols; };
-  auto col_o = [&](int i) { return tmem + 32u + uint32_t(i & 1) * kCols; };
+  auto col_o = [&](int i) { return tmem + 32u + uint32_t(i & 1) * C::kPCols; };
 
   if (MODE == kKeysWindow && threadIdx.x == 96) {  // a lane that waits for nothing yet
     int4 cut = make_int4(-1, 0, 0, 0);
@@ -331,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
       auto page_id = [&](const Walk& w, int t, bool& in) {
         if (w.b != span_of) {
           span_of = w.b;
-          span = unit_span<MODE>(a, lens[w.b], MODE == kKeysRest ? skips[w.b] : 0);
+          span = unit_span<MODE>(a, len_of(w.b), skip_of(w.b));
         }
         const int c = t * kTilePages + lane;
         in = lane < kTilePages && c < span.count;
@@ -383,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
       // ============================ MMA issuer ============================
       if (lane == 0) {
         constexpr uint32_t idesc_s = umma_idesc_f16(kBF16, 128, kCols, false);
-        constexpr uint32_t idesc_o = umma_idesc_f16(kBF16, 128, kCols, false, true);
+        constexpr uint32_t idesc_o = umma_idesc_f16(kBF16, 128, C::kPCols, false, true);
         const uint64_t dk = umma_sdesc_sw128(smem_u32(smem + C::kOffK), 16, 1024);
         // At D 64 both halves of the 128 rows read the same 64 dims; rows 64 .. 127 of O are not used.
         const uint64_t dv = umma_sdesc_sw128(smem_u32(smem + C::kOffV), D == 128 ? kHalf : 0, 1024);
@@ -398,11 +412,11 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
           if (!ok) return;
           tc_fence_after();
           const uint64_t vd = dv + uint64_t((st * C::kTileBytes) >> 4);
-          const uint64_t pd = dp + uint64_t(((j & 1) * 2 * kBHalf) >> 4);
+          const uint64_t pd = dp + uint64_t(((j & 1) * 2 * C::kPHalf) >> 4);
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk)
             umma_f16_ss(col_o(item), vd + uint64_t((kk * 16 * 128) >> 4),
-                        pd + uint64_t(((kk >> 2) * kBHalf + (kk & 3) * 32) >> 4), idesc_o, first && kk == 0 ? 0u : 1u);
+                        pd + uint64_t(((kk >> 2) * C::kPHalf + (kk & 3) * 32) >> 4), idesc_o, first && kk == 0 ? 0u : 1u);
           umma_commit(&v_empty[st]);
           umma_commit(&pv_done[j & 1]);
         };
@@ -457,8 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
       const int key_t = threadIdx.x - 128;
       const uint32_t t_row = uint32_t((warp & 3) * 32) << 16;
       const float scale = kLog2e * rsqrtf(float(D));
-      // this key's place in a row of P: [half][head / 8][head % 8] rows of 128 bytes, 16-byte chunks swizzled
-      const uint32_t p_base = smem_u32(smem + C::kOffP) + (key_t >> 6) * kBHalf + (key_t & 7) * 2;
+      // this key's place in a row of P: [half][column / 8][column % 8] rows of 128 bytes, 16-byte chunks swizzled
+      const uint32_t p_base = smem_u32(smem + C::kOffP) + (key_t >> 6) * C::kPHalf + (key_t & 7) * 2;
       const int p_chunk = (key_t & 63) >> 3;
       // A wait that gives up (ok = false) ends no loop here: the four warps share barriers, so a warp that has
       // failed goes on without waiting or touching TMEM, and the others fail or finish in their own time.
@@ -473,6 +487,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
       } done{};
       done.item = -1;
       float m[HV], l[HV], m_done[HV], l_done[HV];
+      auto load_o = [&](int item, uint32_t(&o)[C::kPCols]) {
+        if constexpr (C::kPCols == 16) tmem_ld_16cols(col_o(item) + t_row, o);
+        else tmem_ld_32cols(col_o(item) + t_row, o);
+      };
       auto finish = [&]() {
         // Sums over the 128 keys: lanes trade halves of the heads until each holds one, then warps meet in `red`.
         float s[HV];
@@ -494,10 +512,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
         if (lane % (32 / HV) == 0) red[(warp & 3) * kCols + mine] = s[0];
         named_barrier(1, kKeys);
         ok = ok && warp_wait(&pv_done[done.tile & 1], (done.tile >> 1) & 1, a.err, 0x434);
-        uint32_t o[16] = {};
+        uint32_t o[C::kPCols] = {};
         if (ok) {
           tc_fence_after();
-          tmem_ld_16cols(col_o(done.item) + t_row, o);
+          load_o(done.item, o);
           tc_fence_before();
         }
         mbar_arrive(&o_empty[done.item & 1]);
@@ -505,7 +523,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
 #pragma unroll
         for (int h = 0; h < HV; ++h) {
           const float L = (red[h] + red[kCols + h]) + (red[2 * kCols + h] + red[3 * kCols + h]);
-          const float v = __uint_as_float(o[h]) / L;
+          // (an infinite V: lo = 0 of it is NaN, hi alone tells)
+          const float hi = __uint_as_float(o[h]);
+          const float sum = fmaf(__uint_as_float(o[C::kLoCol + h]), 1.f / kLoScale<T>, hi);
+          const float v = (fabsf(hi) < INFINITY ? sum : hi) / L;
           if (h >= done.nvh || key_t >= D) continue;
           if (MODE == kKeysWindow && done.at < 0) {
             static_cast<T*>(a.out)[int64_t(done.b) * a.lay.o_ts + int64_t(done.head0 + h) * a.lay.o_hs + key_t] =
@@ -522,8 +543,8 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
         const int b = walk.b;
         const int kvh = walk.u / a.chunks, chunk = walk.u % a.chunks;
         const int head0 = kvh * a.group + chunk * kCols, nvh = min(kCols, a.group - chunk * kCols);
-        const int kv_len = lens[b];
-        const KeySpan span = unit_span<MODE>(a, kv_len, MODE == kKeysRest ? skips[b] : 0);
+        const int kv_len = len_of(b);
+        const KeySpan span = unit_span<MODE>(a, kv_len, skip_of(b));
 #pragma unroll
         for (int h = 0; h < HV; ++h) {
           m[h] = -INFINITY;
@@ -576,25 +597,32 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
             if (t > walk.t0) ok = ok && warp_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, a.err, 0x431);
             if (t > walk.t0 && ok) {
               tc_fence_after();
-              uint32_t o[16];
-              tmem_ld_16cols(col_o(item) + t_row, o);
+              uint32_t o[C::kPCols];
+              load_o(item, o);
 #pragma unroll
-              for (int h = 0; h < HV; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) * f[h]);
-              tmem_st_16cols(col_o(item) + t_row, o);
+              for (int h = 0; h < HV; ++h) {
+                o[h] = __float_as_uint(__uint_as_float(o[h]) * f[h]);
+                o[C::kLoCol + h] = __float_as_uint(__uint_as_float(o[C::kLoCol + h]) * f[h]);
+              }
+              if constexpr (C::kPCols == 16) tmem_st_16cols(col_o(item) + t_row, o);
+              else tmem_st_32cols(col_o(item) + t_row, o);
               tmem_wait_st();
             }
             named_barrier(1, kKeys);  // red is read before its next use
           }
           // P of tile j - 2 has been read
           if (j >= 2) ok = ok && warp_wait(&pv_done[j & 1], ((j >> 1) - 1) & 1, a.err, 0x432);
-          const uint32_t p_row = p_base + (j & 1) * 2 * kBHalf;
+          const uint32_t p_row = p_base + (j & 1) * 2 * C::kPHalf;
 #pragma unroll
           for (int h = 0; h < HV; ++h) {
             const float p = fast_exp2(x[h] - m[h]);
             l[h] += p;
-            const uint32_t packed = pack2<T>(p, 0.f);
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(p_row + h * 128 + ((p_chunk ^ (h & 7)) << 4)),
-                         "h"(uint16_t(packed))
+            const T hi = Elem<T>::from_f(p);
+            const T lo = Elem<T>::from_f((p - Elem<T>::to_f(hi)) * kLoScale<T>);
+            const uint32_t at = p_row + h * 128 + ((p_chunk ^ (h & 7)) << 4);
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(*reinterpret_cast<const uint16_t*>(&hi)) : "memory");
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + C::kLoCol * 128),
+                         "h"(*reinterpret_cast<const uint16_t*>(&lo))
                          : "memory");
           }
           if (ragged) {
@@ -644,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_keys_kernel(const __grid_c
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 64);
+    tmem_dealloc(tmem, C::kTmemCols);
   }
   if (blockIdx.x == gridDim.x - 1) {
     // As a programmatic dependent of the prefix kernel (which writes nothing read here) this grid may run
@@ -705,7 +733,7 @@ __global__ void __launch_bounds__(kCutThreads) keys_cut_kernel(const KeysArgs a)
 template <typename T, int D, int HV, int MODE>
 cudaError_t launch_t(const KeysArgs& a, const void* k_pool, const void* v_pool, int grid, bool dependent,
                      cudaStream_t stream) {
-  using C = Cfg<D>;
+  using C = Cfg<D, HV, MODE>;
   const CUtensorMapDataType tdt =
       std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap kmap, vmap;
