@@ -61,7 +61,14 @@ constexpr int kWgThreads = 128;
 constexpr int kHalfBytes = 128 * 128;  // 128 rows x one 128-byte swizzle span
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.0f;   // lazy-rescale threshold (P <= 2^8)
-
+// Window and prefix launches in fp16, whose numbers end at 2^-24: every P is raised by 2^11 and the reference maximum
+// moves at 2^4, so P stays below 2^15 and a weight keeps its 11 bits down to 2^-25 of the row's largest.  (As the plain
+// form has it they are lost from 2^-14 on, and 2^-25 vanishes from P V while l counts it; a first key that holds nearly
+// all of a row's weight leaves the others there.)
+template <typename T>
+constexpr float kRaiseLog2 = std::is_same<T, __half>::value ? 11.0f : 0.0f;
+template <typename T>
+constexpr float kRaisedRescaleLog2 = std::is_same<T, __half>::value ? 4.0f : kRescaleLog2;
 template <int D>
 struct Cfg {
   static constexpr int kHalves = D / 64;  // 128-byte spans per row of Q / K / V
@@ -137,6 +144,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
   using C = Cfg<D>;
   constexpr int TOK = kTileM / NREP;  // query tokens per tile
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr float kRaise = MODE == kTcPlain ? 0.f : kRaiseLog2<T>;
+  constexpr float kGrow = MODE == kTcPlain ? kRescaleLog2 : kRaisedRescaleLog2<T>;
   // decode mode: the split combine may start once every CTA is resident (prefix mode: the kernel of the
   // sequences' own keys)
   launch_dependents();
@@ -646,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
         // row may see none at all)
         m_ref = mt;
       } else {
-        const bool grow = (mt - m_ref) * scale > kRescaleLog2;
+        const bool grow = (mt - m_ref) * scale > kGrow;
         rescale = __any_sync(0xffffffffu, grow);
         if (grow) {
           corr = fast_exp2((m_ref - mt) * scale);
@@ -654,10 +663,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
           m_ref = mt;
         }
       }
-      // P = 2^((s - m_ref) * scale) <= 2^8, packed to 16 bits into S_i's first 64 columns
+      // P = 2^((s - m_ref) * scale) <= 2^8 (raised in fp16, see kRaiseLog2), packed to 16 bits into S_i's first 64 columns
       // (P = 0 while the row has seen no key).
       const float ms = ((kIlv || MODE != kTcPlain) && m_ref == -INFINITY) ? 0.f : m_ref * scale;
-      const float2 nms2 = make_float2(-ms, -ms);
+      const float up = MODE == kTcPlain ? -ms : kRaise - ms;
+      const float2 nms2 = make_float2(up, up);
       float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       uint32_t pk[64];
 #pragma unroll
@@ -719,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
     // M = max(m_0, m_1), L = sum l_g 2^(m_g - M), out = sum O_g 2^(m_g - M) / L.
     // The groups swap (max, sum) through shared memory and each finishes half of the
     // columns from both O's.
-    const float m_log2 = m_ref * scale;  // -inf for a row that saw no key
+    const float m_log2 = MODE == kTcPlain ? m_ref * scale : m_ref * scale - kRaise;  // -inf for a row that saw no key
     float f_own, f_oth = 0.f, lse;
     int cc_begin = 0, cc_end = D / 32;
     if (ilv) {

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import ref64
-from femtovllm_b200 import ops
+from femtovllm_b200 import ops, workloads
 import test_gpu_shared_prefix as shared
 from test_gpu_sharing import wide
 
@@ -117,3 +117,21 @@ GROUPS = [(20, 16), (3, 20)], [30, 77, 150], [60, 1]
 def test_own_keys_of_sequences_in_groups(dtype, d, n_rep, cuda_device):
     """A bound of 0 on the prefixes leaves every key to its own sequence."""
     _share(shared.make(*GROUPS, 4 * n_rep, 4, d, dtype, cuda_device, seed=n_rep), max_prefix=0)
+
+
+@pytest.mark.parametrize("log2", [13.3, 20.3, 24.3])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_small_weights_behind_a_sink_in_a_prefill_and_a_prefix(dtype, log2, cuda_device):
+    """The same rows on the kernels of 128-row tiles.  A weight of 2^-24.3 still has all of a 16-bit operand's bits."""
+    for n_rep in (2, 8):
+        b = workloads.custom([6000, 900], [200, 33], 4 * n_rep, 4, 64, dtype, seed=2).materialize(cuda_device)
+        md = b.device_metadata(cuda_device)
+        k, v, tables = b.k_pool, b.v_pool, md["block_tables"]
+        _one_key_above(k, v, b.q, tables[0, 0].item(), log2)
+        got = ops.paged_attention_window_gemm(b.q, k, v, md["cu_seqlens"], 200, tables, md["kv_lens"], md["positions"],
+                                              1 << 30, 1)
+        ref64.check_attention(got, ref64.attention(b.q, k, v, tables, md["kv_lens"], md["cu_seqlens"], md["positions"],
+                                                   1 << 30, 1))
+        s = wide(shared.make([(3, 8000)], [5, 300, 20], [], 4 * n_rep, 4, 64, dtype, cuda_device, seed=2))
+        _one_key_above(s["kp"], s["vp"], s["q"], s["tables"][0, 0].item(), log2)
+        ref64.check_attention(shared.call(s), ref64.attention(s["q"], s["kp"], s["vp"], s["tables"], s["kv"]))
