@@ -135,3 +135,13 @@ def test_small_weights_behind_a_sink_in_a_prefill_and_a_prefix(dtype, log2, cuda
         s = wide(shared.make([(3, 8000)], [5, 300, 20], [], 4 * n_rep, 4, 64, dtype, cuda_device, seed=2))
         _one_key_above(s["kp"], s["vp"], s["q"], s["tables"][0, 0].item(), log2)
         ref64.check_attention(shared.call(s), ref64.attention(s["q"], s["kp"], s["vp"], s["tables"], s["kv"]))
+
+
+@pytest.mark.parametrize("n_rep", [1, 2, 4, 5, 8, 12, 16, 20])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_shared_prefixes(dtype, d, n_rep, cuda_device):
+    """Groups of one query tile and of several, prefixes of a page, of part of a tile and of several splits."""
+    for i, shape in enumerate([GROUPS, ([(5, 120), (9, 700), (2, 64)], [1, 20], [33]), ([(3, 2000)], [4], []),
+                               ([(150, 100)], [2], [])]):
+        _share(shared.make(*shape, 4 * n_rep, 4, d, dtype, cuda_device, seed=n_rep + i))
