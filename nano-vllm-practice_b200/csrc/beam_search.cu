@@ -522,13 +522,12 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
   };
   if (again) exact_bases(false);
 
-  // Close scores of two beams, one of them from logits.  (Beams that are each other's copies tie exactly, in
-  // any precision.)
+  // Close scores of two beams, one of them from logits; equal ones too, since rows that differ in their smallest
+  // logits only have one and the same sum in fp32.
   auto near_tie = [&](uint64_t s, int w, uint64_t s2, int w2) {
     const Beam &b = beams[w], &b2 = beams[w2];
     return w != w2 && s2 != ordered64(-INFINITY) && unordered64(s) - unordered64(s2) < kNearTie &&
-           (b.kind == kLive || b2.kind == kLive) &&
-           !(s == s2 && b.kind == b2.kind && b.base == b2.base && b.best == b2.best);
+           (b.kind == kLive || b2.kind == kLive);
   };
   // Entry i of beam w's list of part p, whose key is `key`.  A live beam has a list per part; a beam without
   // logits has one, its first: eos and then every other token (done), or every token (dead), at -inf.

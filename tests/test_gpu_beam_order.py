@@ -1,0 +1,52 @@
+"""Beam selection's order where fp32 sums cannot tell: it is that of the scores in 64 bits (tests/ref64.py).
+
+Tokens and parents must be equal; the oracle's own sums are off by less than 1e-13, and the true scores compared here
+lie further apart than that, or are equal in every bit because their rows are.
+"""
+
+import math
+
+import pytest
+import torch
+
+import ref64
+from femtovllm_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def check(logits, scores, k, finished=None, eos=-1):
+    tokens, parents, got = ops.beam_search_select(logits, scores, k, finished, eos)
+    want = ref64.beam_select(logits, scores, k, finished, eos)
+    assert torch.equal(tokens, want[0]) and torch.equal(parents, want[1])
+    return got, want[2]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_differ_in_one_small_logit(dtype, cuda_device):
+    """The beam with less weight in its tail scores more everywhere, by 1e-12 to 1e-9: it comes first, token by token."""
+    gen = torch.Generator(device=cuda_device).manual_seed(1)
+    for low in (-14.0, -12.0, -10.0, -8.0):
+        for heavy in (0, 1):
+            row = (torch.randn(50001, generator=gen, device=cuda_device) * 2).clamp(min=-7.0).to(dtype)
+            logits = row.repeat(2, 1)
+            logits[:, 40000] = low - 1
+            logits[heavy, 40000] = low
+            lse = torch.logsumexp(logits.double(), 1)
+            assert 1e-12 < (lse[heavy] - lse[1 - heavy]).item() < 1e-7
+            for k in (1, 2, 7, 40):
+                check(logits, torch.zeros(1, 2, device=cuda_device), k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_are_copies(dtype, cuda_device):
+    """Equal in every bit: the lower beam comes first.  (The oracle's sums of copies differ in their last bits, so the
+    order here is that of the logits themselves, which copies share.)"""
+    gen = torch.Generator(device=cuda_device).manual_seed(2)
+    row = (torch.randn(3, 1, 30011, generator=gen, device=cuda_device) * 2).to(dtype)
+    logits = row.expand(3, 5, 30011).reshape(15, -1).contiguous()
+    tokens, parents, _ = ops.beam_search_select(logits, torch.zeros(3, 5, device=cuda_device), 20)
+    at = torch.sort(logits.view(3, -1).double(), dim=1, descending=True, stable=True).indices[:, :20]
+    assert torch.equal(tokens, at % 30011) and torch.equal(parents, at // 30011)
