@@ -422,6 +422,8 @@ struct Beam {
   double base;  // score of its best continuation: score + best - lse, exact whatever the logits' size
   float best;   // its largest logit
   int kind;
+  bool exact;   // base is from fp64 or the caller's score itself
+  bool redo;    // base has to be computed again in fp64
 };
 __device__ __forceinline__ bool finite(double x) { return x >= -DBL_MAX && x <= DBL_MAX; }
 
@@ -438,7 +440,9 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
   __shared__ uint32_t best_of[kFinishThreads / 4];
   __shared__ uint64_t cand_score[kRanked], cand_id[kRanked];
   __shared__ uint32_t bound;
-  __shared__ uint16_t sorted[65];
+  __shared__ uint16_t sorted[kRanked];
+  __shared__ double last_score;
+  __shared__ int last_beam;
   __shared__ uint64_t top_score[kFinishWarps];
   __shared__ uint32_t top_beam[kFinishWarps], top_token[kFinishWarps];
   __shared__ int again, n_cand;
@@ -451,7 +455,8 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
   for (int w = threadIdx.x; w < W; w += kFinishThreads) {
     const double score = a.scores[row0 + w];
     const bool done = a.finished != nullptr && a.finished[row0 + w] != 0;
-    beams[w] = Beam{score, 0.f, !finite(score) ? kDead : done ? kDone : kLive};
+    const int kind = !finite(score) ? kDead : done ? kDone : kLive;
+    beams[w] = Beam{score, 0.f, kind, kind != kLive, false};
   }
   __syncthreads();
   const unsigned long long* lists = reinterpret_cast<const unsigned long long*>(a.keys) + row0 * per_row;
@@ -493,16 +498,21 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
       beams[w].best = best;
       // +inf or only -inf: no distribution.  Otherwise a NaN, or logits so large that x log2e left the
       // range of fp32: fp64 tells.
-      if (best == INFINITY || best == -INFINITY) beams[w].kind = kDead;
-      else if (!finite(beams[w].base)) again = 1;
+      if (best == INFINITY || best == -INFINITY) {
+        beams[w].kind = kDead;
+        beams[w].exact = true;
+      } else if (!finite(beams[w].base)) {
+        beams[w].redo = true;
+        again = 1;
+      }
     }
   }
   __syncthreads();
 
-  // base of the live beams (all, or those without one) in fp64
-  auto exact_bases = [&](bool all) {
+  // base of the beams that ask for it in fp64, and a new start
+  auto exact_bases = [&]() {
     for (int w = 0; w < W; ++w) {
-      if (beams[w].kind != kLive || (!all && finite(beams[w].base))) continue;
+      if (!beams[w].redo) continue;
       const T* p = static_cast<const T*>(a.logits) + (row0 + w) * a.row_stride;
       const double top = double(beams[w].best);
       double s = 0.0;
@@ -516,18 +526,25 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
         for (int k = 0; k < kFinishWarps; ++k) t += red[k];
         beams[w].base = double(a.scores[row0 + w]) - log(t);
         if (!finite(beams[w].base)) beams[w].kind = kDead;
+        beams[w].exact = true;
+        beams[w].redo = false;
       }
       __syncthreads();
     }
+    if (threadIdx.x == 0) again = n_cand = 0;
+    __syncthreads();
   };
-  if (again) exact_bases(false);
+  if (again) exact_bases();
 
-  // Close scores of two beams, one of them from logits; equal ones too, since rows that differ in their smallest
-  // logits only have one and the same sum in fp32.
-  auto near_tie = [&](uint64_t s, int w, uint64_t s2, int w2) {
-    const Beam &b = beams[w], &b2 = beams[w2];
-    return w != w2 && s2 != ordered64(-INFINITY) && unordered64(s) - unordered64(s2) < kNearTie &&
-           (b.kind == kLive || b2.kind == kLive);
+  // Scores of two beams that lie too close for their fp32 sums: both beams' in fp64.  (Equal ones too: rows that differ
+  // in their smallest logits only have one and the same sum in fp32.)  Called for every selected candidate and the next
+  // one, and for the last selected one and every candidate that is not: where any two, one of them selected, are in
+  // doubt, neighbours between them are, or the last one and the second of them.
+  auto compare = [&](double s, int w, double s2, int w2) {
+    if (w == w2 || (beams[w].exact && beams[w2].exact) || !(fabs(s - s2) < kNearTie)) return;
+    beams[w].redo = !beams[w].exact;
+    beams[w2].redo = !beams[w2].exact;
+    again = 1;
   };
   // Entry i of beam w's list of part p, whose key is `key`.  A live beam has a list per part; a beam without
   // logits has one, its first: eos and then every other token (done), or every token (dead), at -inf.
@@ -545,78 +562,73 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
     }
     return h;
   };
-  bool exact = false;  // every live beam's base is from fp64
-  // ---- most requests: the candidates that reach a bound which at least K + 1 do, ranked against each other.
-  // The bound is the (K + 1)-th largest of 64 or 128 groups' best scores, rounded to fp32. ----
-  {
+  auto nth = [&](int i, uint64_t key) {
+    const int w = i / per_row, p = (i - w * per_row) / K;
+    return candidate(w, p, i - w * per_row - p * K, key);
+  };
+  // ---- most requests: the candidates that reach a bound which at least K + 1 do, and those that may be as good as
+  // they are, ranked against each other.  The bound is the (K + 1)-th largest of 64 or 128 groups' best scores, rounded
+  // to fp32.  False where that cannot be done. ----
+  auto select_ranked = [&]() {
     const int shift = K < 32 ? 3 : 2, groups = kFinishThreads >> shift;
     auto rounded = [](uint64_t score) { return score == 0 ? 0u : ordered(float(unordered64(score))); };
-    auto beam_of = [&](int i) { return i / per_row; };
-    auto nth = [&](int i, uint64_t key) {
-      const int w = beam_of(i), p = (i - w * per_row) / K;
-      return candidate(w, p, i - w * per_row - p * K, key);
-    };
     const Head mine = my_key < n_keys ? nth(my_key, first_key) : Head{0, 0};
     uint32_t run = rounded(mine.score);
 #pragma unroll 1
     for (int i = my_key + kFinishThreads; i < n_keys; i += kFinishThreads)
       run = max(run, rounded(nth(i, __ldcg(lists + i)).score));
-    const uint32_t first_run = rounded(mine.score);
     for (int o = 1; o < 1 << shift; o <<= 1) run = max(run, __shfl_xor_sync(0xffffffffu, run, o));
     if ((lane & ((1 << shift) - 1)) == 0) best_of[threadIdx.x >> shift] = run;
     __syncthreads();
     kth_largest<kFinishWarps>(best_of, groups, K, &bound);
     __syncthreads();
-    const uint32_t least = bound;
-    if (least > ordered(-INFINITY)) {
-      auto keep = [&](int i, const Head& h) {
-        const int at = atomicAdd(&n_cand, 1);
-        if (at >= kRanked) return;
-        cand_score[at] = h.score;
-        cand_id[at] = uint64_t(beam_of(i)) << 32 | h.token;
-      };
-      if (first_run != 0 && first_run >= least) keep(my_key, mine);
+    if (bound <= ordered(-INFINITY)) return false;
+    // Every score that rounds to the bound lies above the number before it; the K-th best is one of these or better.
+    const uint64_t least = ordered64(double(unordered(bound - 1)) - kNearTie);
+    auto keep = [&](int i, const Head& h) {
+      if (h.score < least) return;
+      const int at = atomicAdd(&n_cand, 1);
+      if (at >= kRanked) return;
+      cand_score[at] = h.score;
+      cand_id[at] = uint64_t(i / per_row) << 32 | h.token;
+    };
+    keep(my_key, mine);
 #pragma unroll 1
-      for (int i = my_key + kFinishThreads; i < n_keys; i += kFinishThreads) {
-        const Head h = nth(i, __ldcg(lists + i));
-        if (h.score != 0 && rounded(h.score) >= least) keep(i, h);
-      }
-      __syncthreads();
-      const int c = n_cand;
-      if (c <= kRanked) {
-        if (threadIdx.x < c) {  // kRanked <= kFinishThreads
-          const uint64_t score = cand_score[threadIdx.x], id = cand_id[threadIdx.x];
-          int before = 0, equal = 0;
+    for (int i = my_key + kFinishThreads; i < n_keys; i += kFinishThreads) keep(i, nth(i, __ldcg(lists + i)));
+    __syncthreads();
+    const int c = n_cand;
+    if (c > kRanked) return false;
+    if (threadIdx.x < c) {  // kRanked <= kFinishThreads
+      const uint64_t score = cand_score[threadIdx.x], id = cand_id[threadIdx.x];
+      int before = 0, equal = 0;
 #pragma unroll 8
-          for (int j = 0; j < c; ++j) {
-            before += cand_score[j] > score;
-            equal += cand_score[j] == score;
-          }
-          if (equal > 1) {
-            for (int j = 0; j < c; ++j) before += cand_score[j] == score && cand_id[j] < id;
-          }
-          if (before <= K) sorted[before] = threadIdx.x;
-        }
-        __syncthreads();
-        for (int k = threadIdx.x; k < K; k += kFinishThreads) {
-          const uint64_t score = cand_score[sorted[k]], id = cand_id[sorted[k]];
-          const uint64_t score2 = cand_score[sorted[k + 1]], id2 = cand_id[sorted[k + 1]];
-          const int64_t o = int64_t(blockIdx.x) * K + k;
-          a.tokens[o] = uint32_t(id);
-          a.parents[o] = id >> 32;
-          a.out_scores[o] = float(unordered64(score));
-          if (near_tie(score, int(id >> 32), score2, int(id2 >> 32))) again = 1;
-        }
-        __syncthreads();
-        if (again == 0) return;
-        exact_bases(true);
-        exact = true;
+      for (int j = 0; j < c; ++j) {
+        before += cand_score[j] > score;
+        equal += cand_score[j] == score;
       }
+      if (equal > 1) {
+        for (int j = 0; j < c; ++j) before += cand_score[j] == score && cand_id[j] < id;
+      }
+      sorted[before] = threadIdx.x;
     }
-  }
+    __syncthreads();
+    for (int k = threadIdx.x; k < c; k += kFinishThreads) {
+      const uint64_t id = cand_id[sorted[k]];
+      const double score = unordered64(cand_score[sorted[k]]);
+      if (k < K) {
+        const int64_t o = int64_t(blockIdx.x) * K + k;
+        a.tokens[o] = uint32_t(id);
+        a.parents[o] = id >> 32;
+        a.out_scores[o] = float(score);
+      }
+      const int other = sorted[k < K ? min(k + 1, K - 1) : K - 1];
+      compare(score, int(id >> 32), unordered64(cand_score[other]), int(cand_id[other] >> 32));
+    }
+    return true;
+  };
 
-  // ---- else (fewer than K + 1 finite candidates, a crowd of equal ones, or scores computed again above), one
-  // by one: a merge of the W * parts sorted lists, up to kLists a thread ----
+  // ---- else (fewer than K + 1 finite candidates, or a crowd of equal ones), one by one: a merge of the W * parts
+  // sorted lists, up to kLists a thread ----
   auto entry = [&](int l, int i) {
     const int w = l / a.parts;
     return i < K ? candidate(w, l - w * a.parts, i, __ldcg(lists + int64_t(l) * K + i)) : Head{0, 0};
@@ -647,9 +659,7 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
 
   const int L = W * a.parts;
   const int warps = L <= 32 * kLists ? 1 : kFinishWarps;
-  for (int pass = exact ? 1 : 0; pass < 2; ++pass) {
-    __syncthreads();
-    bool near = false;
+  auto select_merged = [&]() {
     if (warp < warps) {
       Head head[kLists], next[kLists];  // each list's first candidate that is left, and the one behind it
       int at[kLists];
@@ -663,9 +673,7 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
           next[j] = entry(l, 1);
         }
       }
-      uint64_t prev = 0;
-      uint32_t prev_w = 0;
-      for (int n = 0; n <= K; ++n) {
+      for (int n = 0; n < K; ++n) {
         const uint32_t w0 = threadIdx.x / a.parts, w1 = (threadIdx.x + 32 * warps) / a.parts;
         const int mine = better(head[1].score, w1, head[1].token, head[0].score, w0, head[0].token) ? 1 : 0;
         uint64_t s = mine ? head[1].score : head[0].score;
@@ -687,12 +695,12 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
           warp_best(s, w, t);
           __syncthreads();
         }
-        if (s == 0) break;  // fewer than K + 1 candidates
         const double best = unordered64(s);
-        if (n > 0 && near_tie(prev, prev_w, s, w)) near = true;
-        prev = s;
-        prev_w = w;
-        if (n == K) break;
+        if (threadIdx.x == 0) {
+          if (n > 0) compare(last_score, last_beam, best, int(w));
+          last_score = best;
+          last_beam = int(w);
+        }
         if (own == s && own_w == w && own_t == t) {  // one list alone holds a beam's token
           const int64_t o = int64_t(blockIdx.x) * K + n;
           a.tokens[o] = t;
@@ -707,10 +715,20 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
         }
       }
     }
-    if (threadIdx.x == 0) again = near && pass == 0;
+    __syncthreads();
+    // the last one and all others (the selected among them are its neighbours' business, and no harm)
+    for (int i = threadIdx.x; i < n_keys; i += kFinishThreads) {
+      if (i / per_row == last_beam) continue;
+      const Head h = nth(i, __ldcg(lists + i));
+      if (h.score != 0) compare(unordered64(h.score), i / per_row, last_score, last_beam);
+    }
+  };
+
+  for (int pass = 0; pass <= W; ++pass) {  // (a second one hardly ever, and one more beam is exact after each)
+    if (!select_ranked()) select_merged();
     __syncthreads();
     if (again == 0) return;
-    exact_bases(true);
+    exact_bases();
   }
 }
 

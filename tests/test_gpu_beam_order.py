@@ -50,3 +50,29 @@ def test_rows_that_are_copies(dtype, cuda_device):
     tokens, parents, _ = ops.beam_search_select(logits, torch.zeros(3, 5, device=cuda_device), 20)
     at = torch.sort(logits.view(3, -1).double(), dim=1, descending=True, stable=True).indices[:, :20]
     assert torch.equal(tokens, at % 30011) and torch.equal(parents, at // 30011)
+
+
+@pytest.mark.parametrize("k", [4, 32, 64])
+@pytest.mark.parametrize("extra", [1, 3, 200])
+def test_rivals_behind_equal_logits_at_the_cut(extra, k, cuda_device):
+    """One beam has more equal largest logits than are selected; the other's, next in line, score 1e-10 to 1e-8 more.
+
+    Its row holds the same logits in another order, so that both sums are one and the same but for fp32's roundings, and
+    one of them is a little smaller.  With 200 equal logits a beam the candidates are too many to be ranked at once.
+    """
+    gen = torch.Generator(device=cuda_device).manual_seed(k + extra)
+    v, n = 60000, 24
+    logits = torch.randn(n, 1, v, generator=gen, device=cuda_device).repeat(1, 2, 1)
+    for i in range(n):
+        logits[i, 0, torch.randperm(v, generator=gen, device=cuda_device)[: k + extra]] = 5.0
+        logits[i, 1] = logits[i, 0][torch.randperm(v, generator=gen, device=cuda_device)]
+        small = int((logits[i, 1] - 2.0).abs().argmin())  # holds about 7e-5 of the weight
+        logits[i, 1, small] -= 10.0 ** (-6 + i % 8 / 4)
+    logits = logits.view(2 * n, v)
+    lse = torch.logsumexp(logits.double(), 1).view(n, 2)
+    assert (lse[:, 0] - lse[:, 1] > 1e-11).all() and (lse[:, 0] - lse[:, 1] < 1e-5).all()
+    scores = torch.zeros(n, 2, device=cuda_device)
+    check(logits, scores, k)
+    order = torch.arange(2 * n, device=cuda_device).view(n, 2).flip(1).reshape(-1)
+    check(logits[order].contiguous(), scores, k)
+
