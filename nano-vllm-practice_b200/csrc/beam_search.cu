@@ -434,7 +434,7 @@ struct Head {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamArgs a) {
+__global__ void __launch_bounds__(kFinishThreads, 1) beam_finish_kernel(const BeamArgs a) {
   __shared__ Beam beams[64];
   __shared__ double red[kFinishWarps];
   __shared__ uint32_t best_of[kFinishThreads / 4];
@@ -516,7 +516,22 @@ __global__ void __launch_bounds__(kFinishThreads) beam_finish_kernel(const BeamA
       const T* p = static_cast<const T*>(a.logits) + (row0 + w) * a.row_stride;
       const double top = double(beams[w].best);
       double s = 0.0;
-      for (int64_t i = threadIdx.x; i < a.vocab; i += kFinishThreads) s += exp(double(Elem<T>::to_f(p[i])) - top);
+      constexpr int kAhead = 8;  // loads in flight: 40 us a beam of 151936 logits, by fp64's rate (one at a time: 84)
+#pragma unroll 1
+      for (int64_t i0 = threadIdx.x; i0 < a.vocab; i0 += kAhead * kFinishThreads) {
+        float x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int64_t i = i0 + u * kFinishThreads;
+          x[u] = i < a.vocab ? Elem<T>::to_f(p[i]) : -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u += 4) {
+          const double e0 = exp(double(x[u]) - top), e1 = exp(double(x[u + 1]) - top);
+          const double e2 = exp(double(x[u + 2]) - top), e3 = exp(double(x[u + 3]) - top);
+          s += (e0 + e1) + (e2 + e3);
+        }
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (lane == 0) red[warp] = s;
