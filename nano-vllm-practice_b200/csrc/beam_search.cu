@@ -12,22 +12,28 @@
 // different beams depends on lse.  Two launches:
 //
 //   partials  CTA (part of a row): its warps stream the part once, fold sum 2^(x log2e - m)
-//             with a lazily moved m, and keep one number per segment of 32 logits, the
+//             with a lazily moved integer m, and keep one number per segment of 32 logits, the
 //             largest.  Of 64 or 128 groups of segments the num_select-th largest maximum is a
 //             bound that at least num_select logits reach, and hardly any more do: only the
 //             segments that reach it are read again, from L2, and their few logits at or above
 //             it are ranked against each other.
 //   finish    CTA per request (programmatic dependent): lse of each beam, then a merge of the
-//             beams' and parts' sorted lists by their scores in fp64, again by a bound.  The sums carry an error of
-//             about 1e-7 from ex2.approx and fp32; where two chosen candidates of different
-//             beams are closer than kNearTie, the lse of the request's beams is computed
-//             again in fp64 (about one request in a thousand), so the order does not
-//             depend on rounding.
+//             beams' and parts' sorted lists by their scores in fp64, again by a bound.
 //
-// Measured: 32 requests x 8 beams x 151936 bf16, 16 chosen (62 MB) 24 us out of L2, 28 us out of HBM.  Of the 24: the
+// A sum of exponentials is off by a share that does not depend on the logits: a tile's 16 or 32 of a lane are added as a
+// tree (five roundings, 5 * 2^-24), tiles in two floats by Knuth's TwoSum and lanes, warps and parts in fp64, all exact
+// beside that since sums relative to different m differ by powers of two.  Add ex2.approx (2^-22), the rounding of
+// x log2e - m (2^-24 of itself, at most 10.8 on a warp's average: 4.5e-7) and log2e's own (1.3e-8 times what the logits
+// lie below the largest on average, at most 22 nats), and an lse is off by less than 1.3e-6, a difference of two by less
+// than 2.6e-6.  Scores of different beams closer than kNearTie are therefore in doubt, where one of them is chosen, and
+// the lse of those beams is computed again in fp64 (2 of 4800 requests of 8 beams x 151936, 16 chosen), so the order does not
+// depend on rounding.  (Added up one by one, 128 equal terms alone can be off by 1.9e-6.)
+//
+// Measured: 32 requests x 8 beams x 151936 bf16, 16 chosen (62 MB) 25 us out of L2, 28.7 us out of HBM.  Of the 25: the
 // loads alone 12.5, the exponentials 3.6 (16 a clock and SM), bound and ranking 4, finish 5 (two overlap with the next
-// part's loads).  1 x 4 x 151936: 8.7 us, two launches' latency.  The first version kept sorted lists in every thread
-// and merged them serially: 110 and 19 us.
+// part's loads).  1 x 4 x 151936: 9 us, two launches' latency.  A beam in doubt takes 40 us more in its request's CTA:
+// 32 x 8 with one such pair 120 us, 1 x 4 90 us; requests whose beams are all copies of one another, 8 of them, 420 us.
+// The first version kept sorted lists in every thread and merged them serially: 110 and 19 us.
 //
 // A finished beam has one continuation, eos at its own score, and its logits are not read.
 // A score that is not a number (a NaN or +inf logit, a row of -inf) counts as -inf.
@@ -44,7 +50,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr double kNearTie = 2e-6;
+constexpr double kNearTie = 3e-6;
 
 struct BeamArgs {
   const void* logits;
@@ -55,7 +61,7 @@ struct BeamArgs {
   int num_beams, num_select, parts;
   int64_t part_vecs;  // 16-byte vectors per part
   uint64_t* keys;     // [row][part][num_select], best first; 0 = none
-  float2* sums;       // [row][part] (m, s): sum of 2^(x log2e) = s 2^m
+  double2* sums;      // [row][part] (m, s): sum of 2^(x log2e) = s 2^m
   int64_t *tokens, *parents;
   float* out_scores;
 };
@@ -91,6 +97,17 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^x of an integer x <= 0, exact; 0 below the normal numbers, and of a NaN.
+__device__ __forceinline__ float pow2(float x) { return __int_as_float((int(fmaxf(x, -127.f)) + 127) << 23); }
+__device__ __forceinline__ double pow2(double x) { return __hiloint2double((int(fmax(x, -1023.0)) + 1023) << 20, 0); }
+
+// hi + lo += x, where only lo's own sum is rounded.
+__device__ __forceinline__ void add_exactly(float& hi, float& lo, float x) {
+  const float sum = __fadd_rn(hi, x), back = __fsub_rn(sum, hi);
+  lo = __fadd_rn(lo, __fadd_rn(__fsub_rn(hi, __fsub_rn(sum, back)), __fsub_rn(x, back)));
+  hi = sum;
 }
 
 // Rows may start at any element: vectors are counted from the 16-byte boundary at or before
@@ -193,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) beam_partials_kernel(const BeamArgs 
   constexpr int kSegVecs = kSegment / VE;  // 4 (16-bit) or 8 (fp32) lanes share a segment
   constexpr int kTile = 32 * kVecs;        // vectors of a warp's tile
   extern __shared__ uint32_t sh[];         // segment maxima as ordered(); then the chosen segments' logits
-  __shared__ float2 sh_sums[kWarps];
+  __shared__ double2 sh_sums[kWarps];
   __shared__ uint32_t sh_runs[kThreads / 2];  // largest segment maximum of each group of two or four lanes
   __shared__ uint64_t cand[kListLogits];
   __shared__ uint16_t list[kListSegs];
@@ -212,7 +229,7 @@ __global__ void __launch_bounds__(kThreads) beam_partials_kernel(const BeamArgs 
   if (threadIdx.x == 0) n_list = n_cand = bound = 0;
   float m = -INFINITY;
   uint32_t run = 0;  // of segments of this thread alone; 0: none
-  float2 s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  float hi = 0.f, lo = 0.f;  // this lane's sum, relative to 2^m
   // Vectors [w0, w1) of the part lie wholly inside the row.
   const int w0 = part_begin == 0 && r.shift != 0 ? 1 : 0;
   const int w1 = int(min((a.vocab + r.shift) / VE - part_begin, int64_t(n_vecs)));
@@ -266,30 +283,37 @@ __global__ void __launch_bounds__(kThreads) beam_partials_kernel(const BeamArgs 
     }
     // ---- sum of exponentials; the warp's m moves only when a tile passes it by more than 2^8 ----
     if (__any_sync(0xffffffffu, g * kLog2e > m + 8.f)) {
-      const float tile_max = unordered(__reduce_max_sync(0xffffffffu, ordered(g))) * kLog2e;
-      const float f = ex2(m - tile_max);  // 0 while m is -inf
-#pragma unroll
-      for (int i = 0; i < 2; ++i) s[i] = __fmul2_rn(s[i], make_float2(f, f));
-      m = tile_max;
+      const float top = ceilf(unordered(__reduce_max_sync(0xffffffffu, ordered(g))) * kLog2e);
+      const float f = pow2(m - top);  // 0 while m is -inf
+      hi *= f;
+      lo *= f;
+      m = top;
     }
     // m is -inf while every logit was: nothing to add, except that a NaN has to show in the sum
     const float ms = m == -INFINITY ? 0.f : -m;
+    float2 v[kVecs];
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
       float f[VE];
       unpack16<T>(x[u], f);
+      float2 e[VE / 2];
 #pragma unroll
-      for (int e = 0; e < VE; e += 2) {
-        const float2 t = __ffma2_rn(make_float2(f[e], f[e + 1]), make_float2(kLog2e, kLog2e), make_float2(ms, ms));
-        s[(e >> 1) & 1] = __fadd2_rn(s[(e >> 1) & 1], make_float2(ex2(t.x), ex2(t.y)));
+      for (int i = 0; i < VE / 2; ++i) {
+        const float2 t =
+            __ffma2_rn(make_float2(f[2 * i], f[2 * i + 1]), make_float2(kLog2e, kLog2e), make_float2(ms, ms));
+        e[i] = make_float2(ex2(t.x), ex2(t.y));
       }
+      v[u] = __fadd2_rn(e[0], e[1]);
+      if constexpr (VE == 8) v[u] = __fadd2_rn(v[u], __fadd2_rn(e[2], e[3]));
     }
+    const float2 tile = __fadd2_rn(__fadd2_rn(v[0], v[1]), __fadd2_rn(v[2], v[3]));
+    add_exactly(hi, lo, __fadd_rn(tile.x, tile.y));
   }
   // ---- the part's sum ----
-  float sum = (s[0].x + s[0].y) + (s[1].x + s[1].y);
+  double sum = double(hi) + double(lo);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);  // m is the warp's
-  if (lane == 0) sh_sums[warp] = make_float2(m, sum);
+  if (lane == 0) sh_sums[warp] = make_double2(double(m), sum);
   const int64_t out = row * a.parts + part;
   const int K = a.num_select;
   // Groups of four lanes give 64 maxima (fp32: 32, every other lane's segments are its neighbour's), pairs twice as
@@ -299,13 +323,13 @@ __global__ void __launch_bounds__(kThreads) beam_partials_kernel(const BeamArgs 
   if (shift == 2) run = max(run, __shfl_xor_sync(0xffffffffu, run, 2));
   if ((lane & ((1 << shift) - 1)) == 0) sh_runs[threadIdx.x >> shift] = run;
   __syncthreads();
-  if (warp == kWarps - 1) {  // (a warp that ranks no group)
-    const float2 v = lane < kWarps ? sh_sums[lane] : make_float2(-INFINITY, 0.f);
-    const float mm = warp_max(v.x);
-    float ss = v.x == -INFINITY ? v.y : v.y * ex2(v.x - mm);
+  if (warp == kWarps - 1) {
+    const double2 v = lane < kWarps ? sh_sums[lane] : make_double2(-INFINITY, 0.0);
+    const double mm = double(warp_max(float(v.x)));
+    double ss = v.x == -INFINITY ? v.y : v.y * pow2(v.x - mm);
 #pragma unroll
     for (int o = kWarps / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (lane == 0) a.sums[out] = make_float2(mm, ss);
+    if (lane == 0) a.sums[out] = make_double2(mm, ss);
   }
   // ---- bound: the K-th largest group (0, every logit, where fewer than K groups have one).  A part of few segments
   // leaves most groups without one, and its segments are groups themselves (the last 107 vectors of a row of 50001
@@ -471,29 +495,29 @@ __global__ void __launch_bounds__(kFinishThreads, 1) beam_finish_kernel(const Be
   // ---- each beam's lse ----
   for (int w = warp; w < W; w += kFinishWarps) {
     if (beams[w].kind != kLive) continue;
-    const float2* sums = a.sums + (row0 + w) * a.parts;
+    const double2* sums = a.sums + (row0 + w) * a.parts;
     const unsigned long long* heads = lists + int64_t(w) * per_row;
     uint64_t first = 0;  // of the parts' best keys, the best
     float m = -INFINITY;
-    float2 v = make_float2(-INFINITY, 0.f);
+    double2 v = make_double2(-INFINITY, 0.0);
     for (int p = lane; p < a.parts; p += 32) {
       v = __ldcg(sums + p);
-      m = fmaxf(m, v.x);
+      m = fmaxf(m, float(v.x));
       first = max(first, uint64_t(__ldcg(heads + int64_t(p) * K)));
     }
     m = warp_max(m);
     const float best = unordered(__reduce_max_sync(0xffffffffu, uint32_t(first >> 32)));
-    float s = 0.f;
+    double s = 0.0;
     for (int p = lane; p < a.parts; p += 32) {
       if (a.parts > 32) v = __ldcg(sums + p);
-      s += v.x == -INFINITY ? v.y : v.y * ex2(v.x - m);
+      s += v.x == -INFINITY ? v.y : v.y * pow2(v.x - double(m));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) {
       // s 2^m = sum 2^(x c), c = kLog2e in fp32; taken relative to the largest logit, so that c's own
       // rounding acts on differences of logits only.
-      const double above = 0.69314718055994530942 * (log2(double(s)) + (double(m) - double(best) * double(kLog2e)));
+      const double above = 0.69314718055994530942 * (log2(s) + (double(m) - double(best) * double(kLog2e)));
       beams[w].base -= above;  // lse - best
       beams[w].best = best;
       // +inf or only -inf: no distribution.  Otherwise a NaN, or logits so large that x log2e left the
@@ -794,7 +818,7 @@ bool beam_supported(int num_requests, int num_beams, int64_t vocab, int esize) {
 
 size_t beam_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select, int esize) {
   const size_t parts = size_t(num_requests) * num_beams * beam_parts(num_requests, num_beams, vocab, esize);
-  return ((parts * num_select * 8 + 255) & ~size_t(255)) + parts * 8;
+  return ((parts * num_select * 8 + 255) & ~size_t(255)) + parts * 16;
 }
 
 cudaError_t launch_beam_select(const void* logits, int64_t row_stride, int num_requests, int num_beams, int64_t vocab,
@@ -816,7 +840,7 @@ cudaError_t launch_beam_select(const void* logits, int64_t row_stride, int num_r
   a.part_vecs = beam_part_vecs(num_requests, num_beams, vocab, es);
   a.keys = static_cast<uint64_t*>(workspace);
   const size_t key_bytes = (size_t(rows) * a.parts * num_select * 8 + 255) & ~size_t(255);
-  a.sums = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + key_bytes);
+  a.sums = reinterpret_cast<double2*>(static_cast<uint8_t*>(workspace) + key_bytes);
   a.tokens = tokens;
   a.parents = parents;
   a.out_scores = out_scores;

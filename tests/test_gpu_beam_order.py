@@ -76,3 +76,39 @@ def test_rivals_behind_equal_logits_at_the_cut(extra, k, cuda_device):
     order = torch.arange(2 * n, device=cuda_device).view(n, 2).flip(1).reshape(-1)
     check(logits[order].contiguous(), scores, k)
 
+
+
+def _plateau(n, v, low, dtype, dev):
+    """Rows of one low value with a zero among every 1024: each warp's sum is relative to zero from its start."""
+    x = torch.full((n, v), low, dtype=dtype, device=dev)
+    x[:, 5::1024] = 0.0
+    return x
+
+
+@pytest.mark.parametrize("low", [(-3.40625, -2.15625), (-2.15625, -3.40625), (-1.3125, -4.6875), (-7.25, -9.5)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_equal_logits(dtype, low, cuda_device):
+    """Thousands of equal terms take the same rounding each time they are added: the sums of two such rows err most.
+
+    150 requests of two beams whose best scores are -2e-6 to 2e-6 apart, in rows of one part, where the sums are longest.
+    """
+    n, v = 150, 131000
+    logits = torch.stack([_plateau(n, v, low[0], dtype, cuda_device), _plateau(n, v, low[1], dtype, cuda_device)], 1)
+    logits = logits.view(2 * n, v)
+    lse = torch.logsumexp(logits[:2].double(), 1)
+    scores = torch.zeros(n, 2, dtype=torch.float64, device=cuda_device)
+    scores[:, 1] = lse[1] - lse[0] + torch.linspace(-2e-6, 2e-6, n, dtype=torch.float64, device=cuda_device)
+    check(logits, scores.float(), 8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scores_by_the_sums_error(dtype, cuda_device):
+    """Every selected score within 1.3e-6, the derived error of a sum, and its own rounding."""
+    gen = torch.Generator(device=cuda_device).manual_seed(3)
+    cases = [_plateau(4, 200000, low, dtype, cuda_device) for low in (-3.40625, -2.15625, -16.0, -12.0, -0.5)]
+    cases += [(torch.randn(4, v, generator=gen, device=cuda_device) * s).to(dtype)
+              for v, s in ((151936, 2.5), (151936, 0.0), (50001, 12.0), (1000, 5.0), (400000, 1.0))]
+    cases.append(torch.linspace(-30, 30, 4 * 100000, device=cuda_device).view(4, -1).to(dtype))
+    for logits in cases:
+        got, want = check(logits, torch.zeros(4, 1, device=cuda_device), 8)
+        assert ((got.double() - want).abs() <= 1.3e-6 + want.abs() * 2.0**-24).all()
