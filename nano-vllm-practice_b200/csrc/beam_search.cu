@@ -26,8 +26,8 @@
 // x log2e - m (2^-24 of itself, at most 10.8 on a warp's average: 4.5e-7) and log2e's own (1.3e-8 times what the logits
 // lie below the largest on average, at most 22 nats), and an lse is off by less than 1.3e-6, a difference of two by less
 // than 2.6e-6.  Scores of different beams closer than kNearTie are therefore in doubt, where one of them is chosen, and
-// the lse of those beams is computed again in fp64 (2 of 4800 requests of 8 beams x 151936, 16 chosen), so the order does not
-// depend on rounding.  (Added up one by one, 128 equal terms alone can be off by 1.9e-6.)
+// the lse of those beams is computed again in fp64 (2 of 4800 requests of 8 beams x 151936, 16 chosen), so the order does
+// not depend on rounding.  (Added up one by one, 128 equal terms alone can be off by 1.9e-6.)
 //
 // Measured: 32 requests x 8 beams x 151936 bf16, 16 chosen (62 MB) 25 us out of L2, 28.7 us out of HBM.  Of the 25: the
 // loads alone 12.5, the exponentials 3.6 (16 a clock and SM), bound and ranking 4, finish 5 (two overlap with the next

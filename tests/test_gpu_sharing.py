@@ -62,3 +62,41 @@ def test_many_groups_again_and_again(dtype, cuda_device):
     want = shared.check(s)
     for _ in range(30):
         assert torch.equal(shared.call(s), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_group_s_first_row_names_the_shared_pages(dtype, cuda_device):
+    """Shows that these calls share: another row's entries for the shared pages are not read, its first row's are."""
+    for hq, d in ((2, 64), (8, 128)):
+        s = wide(shared.make([(2, 5000), (3, 90)], [700, 1], [], hq, 2, d, dtype, cuda_device, seed=4))
+        want = shared.check(s)
+        tables = s["tables"].clone()
+        tables[1, : 5000 // 16] = -1
+        tables[3:5, : 90 // 16] = 1 << 28
+        assert torch.equal(shared.call(dict(s, tables=tables)), want) and ops.read_device_error() == (0, 0)
+        tables[0, 7] = -1
+        shared.call(dict(s, tables=tables))
+        assert ops.read_device_error()[0] == 7
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pool_past_32_bit_offsets(dtype, cuda_device):
+    num_blocks, hkv, d = 135000, 8, 128  # 2.2e9 elements a pool
+    kp = torch.empty(num_blocks, hkv, 16, d, dtype=dtype, device=cuda_device)
+    vp = torch.empty_like(kp)
+    pages = torch.arange(num_blocks - 60, num_blocks, device=cuda_device)
+    for pool in (kp, vp):
+        pool[pages] = torch.randn(60, hkv, 16, d, device=cuda_device).to(dtype)
+    tables = torch.stack([pages[:30], torch.cat([pages[:25], pages[40:45]])]).int().contiguous()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    s = wide(dict(q=torch.randn(32, 2, d, device=cuda_device).to(dtype), kp=kp, vp=vp, tables=tables, kv=i32(480, 461),
+                  max_kv=480, cu=i32(0, 2), prefix=i32(400), max_prefix=400))
+    shared.check(s)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_sequences_than_a_table_holds(dtype, cuda_device):
+    """1024 sequences and one more: the limit of the kernel that takes 16-bit calls."""
+    for n in (1024, 1025):
+        s = shared.make([(n - 30, 40)], [1, 20, 3], [9] * 30, 4, 2, 64, dtype, cuda_device, seed=5)
+        shared.check(wide(s))
