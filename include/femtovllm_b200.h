@@ -290,6 +290,8 @@ FVB_API int fvb_paged_attention_prefill(const void* q, void* out, const void* k_
  * -1 (pages the engine has taken back); keys of such pages, and keys between sinks and window in the pages
  * that are read, may hold anything, NaN included.  Prefill: the positions of a sequence's tokens must not
  * descend.  max_kv_len at most fvb_max_kv_len(), at most 65535 sequences.
+ * Softmax weights: decode holds them to 2^-16 (bf16), 2^-22 (fp16) or in fp32; prefill rounds them to q's type
+ * before they meet V, as fvb_paged_attention_prefill does.
  * Workspace: decode fvb_paged_attention_window_decode_workspace_size bytes, prefill
  * fvb_paged_attention_prefill_workspace_size bytes; 256-byte aligned.
  */
@@ -313,15 +315,17 @@ FVB_API int fvb_paged_attention_window_prefill(const void* q, int64_t q_token_st
                                                void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * Decode paged attention for a batch whose sequences share prefixes by groups: the result of
- * fvb_paged_attention_decode_strided on the same tables, with each group's prefix read once for all its
- * sequences (tensor cores for 16-bit types).  No counterpart in the reference, whose prefix cache shares
+ * Decode paged attention for a batch whose sequences share prefixes by groups: the attention of
+ * fvb_paged_attention_decode_strided on the same tables, up to fp32's rounding and with weights held to 2^-16
+ * (bf16), 2^-22 (fp16) or in fp32, with each group's prefix read once for all its sequences (tensor cores for
+ * 16-bit types).  No counterpart in the reference, whose prefix cache shares
  * the pages but whose decode kernel reads them once per sequence and query head.
  * Group g is sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int32, num_groups + 1 ascending entries within
  * [0, num_seqs]; sequences outside every group share nothing).  The caller says that the table rows of a
  * group agree in their first prefix_lens[g] / 16 pages; those pages are read through the row of the group's
- * first sequence, whatever its kv_len, or, by calls too small to gain from sharing, through each one's own.  prefix_lens[g] need not be a multiple of 16 nor below every
- * kv_len of the group; max_prefix_len bounds it (keys past it are read per sequence).
+ * first sequence, whatever its kv_len, or, by calls too small to gain from sharing, through each one's own.
+ * prefix_lens[g] need not be a multiple of 16 nor below every kv_len of the group; max_prefix_len bounds it
+ * (keys past it are read per sequence).  num_groups may be 0, cu_groups and prefix_lens then NULL.
  * Malformed groups are recorded in the device error word and never read out of bounds.
  * max_kv_len at most fvb_max_kv_len(); workspace 256-byte aligned.
  */
@@ -344,8 +348,9 @@ FVB_API int fvb_paged_attention_shared_prefix_decode(
  * last, in the same order.  finished (one byte per row, may be NULL): a beam with a nonzero entry has the
  * single continuation eos_token_id at scores[r], and its logits are not read.
  * num_beams and num_select 1 to 64, num_select <= num_beams * vocab, at most 1024 parts of 131072 logits a
- * request (num_beams * ceil(vocab / 131072)), rows at any element alignment.  Sums in fp32, the order of the
- * beams' candidates decided in fp64.
+ * request (num_beams * ceil(vocab / 131072)), rows at any element alignment.  Sums within 1.3e-6 of a score;
+ * where candidates of two beams are closer than 3e-6 and one of them is chosen, both beams' are taken again in
+ * fp64, which decides their order.
  * workspace: fvb_beam_search_workspace_size bytes, 256-byte aligned, no initial value.  Two launches.
  */
 FVB_API size_t fvb_beam_search_workspace_size(int num_requests, int num_beams, int64_t vocab, int num_select,

@@ -676,8 +676,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc_kernel(
           m_ref = mt;
         }
       }
-      // P = 2^((s - m_ref) * scale) <= 2^8 (raised in fp16, see kRaiseLog2), packed to 16 bits into S_i's first 64 columns
-      // (P = 0 while the row has seen no key).
+      // P = 2^((s - m_ref) * scale) <= 2^8 (window and prefix in fp16: raised, kRaiseLog2), packed to 16 bits into
+      // S_i's first 64 columns (P = 0 while the row has seen no key).
       const float ms = ((kIlv || MODE != kTcPlain) && m_ref == -INFINITY) ? 0.f : m_ref * scale;
       const float up = MODE == kTcPlain ? -ms : kRaise - ms;
       const float2 nms2 = make_float2(up, up);

@@ -16,9 +16,10 @@
 //            the SMs that the prefix kernel does not take, beside which it then runs;
 //   merge    one or four warps per (sequence, query head).
 //
-// Measured: 32 requests behind 4096 tokens, 32/8 heads x 128, own keys U[64, 1024]: 32 us (86 MB: 2.7 TB/s; every
-// sequence reading all its keys 116); 128 sequences in four groups behind 2048 to 12288 tokens 100 us (0.41 GB: 4.1
-// TB/s; 529).  Of the 100: prefixes 36, bound by the softmax of 128-row tiles, rest 58 at HBM's rate, merge 5.
+// Measured: 32 requests behind 4096 tokens, 32/8 heads x 128, own keys U[64, 1024]: 33 us (86 MB: 2.6 TB/s; every
+// sequence reading all its keys 116); 128 sequences in four groups behind 2048 to 12288 tokens 109 us (0.41 GB: 3.8
+// TB/s; 529).  Of the 109: prefixes 43, bound by the softmax of 128-row tiles and two operands of P, rest 58 at HBM's
+// rate, merge 5.
 //
 // fp32 and larger batches, four launches:
 //
@@ -396,7 +397,7 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
   // one launch of 4 to 10 us.  Which is faster goes by the pages an SM gets at most (halves of D 128 count each), and
   // by what a page costs the split-KV kernel: over 400 calls of random shapes the choice is 1 % off the better way on
   // average, and sharing always 40 %.  (70 sequences x 2 heads x 128 behind up to 182 keys, group 3: 18.0 us shared,
-  // 9.9 each for itself; 8 x 8 x 128 behind 2000, group 2: 12.6 and 20.3; 32 x 8 x 128 behind 4096, group 4: 32.4 and
+  // 9.9 each for itself; 8 x 8 x 128 behind 2000, group 2: 14.9 and 20.3; 32 x 8 x 128 behind 4096, group 4: 33.0 and
   // 116.)
   const int64_t pages = std::max<int64_t>(1, (int64_t(max_kv_len) + kPageSize - 1) / kPageSize) * (head_dim / 64);
   const int64_t direct_pages = dtype == FVB_DTYPE_F32 ? (group <= 8 ? 128 : 64)
@@ -430,11 +431,13 @@ SharedPrefixPlan plan_shared_prefix(int num_seqs, int n_heads, int n_kv_heads, i
     int64_t room = tc ? num_sms : num_sms * 6;
     if (p.keys && num_groups == 1) {
       // Both kernels hold an SM's shared memory alone, so they share the SMs out: a prefix tile (twice the work
-      // in items of two) takes about 1.45 us of an SM from L2, a tile of the sequences' own keys 1.64 us from
-      // HBM.  The contexts behind the prefix are taken for half of what max_kv_len leaves.  (8 beams: 17.2 us
-      // one kernel after the other on all SMs, 12.7 beside each other; 32 requests behind 4096 tokens: 39.6,
-      // 32.2.)  With several groups the number of prefix CTAs is not known here, and a CTA too many holds up
-      // a whole share of the rest (128 sequences in 4 groups: 100 us after each other, 113 beside).
+      // in items of two) takes about 1.5 us of an SM from L2, a tile of the sequences' own keys 1.64 us from
+      // HBM.  The contexts behind the prefix are taken for half of what max_kv_len leaves.  With one operand for P:
+      // 8 beams 17.2 us one kernel after the other on all SMs, 12.7 beside each other; 32 requests behind 4096
+      // tokens 39.6, 32.2; with two operands 14.9 and 33.0 beside each other (the same at 1.65 and 2.9 us a tile; with
+      // a max_kv_len ten times too large 22.3 and 35.3).  With several groups the number of prefix CTAs is not known
+      // here, and a CTA too many holds up a whole share of the rest (128 sequences in 4 groups, one operand: 100 us
+      // after each other, 113 beside).
       const int own = std::max(0, max_kv_len - prefix) / 2;
       const double first = double(ctas) * units * (p.single_tiles ? 1.45 : 2.5);
       const double rest = double(num_seqs) * n_kv_heads * ((group + kKeysCols - 1) / kKeysCols) *

@@ -175,7 +175,8 @@ def paged_attention_window_gemm(
 
     Pages without a key that some query of the sequence sees are not read, as in
     :func:`paged_attention_window_gemv`.  The positions of a sequence's tokens must not descend.  A query
-    whose mask leaves nothing gives zeros.
+    whose mask leaves nothing gives zeros.  As in :func:`paged_attention_gemm`, 16-bit types round each softmax
+    weight to their own precision before it meets V.
     """
     return _cuda_backend.PagedAttentionWindowGemmCuda(q, k_pool, v_pool, cu_seqlens, max_q_len, kv_page_tables, kv_lens,
                                                       positions, window, num_sinks, out_token_major)
@@ -199,7 +200,7 @@ def paged_attention_shared_prefix_gemv(
     sequences outside every group share nothing); the caller says that their table rows agree in the first
     ``prefix_lens[g] // 16`` pages (int32, ``G``), which are read once for the group, through its first
     sequence's row (calls too small to gain from that read them per sequence).  The result is that of
-    ``paged_attention_gemv`` on the same tables.
+    ``paged_attention_gemv`` on the same tables, up to rounding (softmax weights are held to 2^-16 or better).
     ``max_prefix_len`` bounds ``prefix_lens``; keys past it are read per sequence.
     """
     return _cuda_backend.PagedAttentionSharedPrefixGemvCuda(q, k_pool, v_pool, kv_page_tables, kv_lens, max_kv_len,
@@ -374,8 +375,8 @@ def beam_search_select(
 
     ``logits`` is ``(N * W, vocab)``, row ``n * W + w`` for beam ``w`` of request ``n``; ``scores``
     ``(N, W)`` float32 the beams' summed log-probabilities.  A continuation scores
-    ``scores[n, w] + log_softmax(logits)[i]``; ties go to the lowest ``w * vocab + i``, and a score that is
-    not a number (NaN or ``+inf`` logits, a row of ``-inf``) counts as ``-inf``.  ``parents`` (int64) is the
+    ``scores[n, w] + log_softmax(logits)[i]``, in the order of these scores in fp64; ties go to the lowest
+    ``w * vocab + i``, and a score that is not a number (NaN or ``+inf`` logits, a row of ``-inf``) counts as ``-inf``.  ``parents`` (int64) is the
     beam continued, ``tokens`` (int64) the token.  A beam marked in ``finished`` ``(N, W)`` bool goes on with
     ``eos_token_id`` at its own score only.  W and ``num_select`` up to 64; the first step after a
     prompt gives every beam but one a score of ``-inf``.
