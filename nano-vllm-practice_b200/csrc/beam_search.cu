@@ -26,13 +26,14 @@
 // x log2e - m (2^-24 of itself, at most 10.8 on a warp's average: 4.5e-7) and log2e's own (1.3e-8 times what the logits
 // lie below the largest on average, at most 22 nats), and an lse is off by less than 1.3e-6, a difference of two by less
 // than 2.6e-6.  Scores of different beams closer than kNearTie are therefore in doubt, where one of them is chosen, and
-// the lse of those beams is computed again in fp64 (2 of 4800 requests of 8 beams x 151936, 16 chosen), so the order does
-// not depend on rounding.  (Added up one by one, 128 equal terms alone can be off by 1.9e-6.)
+// the lse of those beams is computed again in fp64 (2 of 4800 requests of 8 beams x 151936, 16 chosen), so the order
+// does not depend on rounding.  (Added up one by one, 128 equal terms alone can be off by 1.9e-6.)
 //
 // Measured: 32 requests x 8 beams x 151936 bf16, 16 chosen (62 MB) 25 us out of L2, 28.7 us out of HBM.  Of the 25: the
 // loads alone 12.5, the exponentials 3.6 (16 a clock and SM), bound and ranking 4, finish 5 (two overlap with the next
 // part's loads).  1 x 4 x 151936: 9 us, two launches' latency.  A beam in doubt takes 40 us more in its request's CTA:
-// 32 x 8 with one such pair 120 us, 1 x 4 90 us; requests whose beams are all copies of one another, 8 of them, 420 us.
+// 32 x 8 with one such pair 115 us, 1 x 4 90 us.  One whose row is a copy of a row already summed is found by comparing
+// them, 17 us: requests of 8 beams that are all copies 187 us (420 with a sum each).
 // The first version kept sorted lists in every thread and merged them serially: 110 and 19 us.
 //
 // A finished beam has one continuation, eos at its own score, and its logits are not read.
@@ -443,11 +444,14 @@ __global__ void __launch_bounds__(kThreads) beam_partials_kernel(const BeamArgs 
 // State of one beam in the finish kernel.
 enum { kLive = 0, kDone = 1, kDead = 2 };  // has logits; one continuation; every score is -inf
 struct Beam {
-  double base;  // score of its best continuation: score + best - lse, exact whatever the logits' size
+  double base;   // score of its best continuation: score + best - lse, exact whatever the logits' size
+  double guess;  // lse - best, from the parts' sums
+  double above;  // the same from fp64, of a beam that is summed
   float best;   // its largest logit
   int kind;
   bool exact;   // base is from fp64 or the caller's score itself
   bool redo;    // base has to be computed again in fp64
+  bool summed;  // it has been
 };
 __device__ __forceinline__ bool finite(double x) { return x >= -DBL_MAX && x <= DBL_MAX; }
 
@@ -480,7 +484,7 @@ __global__ void __launch_bounds__(kFinishThreads, 1) beam_finish_kernel(const Be
     const double score = a.scores[row0 + w];
     const bool done = a.finished != nullptr && a.finished[row0 + w] != 0;
     const int kind = !finite(score) ? kDead : done ? kDone : kLive;
-    beams[w] = Beam{score, 0.f, kind, kind != kLive, false};
+    beams[w] = Beam{score, 0.0, 0.0, 0.f, kind, kind != kLive, false, false};
   }
   __syncthreads();
   const unsigned long long* lists = reinterpret_cast<const unsigned long long*>(a.keys) + row0 * per_row;
@@ -518,7 +522,8 @@ __global__ void __launch_bounds__(kFinishThreads, 1) beam_finish_kernel(const Be
       // s 2^m = sum 2^(x c), c = kLog2e in fp32; taken relative to the largest logit, so that c's own
       // rounding acts on differences of logits only.
       const double above = 0.69314718055994530942 * (log2(s) + (double(m) - double(best) * double(kLog2e)));
-      beams[w].base -= above;  // lse - best
+      beams[w].base -= above;
+      beams[w].guess = above;
       beams[w].best = best;
       // +inf or only -inf: no distribution.  Otherwise a NaN, or logits so large that x log2e left the
       // range of fp32: fp64 tells.
@@ -534,38 +539,62 @@ __global__ void __launch_bounds__(kFinishThreads, 1) beam_finish_kernel(const Be
   __syncthreads();
 
   // base of the beams that ask for it in fp64, and a new start
+  constexpr int kAhead = 8;  // loads in flight: 40 us a beam of 151936 logits, by fp64's rate (one at a time: 84)
   auto exact_bases = [&]() {
     for (int w = 0; w < W; ++w) {
       if (!beams[w].redo) continue;
       const T* p = static_cast<const T*>(a.logits) + (row0 + w) * a.row_stride;
-      const double top = double(beams[w].best);
-      double s = 0.0;
-      constexpr int kAhead = 8;  // loads in flight: 40 us a beam of 151936 logits, by fp64's rate (one at a time: 84)
+      // a beam that has been summed and may hold the same row: comparing takes less than half of the sum's time
+      int twin = 0;
+      auto alike = [&](const Beam& b) { return b.summed && b.guess == beams[w].guess && b.best == beams[w].best; };
+      while (twin < W && !alike(beams[twin])) ++twin;
+      bool same = twin < W;
+      if (same) {
+        using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+        const Bits* x = reinterpret_cast<const Bits*>(p);
+        const Bits* y =
+            reinterpret_cast<const Bits*>(static_cast<const T*>(a.logits) + (row0 + twin) * a.row_stride);
+        Bits differ = 0;
+#pragma unroll 32
+        for (int64_t i = threadIdx.x; i < a.vocab; i += kFinishThreads) differ |= x[i] ^ y[i];
+        same = __syncthreads_and(differ == 0);
+      }
+      double above = 0.0;
+      if (same) {
+        above = beams[twin].above;
+      } else {
+        const double top = double(beams[w].best);
+        double s = 0.0;
 #pragma unroll 1
-      for (int64_t i0 = threadIdx.x; i0 < a.vocab; i0 += kAhead * kFinishThreads) {
-        float x[kAhead];
+        for (int64_t i0 = threadIdx.x; i0 < a.vocab; i0 += kAhead * kFinishThreads) {
+          float x[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const int64_t i = i0 + u * kFinishThreads;
-          x[u] = i < a.vocab ? Elem<T>::to_f(p[i]) : -INFINITY;
+          for (int u = 0; u < kAhead; ++u) {
+            const int64_t i = i0 + u * kFinishThreads;
+            x[u] = i < a.vocab ? Elem<T>::to_f(p[i]) : -INFINITY;
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; u += 4) {
+            const double e0 = exp(double(x[u]) - top), e1 = exp(double(x[u + 1]) - top);
+            const double e2 = exp(double(x[u + 2]) - top), e3 = exp(double(x[u + 3]) - top);
+            s += (e0 + e1) + (e2 + e3);
+          }
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; u += 4) {
-          const double e0 = exp(double(x[u]) - top), e1 = exp(double(x[u + 1]) - top);
-          const double e2 = exp(double(x[u + 2]) - top), e3 = exp(double(x[u + 3]) - top);
-          s += (e0 + e1) + (e2 + e3);
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) red[warp] = s;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          double t = 0.0;
+          for (int k = 0; k < kFinishWarps; ++k) t += red[k];
+          above = log(t);
         }
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) red[warp] = s;
-      __syncthreads();
       if (threadIdx.x == 0) {
-        double t = 0.0;
-        for (int k = 0; k < kFinishWarps; ++k) t += red[k];
-        beams[w].base = double(a.scores[row0 + w]) - log(t);
+        beams[w].above = above;
+        beams[w].base = double(a.scores[row0 + w]) - above;
         if (!finite(beams[w].base)) beams[w].kind = kDead;
-        beams[w].exact = true;
+        beams[w].exact = beams[w].summed = true;
         beams[w].redo = false;
       }
       __syncthreads();

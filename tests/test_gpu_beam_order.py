@@ -112,3 +112,21 @@ def test_scores_by_the_sums_error(dtype, cuda_device):
     for logits in cases:
         got, want = check(logits, torch.zeros(4, 1, device=cuda_device), 8)
         assert ((got.double() - want).abs() <= 1.3e-6 + want.abs() * 2.0**-24).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_copies_among_rows_that_nearly_are(dtype, cuda_device):
+    """Twins and beams that differ from them in one small logit only, in every order: each kind by its own score."""
+    gen = torch.Generator(device=cuda_device).manual_seed(4)
+    row = (torch.randn(40001, generator=gen, device=cuda_device) * 2).clamp(min=-7.0).to(dtype)
+    kinds = torch.tensor([[0, 1, 0, 2, 1, 0], [2, 2, 1, 1, 0, 0], [1, 0, 2, 0, 2, 2], [0, 0, 0, 0, 0, 1]])
+    logits = row.repeat(24, 1)
+    for r, kind in enumerate(kinds.view(-1).tolist()):
+        logits[r, 33333] = -9.0 - kind  # the higher the kind, the less weight in the tail: it scores more
+    tokens, parents, _ = ops.beam_search_select(logits, torch.zeros(4, 6, device=cuda_device), 30)
+    value, at = torch.sort(row.double(), descending=True, stable=True)
+    assert (value[:30] > -7.0).all()
+    for n in range(4):
+        # by value, then by kind, then by beam, then by token
+        want = sorted(((-value[i].item(), -kinds[n, w].item(), w, at[i].item()) for i in range(31) for w in range(6)))[:30]
+        assert list(zip(parents[n].tolist(), tokens[n].tolist())) == [(w, i) for _, _, w, i in want]
